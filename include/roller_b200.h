@@ -320,6 +320,111 @@ int roller_b200_last_status(roller_plan* plan, uint32_t* device_status);
  * garbage collector, src/roller.py:504-505). */
 int roller_b200_gemm_destroy(roller_plan* plan);
 
+/* ---- Gated feed-forward block ------------------------------------------------------------
+ *
+ *   G = X Wg^T,  U = X Wu^T,  H = act(G) * U,  Y = H Wd^T
+ *
+ * X, Y are tokens x d_model, Wg and Wu d_ff x d_model, Wd d_model x d_ff, G, U, H tokens x d_ff, all
+ * row-major 16-bit floats of the plan's type (the layout in which a linear layer keeps its weight,
+ * outputs x inputs). Sums are kept in fp32. H and the gradients of G and U are rounded to the
+ * operand type once, because they are operands of a tensor-core product; Y, G, U and the
+ * gradients are rounded once when they are stored. Any d_model, d_ff and tokens are accepted, and any row
+ * stride that is at least the row's length; a product's operand whose base or row stride is not a
+ * multiple of 16 bytes is first copied into rows that are. */
+typedef struct roller_ffn_plan roller_ffn_plan;
+
+#define ROLLER_ACT_SILU 0      /* v / (1 + exp(-v)) */
+#define ROLLER_ACT_GELU 1      /* v (1 + erf(v / sqrt 2)) / 2 */
+#define ROLLER_ACT_GELU_TANH 2 /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+
+/* Flags for roller_b200_ffn_create. */
+#define ROLLER_FFN_TRAINING 1 /* the plan will run roller_b200_ffn_backward: adds the workspace for
+                                 the gradients of G and U (2 x max_tokens x d_ff) */
+
+/* A matrix in device memory owned by the caller: base and row stride in elements. */
+typedef struct roller_mat {
+  void* ptr;
+  long long ld;
+} roller_mat;
+
+/* Operands of one call. An output must not share memory with any other operand. */
+typedef struct roller_ffn_io {
+  int tokens;             /* 0 .. the plan's max_tokens */
+  roller_mat x, wg, wu, wd;
+  roller_mat y;           /* forward: output */
+  roller_mat g, u;        /* forward: outputs, or both null; backward: inputs */
+  roller_mat dy;          /* backward: input */
+  roller_mat dx, dwg, dwu, dwd; /* backward: outputs (overwritten, not added to) */
+} roller_ffn_io;
+
+/* Binds the block to the current device. `mode` is ROLLER_MODE_BF16 or ROLLER_MODE_F16,
+ * `activation` a ROLLER_ACT_*. Allocates the workspaces (H, partial sums, padded copies of operands
+ * whose rows are not a multiple of 16 bytes when they are contiguous). max_tokens and the widths
+ * are 1 .. 2^20. There is no counterpart in the reference, whose generated kernels have no
+ * epilogue (src/roller.py:47-68). */
+int roller_b200_ffn_create(int max_tokens, int d_model, int d_ff, int mode, int activation, int flags,
+                           roller_ffn_plan** out);
+
+/* Enqueues y (and g, u when given) on `stream`. Like roller_b200_gemm_run it only enqueues and may
+ * be captured in a CUDA graph, with one exception: the first call that passes an unaligned operand
+ * for which the plan has no padded copy yet allocates one, which a capturing stream refuses
+ * (ROLLER_ERR_UNSUPPORTED; make one such call before the capture). Launches of one plan, and
+ * replays of graphs captured from it, share its workspaces and have to be ordered on the device.
+ * There is no counterpart in the reference (src/roller.py:47-68 emits a plain matmul). */
+int roller_b200_ffn_forward(roller_ffn_plan* plan, const roller_ffn_io* io, void* stream);
+
+/* Enqueues dx, dwg, dwu and dwd for the gradient dy of y, from x, the weights and the g and u that
+ * a forward call wrote. With no tokens the weights' gradients are zero. Same conditions as the
+ * forward call; ROLLER_ERR_UNSUPPORTED without ROLLER_FFN_TRAINING. There is no counterpart in
+ * the reference (src/roller.py:47-68 has no backward pass). */
+int roller_b200_ffn_backward(roller_ffn_plan* plan, const roller_ffn_io* io, void* stream);
+
+/* Reads and clears the plan's device status word, as roller_b200_last_status does for a GEMM plan
+ * (stands in for the per-hint try/except, src/benchmark.py:43-58). Synchronises the device. */
+int roller_b200_ffn_status(roller_ffn_plan* plan, uint32_t* device_status);
+
+/* Releases the plan and its workspaces (module lifetime in the reference, src/roller.py:504-505). */
+int roller_b200_ffn_destroy(roller_ffn_plan* plan);
+
+/* ---- Orthogonalised update ---------------------------------------------------------------
+ *
+ *   X <- G / (|G| + eps), then `steps` times  X <- a X + (b X X^T + c (X X^T)^2) X
+ *
+ * the Newton-Schulz iteration that drives the singular values of each matrix of a batch towards
+ * one, as the Muon optimiser does with the update of a weight matrix. |G| is the Frobenius norm
+ * of one matrix. The products run on the shorter side of the matrix, in fp16 with fp32 sums; X
+ * itself is carried as a pair of fp16 numbers (22 bits), because whatever is rounded off it in a
+ * weak direction grows with that direction, about a-fold per step. */
+typedef struct roller_ortho_plan roller_ortho_plan;
+
+#define ROLLER_ORTHO_IN_F32 0
+#define ROLLER_ORTHO_IN_BF16 1
+#define ROLLER_ORTHO_IN_F16 2
+
+/* Binds a batch of rows x cols matrices (each 1 .. 65536, the shorter side up to 16384) to the
+ * current device and allocates the workspaces. `in_type` is a ROLLER_ORTHO_IN_*; results are bf16.
+ * steps 1 .. 32. The coefficients have to keep singular values from [0, 1] below 4 and the
+ * polynomial b s^2 + c s^4 below 32 in magnitude at every step (ROLLER_ERR_INVALID otherwise):
+ * larger ones would leave the range of the operands. There is no counterpart in the reference,
+ * which multiplies two matrices (src/roller.py:47-68). */
+int roller_b200_ortho_create(int batch, int rows, int cols, int in_type, int steps, float a, float b,
+                             float c, float eps, roller_ortho_plan** out);
+
+/* Enqueues the iteration for `batch` matrices at g (row stride ld_g, matrix stride zs_g, in
+ * elements) into out (bf16). Matrices may follow one another or be interleaved row by row; g is
+ * not changed, out must not share memory with it. Only enqueues; may be captured. Launches of one
+ * plan, and replays of graphs captured from it, have to be ordered on the device. There is no
+ * counterpart in the reference (src/roller.py:47-68). */
+int roller_b200_ortho_run(roller_ortho_plan* plan, const void* g, long long ld_g, long long zs_g,
+                          void* out, long long ld_out, long long zs_out, void* stream);
+
+/* Reads and clears the plan's device status word (stands in for the per-hint try/except,
+ * src/benchmark.py:43-58). Synchronises the device. */
+int roller_b200_ortho_status(roller_ortho_plan* plan, uint32_t* device_status);
+
+/* Releases the plan and its workspaces (module lifetime in the reference, src/roller.py:504-505). */
+int roller_b200_ortho_destroy(roller_ortho_plan* plan);
+
 /* Text for a roller_status; the Python layer raises it as the exception message that the
  * sweep prints per failed hint (src/benchmark.py:55-58). */
 const char* roller_b200_strerror(int status);

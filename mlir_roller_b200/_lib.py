@@ -37,6 +37,16 @@ DEV_TIMEOUT_FIXUP = 7
 DEV_TIMEOUT_SLOT = 8
 DEV_TIMEOUT_PEER = 9
 
+# gated feed-forward block (roller_b200_ffn_*)
+ACT_SILU = 0
+ACT_GELU = 1
+ACT_GELU_TANH = 2
+FFN_TRAINING = 1
+# orthogonalised update (roller_b200_ortho_*)
+ORTHO_IN_F32 = 0
+ORTHO_IN_BF16 = 1
+ORTHO_IN_F16 = 2
+
 OK = 0
 ERR_INVALID = -1
 ERR_UNSUPPORTED = -2
@@ -79,6 +89,17 @@ class KTile(C.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class Mat(C.Structure):
+    """roller_mat: a row-major matrix in device memory."""
+    _fields_ = [("ptr", C.c_void_p), ("ld", C.c_longlong)]
+
+
+class FfnIo(C.Structure):
+    """roller_ffn_io: the operands of one call of a feed-forward plan."""
+    _fields_ = [("tokens", C.c_int)] + [(n, Mat) for n in (
+        "x", "wg", "wu", "wd", "y", "g", "u", "dy", "dx", "dwg", "dwu", "dwd")]
+
+
 # name -> (restype, argtypes); every symbol include/roller_b200.h declares.
 SIGNATURES = {
     "roller_b200_device_info": (C.c_int, [C.c_int, C.POINTER(DevInfo)]),
@@ -114,6 +135,16 @@ SIGNATURES = {
                                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "roller_b200_last_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32)]),
     "roller_b200_gemm_destroy": (C.c_int, [C.c_void_p]),
+    "roller_b200_ffn_create": (C.c_int, [C.c_int] * 6 + [C.POINTER(C.c_void_p)]),
+    "roller_b200_ffn_forward": (C.c_int, [C.c_void_p, C.POINTER(FfnIo), C.c_void_p]),
+    "roller_b200_ffn_backward": (C.c_int, [C.c_void_p, C.POINTER(FfnIo), C.c_void_p]),
+    "roller_b200_ffn_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32)]),
+    "roller_b200_ffn_destroy": (C.c_int, [C.c_void_p]),
+    "roller_b200_ortho_create": (C.c_int, [C.c_int] * 5 + [C.c_float] * 4 + [C.POINTER(C.c_void_p)]),
+    "roller_b200_ortho_run": (C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p,
+                                        C.c_longlong, C.c_longlong, C.c_void_p]),
+    "roller_b200_ortho_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32)]),
+    "roller_b200_ortho_destroy": (C.c_int, [C.c_void_p]),
     "roller_b200_strerror": (C.c_char_p, [C.c_int]),
     "roller_b200_last_cuda_error": (C.c_char_p, []),
 }

@@ -14,8 +14,10 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libroller_b200.so"
 
-SOURCES = ["gemm_variants.cu", "gemm_variants_16.cu", "capi.cu", "noalloc.cu", "peer_flags.cu", "skinny_simt.cu"]
-HEADERS = ["ptx_sm100.cuh", "gemm_tf32_sm100.cuh", "gemm_launch.h", "gemm_variant_make.cuh"]
+SOURCES = ["gemm_variants.cu", "gemm_variants_16.cu", "capi.cu", "noalloc.cu", "peer_flags.cu", "skinny_simt.cu",
+           "fused_gemm.cu", "fused_ffn_bf16.cu", "fused_ffn_f16.cu", "fused_ortho.cu", "ffn.cu", "orthogonal.cu"]
+HEADERS = ["ptx_sm100.cuh", "gemm_tf32_sm100.cuh", "gemm_launch.h", "gemm_variant_make.cuh", "host_util.h",
+           "fused_gemm.h", "fused_gemm_sm100.cuh", "fused_variant_make.cuh", "fused_product.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

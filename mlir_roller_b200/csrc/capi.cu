@@ -7,6 +7,7 @@
 #include <new>
 
 #include "gemm_launch.h"
+#include "host_util.h"
 
 namespace {
 
@@ -136,6 +137,43 @@ void pad_rows(const void* src, long long ld_src, void* dst, long long ld_dst, in
 }
 
 }  // namespace
+
+// What the other translation units of the library share with this one (host_util.h).
+namespace rb200 {
+
+int report_cuda_error(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+
+int encode_batch16(CUtensorMap* tm, const void* base, long long cols, long long rows, long long z,
+                   long long ld, long long z_stride, int box_cols, int box_rows,
+                   CUtensorMapSwizzle swz, bool bf16) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) {
+    snprintf(g_cuda_err, sizeof(g_cuda_err), "cuTensorMapEncodeTiled entry point not found");
+    return ROLLER_ERR_CUDA;
+  }
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows),
+                        static_cast<cuuint64_t>(z)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2,
+                           static_cast<cuuint64_t>(z > 1 ? z_stride : ld) * 2};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    snprintf(g_cuda_err, sizeof(g_cuda_err), "cuTensorMapEncodeTiled failed with CUresult %d",
+             static_cast<int>(r));
+    return ROLLER_ERR_CUDA;
+  }
+  return ROLLER_OK;
+}
+
+void pad_rows16(const void* src, long long ld_src, void* dst, long long ld_dst, int rows, int cols,
+                int blocks, cudaStream_t st) {
+  pad_rows(src, ld_src, dst, ld_dst, rows, cols, 2, blocks, st);
+}
+
+}  // namespace rb200
 
 struct roller_plan;
 static int plan_configure(roller_plan* p);

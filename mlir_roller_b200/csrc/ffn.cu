@@ -1,0 +1,253 @@
+// The gated feed-forward block: plan, workspaces and the order of its products. The arithmetic is
+// in fused_gemm_sm100.cuh; the contract of the entry points in include/roller_b200.h.
+//
+//   forward    kOpGate:  h = act(x Wg^T) * (x Wu^T)        kOpDown:  y = h Wd^T
+//   backward   kOpDact:  dh = dy Wd, from which dg, du and h leave together (dh itself stays in the
+//                        accumulator, and h is made again from g and u rather than kept)
+//              kOpDw:    dWg = dg^T x and dWu = du^T x in one launch; dWd = dy^T h
+//              kOpDx:    dx = dg Wg + du Wu, one reduction over both
+#include <cstring>
+#include <new>
+
+#include "fused_product.h"
+
+using namespace rb200;
+
+namespace {
+
+constexpr int kMaxExtent = 1 << 20;
+
+enum Operand { kX = 0, kWg, kWu, kWd, kDy, kOperands };
+
+}  // namespace
+
+struct roller_ffn_plan {
+  FusedContext ctx;
+  int max_tokens, d, f;
+  int dt;                  // 1 = bf16, 2 = fp16
+  int act;
+  bool training;
+  long long ldf;           // row stride of h, dg, du
+  void* h;                 // [max_tokens, ldf]
+  void* dgu;               // [2][max_tokens, ldf]
+  void* pad[kOperands];    // copies of unaligned operands, made when one is needed
+};
+
+namespace {
+
+int rows_of(const roller_ffn_plan* p, int which) {
+  return which == kX || which == kDy ? p->max_tokens : which == kWd ? p->d : p->f;
+}
+int cols_of(const roller_ffn_plan* p, int which) { return which == kWd ? p->f : p->d; }
+
+size_t pad_bytes(const roller_ffn_plan* p, int which) {
+  return static_cast<size_t>(rows_of(p, which)) * up64(cols_of(p, which)) * 2;
+}
+
+// The operand as the tensor maps may take it: itself, or its copy with aligned rows.
+int usable(roller_ffn_plan* p, int which, const roller_mat& m, int rows, cudaStream_t st, const void** ptr,
+           long long* ld) {
+  if (aligned16(m.ptr, m.ld)) {
+    *ptr = m.ptr;
+    *ld = m.ld;
+    return ROLLER_OK;
+  }
+  const long long ldp = up64(cols_of(p, which));
+  if (!p->pad[which]) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    FUSED_CUDA(cudaStreamIsCapturing(st, &cap));
+    if (cap != cudaStreamCaptureStatusNone) return ROLLER_ERR_UNSUPPORTED;
+    if (cudaMalloc(&p->pad[which], pad_bytes(p, which)) != cudaSuccess) {
+      cudaGetLastError();
+      p->pad[which] = nullptr;
+      return ROLLER_ERR_NOMEM;
+    }
+  }
+  pad_rows16(m.ptr, m.ld, p->pad[which], ldp, rows, cols_of(p, which), p->ctx.sm_count * 8, st);
+  FUSED_CUDA(cudaGetLastError());
+  *ptr = p->pad[which];
+  *ld = ldp;
+  return ROLLER_OK;
+}
+
+bool given(const roller_mat& m, long long cols) { return m.ptr && m.ld >= cols; }
+
+int check_plan(const roller_ffn_plan* p, const roller_ffn_io* io) {
+  if (!p || !io || io->tokens < 0) return ROLLER_ERR_INVALID;
+  if (io->tokens > p->max_tokens) return ROLLER_ERR_TOO_LARGE;
+  int cur = -1;
+  if (cudaGetDevice(&cur) != cudaSuccess || cur != p->ctx.device) return ROLLER_ERR_DEVICE;
+  return ROLLER_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int roller_b200_ffn_create(int max_tokens, int d_model, int d_ff, int mode, int activation, int flags,
+                           roller_ffn_plan** out) {
+  if (!out) return ROLLER_ERR_INVALID;
+  *out = nullptr;
+  if (max_tokens < 1 || d_model < 1 || d_ff < 1 || max_tokens > kMaxExtent || d_model > kMaxExtent ||
+      d_ff > kMaxExtent)
+    return ROLLER_ERR_INVALID;
+  if (mode != ROLLER_MODE_BF16 && mode != ROLLER_MODE_F16) return ROLLER_ERR_INVALID;
+  if (activation < ROLLER_ACT_SILU || activation > ROLLER_ACT_GELU_TANH) return ROLLER_ERR_INVALID;
+  if (flags & ~ROLLER_FFN_TRAINING) return ROLLER_ERR_INVALID;
+  roller_ffn_plan* p = new (std::nothrow) roller_ffn_plan();
+  if (!p) return ROLLER_ERR_NOMEM;
+  memset(p, 0, sizeof(*p));
+  const int rc = fused_context_create(&p->ctx);
+  if (rc != ROLLER_OK) {
+    delete p;
+    return rc;
+  }
+  p->max_tokens = max_tokens;
+  p->d = d_model;
+  p->f = d_ff;
+  p->dt = mode == ROLLER_MODE_BF16 ? 1 : 2;
+  p->act = activation;
+  p->training = (flags & ROLLER_FFN_TRAINING) != 0;
+  p->ldf = up64(d_ff);
+  const size_t h_bytes = static_cast<size_t>(max_tokens) * p->ldf * 2;
+  cudaError_t e = cudaMalloc(&p->h, h_bytes);
+  if (e == cudaSuccess && p->training) e = cudaMalloc(&p->dgu, 2 * h_bytes);
+  for (int i = 0; i < kOperands && e == cudaSuccess; ++i)
+    if (cols_of(p, i) % 8 != 0 && (i != kDy || p->training)) e = cudaMalloc(&p->pad[i], pad_bytes(p, i));
+  if (e != cudaSuccess) {
+    const int failed = e == cudaErrorMemoryAllocation ? ROLLER_ERR_NOMEM : report_cuda_error(e, "ffn plan setup");
+    cudaGetLastError();
+    roller_b200_ffn_destroy(p);
+    return failed;
+  }
+  *out = p;
+  return ROLLER_OK;
+}
+
+int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* stream) {
+  FUSED_OK(check_plan(p, io));
+  const int T = io->tokens, D = p->d, F = p->f;
+  if (T == 0) return ROLLER_OK;
+  if (!given(io->x, D) || !given(io->wg, D) || !given(io->wu, D) || !given(io->wd, F) || !given(io->y, D))
+    return ROLLER_ERR_INVALID;
+  const bool save = io->g.ptr || io->u.ptr;
+  if (save && (!given(io->g, F) || !given(io->u, F))) return ROLLER_ERR_INVALID;
+  const void* outs[] = {io->y.ptr, io->g.ptr, io->u.ptr};
+  const void* all[] = {io->x.ptr, io->wg.ptr, io->wu.ptr, io->wd.ptr, io->y.ptr, io->g.ptr, io->u.ptr};
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 4 + i; ++j)
+      if (outs[i] && outs[i] == all[j]) return ROLLER_ERR_INVALID;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool bf16 = p->dt == 1;
+  const void *x, *wg, *wu, *wd;
+  long long ldx, ldg, ldu, ldd;
+  FUSED_OK(usable(p, kX, io->x, T, st, &x, &ldx));
+  FUSED_OK(usable(p, kWg, io->wg, F, st, &wg, &ldg));
+  FUSED_OK(usable(p, kWu, io->wu, F, st, &wu, &ldu));
+  FUSED_OK(usable(p, kWd, io->wd, D, st, &wd, &ldd));
+  {
+    Product g(p->ctx, kOpGate, p->dt, T, F, D, 1);
+    g.p.act = p->act;
+    FUSED_OK(g.a_k(x, D, T, 1, ldx, 0));
+    FUSED_OK(g.b_k(0, wg, D, F, 1, ldg, 0));
+    FUSED_OK(g.b_k(1, wu, D, F, 1, ldu, 0));
+    FUSED_OK(g.output(0, p->h, 1, p->ldf, 0, bf16));
+    if (save) {
+      FUSED_OK(g.output(1, io->g.ptr, 1, io->g.ld, 0, bf16));
+      FUSED_OK(g.output(2, io->u.ptr, 1, io->u.ld, 0, bf16));
+      g.p.flags |= kFusedSave;
+    }
+    FUSED_OK(g.launch(st));
+  }
+  Product d(p->ctx, kOpDown, p->dt, T, D, F, 1);
+  FUSED_OK(d.a_k(p->h, F, T, 1, p->ldf, 0));
+  FUSED_OK(d.b_k(0, wd, F, D, 1, ldd, 0));
+  FUSED_OK(d.output(0, io->y.ptr, 1, io->y.ld, 0, bf16));
+  return d.launch(st);
+}
+
+int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* stream) {
+  FUSED_OK(check_plan(p, io));
+  if (!p->training) return ROLLER_ERR_UNSUPPORTED;
+  const int T = io->tokens, D = p->d, F = p->f;
+  if (!given(io->dwg, D) || !given(io->dwu, D) || !given(io->dwd, F)) return ROLLER_ERR_INVALID;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (T == 0) {
+    FUSED_CUDA(cudaMemset2DAsync(io->dwg.ptr, io->dwg.ld * 2, 0, static_cast<size_t>(D) * 2, F, st));
+    FUSED_CUDA(cudaMemset2DAsync(io->dwu.ptr, io->dwu.ld * 2, 0, static_cast<size_t>(D) * 2, F, st));
+    FUSED_CUDA(cudaMemset2DAsync(io->dwd.ptr, io->dwd.ld * 2, 0, static_cast<size_t>(F) * 2, D, st));
+    return ROLLER_OK;
+  }
+  if (!given(io->x, D) || !given(io->wg, D) || !given(io->wu, D) || !given(io->wd, F) || !given(io->g, F) ||
+      !given(io->u, F) || !given(io->dy, D) || !given(io->dx, D))
+    return ROLLER_ERR_INVALID;
+  const void* all[] = {io->x.ptr, io->wg.ptr, io->wu.ptr, io->wd.ptr, io->g.ptr,  io->u.ptr,
+                       io->dy.ptr, io->dx.ptr, io->dwg.ptr, io->dwu.ptr, io->dwd.ptr};
+  for (int i = 7; i < 11; ++i)
+    for (int j = 0; j < i; ++j)
+      if (all[i] == all[j]) return ROLLER_ERR_INVALID;
+  const bool bf16 = p->dt == 1;
+  const void *x, *wg, *wu, *wd, *dy;
+  long long ldx, ldg, ldu, ldd, ldy;
+  FUSED_OK(usable(p, kX, io->x, T, st, &x, &ldx));
+  FUSED_OK(usable(p, kWg, io->wg, F, st, &wg, &ldg));
+  FUSED_OK(usable(p, kWu, io->wu, F, st, &wu, &ldu));
+  FUSED_OK(usable(p, kWd, io->wd, D, st, &wd, &ldd));
+  FUSED_OK(usable(p, kDy, io->dy, T, st, &dy, &ldy));
+  const long long zs = static_cast<long long>(p->max_tokens) * p->ldf;   // dg to du
+  {
+    Product a(p->ctx, kOpDact, p->dt, T, F, D, 1);
+    a.p.act = p->act;
+    FUSED_OK(a.a_k(dy, D, T, 1, ldy, 0));
+    FUSED_OK(a.b_mn(0, wd, F, D, 1, ldd, 0));
+    FUSED_OK(a.output(0, p->dgu, 1, p->ldf, 0, bf16));
+    FUSED_OK(a.output(1, static_cast<uint16_t*>(p->dgu) + zs, 1, p->ldf, 0, bf16));
+    FUSED_OK(a.output(2, p->h, 1, p->ldf, 0, bf16));
+    a.p.in[0] = io->g.ptr;
+    a.p.in[1] = io->u.ptr;
+    a.p.in_ld[0] = io->g.ld;
+    a.p.in_ld[1] = io->u.ld;
+    a.p.in_cols = F;
+    a.p.in_vec = aligned16(io->g.ptr, io->g.ld) && aligned16(io->u.ptr, io->u.ld);
+    FUSED_OK(a.launch(st));
+  }
+  {
+    Product w(p->ctx, kOpDw, p->dt, F, D, T, 2);
+    FUSED_OK(w.a_mn(p->dgu, F, T, 2, p->ldf, zs));
+    FUSED_OK(w.b_mn(0, x, D, T, 1, ldx, 0));
+    FUSED_OK(w.output(0, io->dwg.ptr, 1, io->dwg.ld, 0, bf16));
+    FUSED_OK(w.output(1, io->dwu.ptr, 1, io->dwu.ld, 0, bf16));
+    FUSED_OK(w.launch(st));
+  }
+  {
+    Product w(p->ctx, kOpDw, p->dt, D, F, T, 1);
+    FUSED_OK(w.a_mn(dy, D, T, 1, ldy, 0));
+    FUSED_OK(w.b_mn(0, p->h, F, T, 1, p->ldf, 0));
+    FUSED_OK(w.output(0, io->dwd.ptr, 1, io->dwd.ld, 0, bf16));
+    FUSED_OK(w.launch(st));
+  }
+  Product g(p->ctx, kOpDx, p->dt, T, D, F, 1);
+  FUSED_OK(g.a_k(p->dgu, F, T, 2, p->ldf, zs));
+  FUSED_OK(g.b_mn(0, wg, D, F, 1, ldg, 0));
+  FUSED_OK(g.b_mn(1, wu, D, F, 1, ldu, 0));
+  FUSED_OK(g.output(0, io->dx.ptr, 1, io->dx.ld, 0, bf16));
+  return g.launch(st);
+}
+
+int roller_b200_ffn_status(roller_ffn_plan* p, uint32_t* device_status) {
+  if (!p) return ROLLER_ERR_INVALID;
+  return fused_context_status(&p->ctx, device_status);
+}
+
+int roller_b200_ffn_destroy(roller_ffn_plan* p) {
+  if (!p) return ROLLER_OK;
+  cudaFree(p->h);
+  cudaFree(p->dgu);
+  for (void* b : p->pad) cudaFree(b);
+  fused_context_destroy(&p->ctx);
+  cudaGetLastError();
+  delete p;
+  return ROLLER_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,87 @@
+// Host-side interface of the fused 16-bit products (fused_gemm_sm100.cuh): launch parameters, the
+// table of compiled kernels, and the choice of tile and reduction split.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace rb200 {
+
+enum FusedOp : int {
+  kOpGate = 0, kOpDown, kOpDact, kOpDx, kOpDw,
+  kOpGramWide, kOpGramTall, kOpPoly, kOpUpdateWide, kOpUpdateTall,
+  kFusedOps
+};
+enum Activation : int { kActSilu = 0, kActGelu = 1, kActGeluTanh = 2 };
+template <int V>
+struct IntTag {
+  static constexpr int value = V;
+};
+
+constexpr int kFusedSave = 1;   // kOpGate: g and u are written too
+constexpr int kFusedLast = 2;   // kOpUpdate*: the result leaves as bf16, divided by the scale
+
+// Everything one launch needs. Matrices are [z][rows][columns]; leading dimensions in elements.
+struct FusedParams {
+  CUtensorMap a;        // first operand
+  CUtensorMap b[2];     // second operand (kOpGate: Wg, Wu; kOpDx: the operand of each half)
+  CUtensorMap o[3];     // outputs as store destinations, where out_tma says so
+  void* out[3];
+  long long out_ld[3];
+  long long out_zstride;
+  int out_cols;         // columns of the outputs (those beyond are not written)
+  int out_tma;          // bit o: output o leaves through o[o] (16-byte aligned base and rows)
+  const void* in[2];    // element-wise inputs of the epilogue
+  long long in_ld[2];
+  long long in_zstride;
+  int in_cols;          // columns that may be read
+  int in_vec;           // their rows are 16-byte aligned
+  float* vec;           // kOpPoly writes, kOpUpdate* reads: one value per row of q, [z][vec_ld]
+  int vec_ld;
+  int M;                // rows of D
+  int num_kb;           // k-blocks of 64 (of each half in kOpDx)
+  int a_bytes;          // bytes one TMA load of A brings (fewer rows than 128 on single CTAs)
+  int tiles_m, tiles_n, tiles_per_z, zcount;
+  int nsplit;           // parts each tile's reduction is cut into (at most its k-blocks)
+  float* ws;            // partial tiles, tiles * cta_group * nsplit * 128 * block_n floats
+  uint32_t* counters;   // one per tile and CTA of a pair; zero between launches
+  int act;
+  int flags;
+  float coef_a, coef_b, coef_c, inv_scale;
+  uint32_t* status;
+  long long spin_limit;
+};
+
+struct FusedVariant {
+  int op, cta_group, block_n, dt;   // dt: 1 = bf16, 2 = fp16
+  int threads, smem_bytes;
+  const void* func;
+  cudaError_t (*launch)(const FusedParams& p, int grid, cudaStream_t stream);
+};
+
+// The compiled kernels of one operand type (1 = bf16, 2 = fp16); fp16 also has the Newton-Schulz
+// products. nullptr where none was compiled.
+const FusedVariant* fused_variants_bf16(int* n);
+const FusedVariant* fused_variants_f16(int* n);
+const FusedVariant* fused_variants_ortho(int* n);
+const FusedVariant* fused_find(int op, int cta_group, int block_n, int dt);
+
+// A problem as the choice of a kernel sees it.
+struct FusedShape {
+  int op, dt;
+  long long M, N;       // of D (kOpGate: N = columns of one weight's product)
+  long long K;          // of one half in kOpDx
+  int zcount;
+};
+struct FusedChoice {
+  const FusedVariant* kv;
+  int tiles_m, tiles_n, tiles_per_z, num_kb, nsplit, grid;
+};
+// Workspace that every choice fits in.
+constexpr int kFusedMaxUnits = 2 * 160;                   // units of a split launch
+constexpr size_t kFusedWsBytes = static_cast<size_t>(160) * 2 * 128 * 256 * 4;
+FusedChoice fused_choose(const FusedShape& s, int sm_count, int max_pairs);
+}  // namespace rb200

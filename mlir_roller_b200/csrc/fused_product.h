@@ -1,0 +1,106 @@
+// Builds the launch of one fused product: choice of kernel, tensor maps, parameters.
+#pragma once
+
+#include <cstring>
+
+#include "../../include/roller_b200.h"
+#include "fused_gemm.h"
+#include "gemm_launch.h"
+#include "host_util.h"
+
+namespace rb200 {
+
+#define FUSED_CUDA(call)                                               \
+  do {                                                                 \
+    cudaError_t e_ = (call);                                           \
+    if (e_ != cudaSuccess) return rb200::report_cuda_error(e_, #call); \
+  } while (0)
+#define FUSED_OK(call)                \
+  do {                                \
+    int rc_ = (call);                 \
+    if (rc_ != ROLLER_OK) return rc_; \
+  } while (0)
+
+inline long long up64(long long x) { return (x + 63) / 64 * 64; }
+
+inline bool aligned16(const void* p, long long ld) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0;
+}
+
+// What the products of one plan share.
+struct FusedContext {
+  int device, sm_count, max_pairs;
+  float* ws;            // partial tiles
+  uint32_t* counters;
+  uint32_t* status;
+};
+int fused_context_create(FusedContext* c);    // on the current device; a roller_status
+void fused_context_destroy(FusedContext* c);
+int fused_context_status(FusedContext* c, uint32_t* device_status);   // reads and clears
+
+// D is M x N, reduced over K, for z matrices; operand matrices are [z][rows][cols] in memory.
+struct Product {
+  FusedParams p;
+  FusedChoice c;
+  int op;
+  bool bf16;
+
+  Product(const FusedContext& x, int op_, int dt, long long M, long long N, long long K, int z)
+      : op(op_), bf16(dt == 1) {
+    memset(&p, 0, sizeof(p));
+    c = fused_choose(FusedShape{op, dt, M, N, K, z}, x.sm_count, x.max_pairs);
+    p.M = static_cast<int>(M);
+    p.out_cols = static_cast<int>(N);
+    p.num_kb = c.num_kb;
+    p.tiles_m = c.tiles_m;
+    p.tiles_n = c.tiles_n;
+    p.tiles_per_z = c.tiles_per_z;
+    p.zcount = z;
+    p.nsplit = c.nsplit;
+    p.ws = x.ws;
+    p.counters = x.counters;
+    p.status = x.status;
+    p.spin_limit = kSpinLimitCycles;
+  }
+  // First operand, rows along k.
+  int a_k(const void* base, long long cols, long long rows, long long z, long long ld, long long zs) {
+    // with few rows a load brings only those (the accumulator's rows beyond are never looked at)
+    int box = 128;
+    if (c.kv->cta_group == 1 && rows < 128) box = static_cast<int>((rows + 7) / 8 * 8);
+    p.a_bytes = box * 128;
+    return encode_batch16(&p.a, base, cols, rows, z, ld, zs, 64, box, CU_TENSOR_MAP_SWIZZLE_128B, bf16);
+  }
+  // First operand, rows along m (its memory rows are k).
+  int a_mn(const void* base, long long cols, long long rows, long long z, long long ld, long long zs) {
+    p.a_bytes = 128 * 128;
+    return encode_batch16(&p.a, base, cols, rows, z, ld, zs, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, bf16);
+  }
+  int b_k(int i, const void* base, long long cols, long long rows, long long z, long long ld, long long zs) {
+    const int box = op == kOpGate ? c.kv->block_n / 2 : c.kv->block_n / c.kv->cta_group;
+    return encode_batch16(&p.b[i], base, cols, rows, z, ld, zs, 64, box, CU_TENSOR_MAP_SWIZZLE_128B, bf16);
+  }
+  int b_mn(int i, const void* base, long long cols, long long rows, long long z, long long ld, long long zs) {
+    return encode_batch16(&p.b[i], base, cols, rows, z, ld, zs, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, bf16);
+  }
+  int output(int i, void* base, long long z, long long ld, long long zs, bool as_bf16) {
+    p.out[i] = base;
+    p.out_ld[i] = ld;
+    p.out_zstride = zs;
+    if (!aligned16(base, ld) || (z > 1 && (zs % 8 != 0 || zs < ld * p.M))) return ROLLER_OK;
+    p.out_tma |= 1 << i;
+    // the box that one epilogue warp hands over (FusedCfg::BOX_COLS)
+    const bool narrow = op == kOpDact || (op == kOpGate && c.kv->block_n == 128);
+    return encode_batch16(&p.o[i], base, p.out_cols, p.M, z, ld, zs, narrow ? 32 : 64, 32,
+                          narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, as_bf16);
+  }
+  // The mirror image of a symmetric output (always the library's own, aligned memory).
+  int mirror(void* base, long long z, long long ld, long long zs) {
+    return encode_batch16(&p.o[1], base, p.out_cols, p.M, z, ld, zs, 32, 64, CU_TENSOR_MAP_SWIZZLE_NONE, bf16);
+  }
+  int launch(cudaStream_t st) {
+    FUSED_CUDA(c.kv->launch(p, c.grid, st));
+    return ROLLER_OK;
+  }
+};
+
+}  // namespace rb200

@@ -1,0 +1,22 @@
+// Host-side helpers defined in capi.cu and used by the other entry points' translation units.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+namespace rb200 {
+
+// Records the text behind roller_b200_last_cuda_error, clears the error, returns ROLLER_ERR_CUDA.
+int report_cuda_error(cudaError_t e, const char* what);
+
+// Tensor map of a batch of `z` row-major 16-bit matrices. base, ld and z_stride have to be
+// multiples of 16 bytes.
+int encode_batch16(CUtensorMap* tm, const void* base, long long cols, long long rows, long long z,
+                   long long ld, long long z_stride, int box_cols, int box_rows,
+                   CUtensorMapSwizzle swz, bool bf16);
+
+// Copies 16-bit rows into rows whose stride is a multiple of 16 bytes.
+void pad_rows16(const void* src, long long ld_src, void* dst, long long ld_dst, int rows, int cols,
+                int blocks, cudaStream_t st);
+
+}  // namespace rb200

@@ -1,0 +1,349 @@
+// The Newton-Schulz iteration on a batch of matrices: norm, conversion, and three products a
+// step. The products are in fused_gemm_sm100.cuh; the contract in include/roller_b200.h.
+//
+// With m the shorter side and x on that side (x x^T for a wide matrix, x^T x for a tall one):
+//     p = x x^T          m m n / 2   multiplications (one triangle of a symmetric product)
+//     q = b p + c p p    m m m / 2
+//     x = a x + q x      m m n
+// Numbers. Everything is scaled by S = 2^10, so that the entries of x (about 1 / sqrt(m n) at the
+// start, 1 / sqrt(n) at the end), p and q sit in fp16's normal range. The operands of the products
+// are fp16: 2^-12 a rounding, where bf16 would lose 2^-9. The iteration multiplies weak
+// directions by a = 3.4 a step, and with them whatever was rounded off x in those directions, so a
+// matrix of low rank would come out with 4e-2 (rank 8) to 1.5e-1 (rank 1) of noise; x is
+// therefore carried as hi + lo, two fp16 numbers, and only q x reads hi alone: there a weak
+// direction's error meets the weak direction's q, which is small. What rounding loses on q's
+// diagonal (as large as all its other roundings together, once p is near the identity) goes into
+// the fp32 factor of x. Against 64 bits: 0.3-2e-3 of |x| before the last rounding to bf16.
+#include <cmath>
+#include <new>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "fused_product.h"
+
+using namespace rb200;
+
+namespace {
+
+constexpr float kScale = 1024.0f;   // S
+constexpr int kSumBlocks = 296;     // blocks of the norm per matrix, at most
+constexpr int kMaxSide = 65536, kMaxShort = 16384, kMaxBatch = 4096;
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+
+// Eight consecutive elements of a row (those beyond the row's end are zero).
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int col, int cols, bool vec, float (&v)[8]) {
+  if (vec && col + 8 <= cols) {
+    alignas(16) T t[8];
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+      reinterpret_cast<uint4*>(t)[i] = __ldg(reinterpret_cast<const uint4*>(row + col) + i);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_float(t[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = col + j < cols ? to_float(row[col + j]) : 0.0f;
+  }
+}
+
+struct Source {
+  const void* g;
+  long long ld, zs;
+  int rows, cols;
+  int vec;     // rows and matrices start on 16 bytes
+  int tx;      // threads along a row (power of two), the other 256 / tx take further rows
+};
+
+// Sum of squares of each matrix, in fp64 (bound by the read: 8 bytes of fp64 work per element are
+// a few per cent of it), one partial sum per block.
+template <typename T>
+__global__ void __launch_bounds__(256) ortho_sumsq(Source s, double* __restrict__ part) {
+  const T* g = static_cast<const T*>(s.g) + blockIdx.y * s.zs;
+  const int x = threadIdx.x % s.tx, y = threadIdx.x / s.tx, ty = 256 / s.tx;
+  double sum = 0.0;
+  for (long long r = static_cast<long long>(blockIdx.x) * ty + y; r < s.rows; r += static_cast<long long>(gridDim.x) * ty) {
+    const T* row = g + r * s.ld;
+    for (int c = x * 8; c < s.cols; c += s.tx * 8) {
+      float v[8];
+      load8(row, c, s.cols, s.vec, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += static_cast<double>(v[j]) * static_cast<double>(v[j]);
+    }
+  }
+  __shared__ double warp_sum[8];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int i = 0; i < 8; ++i) t += warp_sum[i];
+    part[blockIdx.y * kSumBlocks + blockIdx.x] = t;
+  }
+}
+
+// x = S g / (|g| + eps) as hi + lo. Every block adds the partial sums in the same order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+ortho_scale(Source s, const double* __restrict__ part, int parts, double eps, __half* __restrict__ hi,
+            __half* __restrict__ lo, long long ldx, long long zsx) {
+  __shared__ double warp_sum[8];
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < parts; i += 256) sum += part[blockIdx.y * kSumBlocks + i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (int i = 0; i < 8; ++i) sum += warp_sum[i];
+  const float scale = static_cast<float>(static_cast<double>(kScale) / (sqrt(sum) + eps));
+
+  const T* g = static_cast<const T*>(s.g) + blockIdx.y * s.zs;
+  const int x = threadIdx.x % s.tx, y = threadIdx.x / s.tx, ty = 256 / s.tx;
+  for (long long r = static_cast<long long>(blockIdx.x) * ty + y; r < s.rows; r += static_cast<long long>(gridDim.x) * ty) {
+    const T* row = g + r * s.ld;
+    const long long at = blockIdx.y * zsx + r * ldx;
+    for (int c = x * 8; c < s.cols; c += s.tx * 8) {
+      float v[8];
+      load8(row, c, s.cols, s.vec, v);
+      alignas(16) __half h[8], l[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float f = v[j] * scale;
+        h[j] = __float2half_rn(f);
+        l[j] = __float2half_rn(f - __half2float(h[j]));
+      }
+      *reinterpret_cast<uint4*>(hi + at + c) = *reinterpret_cast<const uint4*>(h);
+      *reinterpret_cast<uint4*>(lo + at + c) = *reinterpret_cast<const uint4*>(l);
+    }
+  }
+}
+
+template <typename T>
+int convert(const Source& s, int batch, int blocks, double* part, double eps, __half* hi, __half* lo,
+            long long ldx, long long zsx, cudaStream_t st) {
+  const dim3 sums(static_cast<unsigned>(blocks < kSumBlocks ? blocks : kSumBlocks), static_cast<unsigned>(batch));
+  ortho_sumsq<T><<<sums, 256, 0, st>>>(s, part);
+  FUSED_CUDA(cudaGetLastError());
+  const dim3 grid(static_cast<unsigned>(blocks < 4 * kSumBlocks ? blocks : 4 * kSumBlocks), static_cast<unsigned>(batch));
+  ortho_scale<T><<<grid, 256, 0, st>>>(s, part, static_cast<int>(sums.x), eps, hi, lo, ldx, zsx);
+  FUSED_CUDA(cudaGetLastError());
+  return ROLLER_OK;
+}
+
+// The largest |s (a + b s^2 + c s^4)| for s in [0, r], and the largest |b s^2 + c s^4|.
+void polynomial_range(double a, double b, double c, double r, double* out, double* poly) {
+  *out = *poly = 0.0;
+  for (int i = 0; i <= 4096; ++i) {
+    const double s = r * i / 4096.0, q = b * s * s + c * s * s * s * s;
+    *out = fmax(*out, fabs(s * (a + q)));
+    *poly = fmax(*poly, fabs(q));
+  }
+}
+
+}  // namespace
+
+struct roller_ortho_plan {
+  FusedContext ctx;
+  int batch, rows, cols, in_type, steps;
+  int m, n;                // shorter and longer side
+  bool tall;
+  float a, b, c, eps;
+  long long ldx, zsx, ldm, zsm;
+  double* part;            // partial sums of squares
+  __half* x[2][2];         // [which][hi, lo], [batch][rows][ldx]
+  __half *pm, *qm;         // p and q, [batch][m][ldm]
+  float* vec;              // [batch][ldm]
+};
+
+extern "C" {
+
+int roller_b200_ortho_create(int batch, int rows, int cols, int in_type, int steps, float a, float b,
+                             float c, float eps, roller_ortho_plan** out) {
+  if (!out) return ROLLER_ERR_INVALID;
+  *out = nullptr;
+  if (batch < 1 || batch > kMaxBatch || rows < 1 || cols < 1 || rows > kMaxSide || cols > kMaxSide)
+    return ROLLER_ERR_INVALID;
+  if ((rows < cols ? rows : cols) > kMaxShort) return ROLLER_ERR_TOO_LARGE;
+  if (in_type < ROLLER_ORTHO_IN_F32 || in_type > ROLLER_ORTHO_IN_F16 || steps < 1 || steps > 32)
+    return ROLLER_ERR_INVALID;
+  if (!(eps >= 0.0f) || !std::isfinite(eps) || !std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c))
+    return ROLLER_ERR_INVALID;
+  double r = 1.0;
+  for (int i = 0; i < steps; ++i) {
+    double next, poly;
+    polynomial_range(a, b, c, r, &next, &poly);
+    if (!(poly < 32.0) || !(next < 4.0)) return ROLLER_ERR_INVALID;
+    r = fmax(r, next);
+  }
+  roller_ortho_plan* p = new (std::nothrow) roller_ortho_plan();
+  if (!p) return ROLLER_ERR_NOMEM;
+  memset(static_cast<void*>(p), 0, sizeof(*p));
+  const int rc = fused_context_create(&p->ctx);
+  if (rc != ROLLER_OK) {
+    delete p;
+    return rc;
+  }
+  p->batch = batch;
+  p->rows = rows;
+  p->cols = cols;
+  p->in_type = in_type;
+  p->steps = steps;
+  p->tall = rows > cols;
+  p->m = p->tall ? cols : rows;
+  p->n = p->tall ? rows : cols;
+  p->a = a;
+  p->b = b;
+  p->c = c;
+  p->eps = eps;
+  p->ldx = up64(cols);
+  p->zsx = p->ldx * rows;
+  p->ldm = up64(p->m);
+  p->zsm = p->ldm * p->m;
+  cudaError_t e = cudaMalloc(&p->part, sizeof(double) * kSumBlocks * batch);
+  for (int i = 0; i < 4 && e == cudaSuccess; ++i)
+    e = cudaMalloc(&p->x[i / 2][i % 2], sizeof(__half) * p->zsx * batch);
+  if (e == cudaSuccess) e = cudaMalloc(&p->pm, sizeof(__half) * p->zsm * batch);
+  if (e == cudaSuccess) e = cudaMalloc(&p->qm, sizeof(__half) * p->zsm * batch);
+  if (e == cudaSuccess) e = cudaMalloc(&p->vec, sizeof(float) * p->ldm * batch);
+  if (e != cudaSuccess) {
+    const int failed = e == cudaErrorMemoryAllocation ? ROLLER_ERR_NOMEM : report_cuda_error(e, "ortho plan setup");
+    cudaGetLastError();
+    roller_b200_ortho_destroy(p);
+    return failed;
+  }
+  *out = p;
+  return ROLLER_OK;
+}
+
+// Whether rows of `cols` elements, `ld` apart in matrices `zs` apart, never overlap: matrices one
+// after the other, or interleaved row by row.
+static bool strides_ok(long long batch, long long rows, long long cols, long long ld, long long zs) {
+  if (rows == 1) return batch == 1 || zs >= cols;
+  if (ld < cols) return false;
+  if (batch == 1) return true;
+  return zs >= ld * (rows - 1) + cols || (zs >= cols && ld >= zs * (batch - 1) + cols);
+}
+
+int roller_b200_ortho_run(roller_ortho_plan* p, const void* g, long long ld_g, long long zs_g, void* out,
+                          long long ld_out, long long zs_out, void* stream) {
+  if (!p || !g || !out || g == out) return ROLLER_ERR_INVALID;
+  int cur = -1;
+  if (cudaGetDevice(&cur) != cudaSuccess || cur != p->ctx.device) return ROLLER_ERR_DEVICE;
+  if (p->rows == 1) ld_g = ld_out = up64(p->cols);   // there is no second row to step to
+  if (!strides_ok(p->batch, p->rows, p->cols, ld_g, zs_g) || !strides_ok(p->batch, p->rows, p->cols, ld_out, zs_out))
+    return ROLLER_ERR_INVALID;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Source s;
+  s.g = g;
+  s.ld = ld_g;
+  s.zs = zs_g;
+  s.rows = p->rows;
+  s.cols = p->cols;
+  const int per16 = p->in_type == ROLLER_ORTHO_IN_F32 ? 4 : 8;
+  s.vec = (reinterpret_cast<uintptr_t>(g) & 15) == 0 && ld_g % per16 == 0 && (p->batch == 1 || zs_g % per16 == 0);
+  s.tx = 1;
+  while (s.tx < 256 && s.tx * 8 < p->cols) s.tx *= 2;
+  const int ty = 256 / s.tx;
+  const int blocks = (p->rows + ty - 1) / ty;
+  if (p->in_type == ROLLER_ORTHO_IN_F32)
+    FUSED_OK(convert<float>(s, p->batch, blocks, p->part, p->eps, p->x[0][0], p->x[0][1], p->ldx, p->zsx, st));
+  else if (p->in_type == ROLLER_ORTHO_IN_BF16)
+    FUSED_OK(convert<__nv_bfloat16>(s, p->batch, blocks, p->part, p->eps, p->x[0][0], p->x[0][1], p->ldx, p->zsx, st));
+  else
+    FUSED_OK(convert<__half>(s, p->batch, blocks, p->part, p->eps, p->x[0][0], p->x[0][1], p->ldx, p->zsx, st));
+
+  const int R = p->rows, C = p->cols, Z = p->batch, m = p->m, n = p->n;
+  for (int i = 0; i < p->steps; ++i) {
+    __half *hi = p->x[i & 1][0], *lo = p->x[i & 1][1];
+    {
+      Product q(p->ctx, p->tall ? kOpGramTall : kOpGramWide, 2, m, m, n, Z);
+      if (p->tall) {
+        FUSED_OK(q.a_mn(hi, C, R, Z, p->ldx, p->zsx));
+        FUSED_OK(q.b_mn(0, hi, C, R, Z, p->ldx, p->zsx));
+      } else {
+        FUSED_OK(q.a_k(hi, C, R, Z, p->ldx, p->zsx));
+        FUSED_OK(q.b_k(0, hi, C, R, Z, p->ldx, p->zsx));
+      }
+      FUSED_OK(q.output(0, p->pm, Z, p->ldm, p->zsm, false));
+      FUSED_OK(q.mirror(p->pm, Z, p->ldm, p->zsm));
+      q.p.inv_scale = 1.0f / kScale;
+      FUSED_OK(q.launch(st));
+    }
+    {
+      Product q(p->ctx, kOpPoly, 2, m, m, m, Z);
+      FUSED_OK(q.a_k(p->pm, m, m, Z, p->ldm, p->zsm));
+      FUSED_OK(q.b_k(0, p->pm, m, m, Z, p->ldm, p->zsm));
+      FUSED_OK(q.output(0, p->qm, Z, p->ldm, p->zsm, false));
+      FUSED_OK(q.mirror(p->qm, Z, p->ldm, p->zsm));
+      q.p.in[0] = p->pm;
+      q.p.in_ld[0] = p->ldm;
+      q.p.in_zstride = p->zsm;
+      q.p.in_cols = static_cast<int>(p->ldm);
+      q.p.in_vec = 1;
+      q.p.vec = p->vec;
+      q.p.vec_ld = static_cast<int>(p->ldm);
+      q.p.coef_a = p->a;
+      q.p.coef_b = p->b;
+      q.p.coef_c = p->c / kScale;
+      q.p.inv_scale = 1.0f / kScale;
+      FUSED_OK(q.launch(st));
+    }
+    Product u(p->ctx, p->tall ? kOpUpdateTall : kOpUpdateWide, 2, R, C, m, Z);
+    if (p->tall) {
+      FUSED_OK(u.a_k(hi, C, R, Z, p->ldx, p->zsx));
+      FUSED_OK(u.b_k(0, p->qm, m, m, Z, p->ldm, p->zsm));
+    } else {
+      FUSED_OK(u.a_k(p->qm, m, m, Z, p->ldm, p->zsm));
+      FUSED_OK(u.b_mn(0, hi, C, R, Z, p->ldx, p->zsx));
+    }
+    u.p.in[0] = hi;
+    u.p.in[1] = lo;
+    u.p.in_ld[0] = u.p.in_ld[1] = p->ldx;
+    u.p.in_zstride = p->zsx;
+    u.p.in_cols = static_cast<int>(p->ldx);
+    u.p.in_vec = 1;
+    u.p.vec = p->vec;
+    u.p.vec_ld = static_cast<int>(p->ldm);
+    u.p.inv_scale = 1.0f / kScale;
+    if (i + 1 == p->steps) {
+      u.p.flags |= kFusedLast;
+      FUSED_OK(u.output(0, out, Z, ld_out, zs_out, true));
+    } else {
+      FUSED_OK(u.output(0, p->x[~i & 1][0], Z, p->ldx, p->zsx, false));
+      FUSED_OK(u.output(1, p->x[~i & 1][1], Z, p->ldx, p->zsx, false));
+    }
+    FUSED_OK(u.launch(st));
+  }
+  return ROLLER_OK;
+}
+
+int roller_b200_ortho_status(roller_ortho_plan* p, uint32_t* device_status) {
+  if (!p) return ROLLER_ERR_INVALID;
+  return fused_context_status(&p->ctx, device_status);
+}
+
+int roller_b200_ortho_destroy(roller_ortho_plan* p) {
+  if (!p) return ROLLER_OK;
+  cudaFree(p->part);
+  for (auto& pair : p->x)
+    for (__half* b : pair) cudaFree(b);
+  cudaFree(p->pm);
+  cudaFree(p->qm);
+  cudaFree(p->vec);
+  fused_context_destroy(&p->ctx);
+  cudaGetLastError();
+  delete p;
+  return ROLLER_OK;
+}
+
+}  // extern "C"

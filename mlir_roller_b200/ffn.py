@@ -1,0 +1,148 @@
+"""The gated feed-forward block on B200: forward for serving and training, and its backward pass.
+
+    g = x Wg^T    u = x Wu^T    h = act(g) * u    y = h Wd^T
+
+x and y are [tokens, d_model], Wg and Wu [d_ff, d_model], Wd [d_model, d_ff] (a linear layer's
+weight: outputs x inputs), all bf16 or all fp16, row-major with any row stride. As with the GEMM
+plans (`_lib.GemmPlan`), a plan owns the workspaces, the caller owns operands and outputs, calls only
+enqueue on a stream, and calls of one plan have to be ordered on the device: use one plan per
+stream, and do not replay two graphs captured from one plan at the same time. Sums are kept in
+fp32. There is no CPU fallback.
+
+    plan = GatedFfnPlan(4096, d_model, d_ff, activation="silu", training=True)
+    g, u = plan.new_saved(x.shape[0])
+    plan.forward(x, wg, wu, wd, y, g, u)                        # g, u only when a backward pass follows
+    plan.backward(x, wg, wu, wd, g, u, dy, dx, dwg, dwu, dwd)   # gradients are overwritten
+
+The reference has no counterpart: its generated kernels compute one matrix product with no
+epilogue (src/roller.py:47-68).
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _lib
+
+ACTIVATIONS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
+
+
+def check_matrix(t, name: str, dtype, device, rows: int, cols: int) -> int:
+    """Row stride of a 2-D tensor after checking its type, device, shape and order."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name} is {t.dtype}, this plan needs {dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, this plan is bound to {device}")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({rows}, {cols})")
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
+        raise ValueError(f"{name} needs contiguous rows, its column stride is {step}")
+    if rows < 2:        # there is no second row to step to: any stride is as good
+        return (cols + 7) // 8 * 8
+    if ld < cols:
+        raise ValueError(f"{name} has overlapping rows (row stride {ld} for {cols} columns)")
+    return ld
+
+
+class GatedFfnPlan:
+    """The block bound to widths, type, activation and device, for up to `max_tokens` tokens."""
+
+    def __init__(self, max_tokens: int, d_model: int, d_ff: int, *, dtype=None, activation: str = "silu",
+                 training: bool = False):
+        import torch
+        self._h = C.c_void_p()
+        self._lib = _lib.load()
+        dtype = torch.bfloat16 if dtype is None else dtype
+        modes = {torch.bfloat16: _lib.MODE_BF16, torch.float16: _lib.MODE_F16}
+        if dtype not in modes:
+            raise TypeError(f"the block exists for bf16 and fp16 operands, not {dtype}")
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation {activation!r} is not one of {sorted(ACTIVATIONS)}")
+        self.max_tokens, self.d_model, self.d_ff = max_tokens, d_model, d_ff
+        self.dtype, self.activation, self.training = dtype, activation, training
+        _lib.check(self._lib.roller_b200_ffn_create(max_tokens, d_model, d_ff, modes[dtype],
+                                                    ACTIVATIONS[activation],
+                                                    _lib.FFN_TRAINING if training else 0, C.byref(self._h)),
+                   "roller_b200_ffn_create")
+        self.device = torch.device("cuda", torch.cuda.current_device())
+        self._io = _lib.FfnIo()
+
+    def new_saved(self, tokens: int):
+        """Two tensors for g and u, with rows that start on 16 bytes (the fast layout for odd d_ff)."""
+        import torch
+        ld = (self.d_ff + 7) // 8 * 8
+        return tuple(torch.empty(tokens, ld, dtype=self.dtype, device=self.device)[:, :self.d_ff]
+                     for _ in range(2))
+
+    def _set(self, t, name: str, rows: int, cols: int) -> None:
+        m = getattr(self._io, name)
+        if t is None:
+            m.ptr, m.ld = None, 0
+            return
+        m.ld = check_matrix(t, name, self.dtype, self.device, rows, cols)
+        m.ptr = t.data_ptr()
+
+    def _call(self, fn, name: str, stream) -> None:
+        import torch
+        if not self._h:
+            raise RuntimeError("the plan has been destroyed")
+        with torch.cuda.device(self.device):
+            if stream is None:
+                stream = torch.cuda.current_stream()
+            _lib.check(fn(self._h, C.byref(self._io), C.c_void_p(getattr(stream, "cuda_stream", stream))), name)
+
+    def _operands(self, x, wg, wu, wd) -> int:
+        tokens = x.shape[0]
+        if tokens > self.max_tokens:
+            raise _lib.RollerError(_lib.ERR_TOO_LARGE, f"{tokens} tokens, the plan was made for {self.max_tokens}")
+        d, f = self.d_model, self.d_ff
+        self._io.tokens = tokens
+        self._set(x, "x", tokens, d)
+        self._set(wg, "wg", f, d)
+        self._set(wu, "wu", f, d)
+        self._set(wd, "wd", d, f)
+        return tokens
+
+    def forward(self, x, wg, wu, wd, y, g=None, u=None, stream=None) -> None:
+        """Writes y, and g and u when they are given (both or neither)."""
+        if (g is None) != (u is None):
+            raise ValueError("g and u are written together: give both or neither")
+        tokens = self._operands(x, wg, wu, wd)
+        self._set(y, "y", tokens, self.d_model)
+        self._set(g, "g", tokens, self.d_ff)
+        self._set(u, "u", tokens, self.d_ff)
+        self._call(self._lib.roller_b200_ffn_forward, "roller_b200_ffn_forward", stream)
+
+    def backward(self, x, wg, wu, wd, g, u, dy, dx, dwg, dwu, dwd, stream=None) -> None:
+        """Writes dx, dwg, dwu and dwd (not added to) for the gradient dy of y. g and u are what
+        `forward` wrote for the same x and weights. The plan has to be made with training=True."""
+        d, f = self.d_model, self.d_ff
+        tokens = self._operands(x, wg, wu, wd)
+        self._set(g, "g", tokens, f)
+        self._set(u, "u", tokens, f)
+        self._set(dy, "dy", tokens, d)
+        self._set(dx, "dx", tokens, d)
+        self._set(dwg, "dwg", f, d)
+        self._set(dwu, "dwu", f, d)
+        self._set(dwd, "dwd", d, f)
+        self._call(self._lib.roller_b200_ffn_backward, "roller_b200_ffn_backward", stream)
+
+    def check_status(self) -> None:
+        """Raises RollerError(TIMEOUT) if a launch since the last check gave up on a device-side
+        wait. Synchronises the device."""
+        st = C.c_uint32()
+        rc = self._lib.roller_b200_ffn_status(self._h, C.byref(st))
+        if rc == _lib.ERR_TIMEOUT:
+            raise _lib.RollerError(rc, f"device status word = {st.value}")
+        _lib.check(rc, "roller_b200_ffn_status")
+
+    def destroy(self) -> None:
+        if self._h:
+            self._lib.roller_b200_ffn_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
