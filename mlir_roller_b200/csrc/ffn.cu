@@ -63,7 +63,7 @@ int usable(roller_ffn_plan* p, int which, const roller_mat& m, int rows, cudaStr
       return ROLLER_ERR_NOMEM;
     }
   }
-  pad_rows16(m.ptr, m.ld, p->pad[which], ldp, rows, cols_of(p, which), p->ctx.sm_count * 8, st);
+  pad_rows16(m.ptr, m.ld, p->pad[which], ldp, rows, cols_of(p, which), p->ctx.dev.sm_count * 8, st);
   FUSED_CUDA(cudaGetLastError());
   *ptr = p->pad[which];
   *ld = ldp;
@@ -160,6 +160,7 @@ int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* s
     FUSED_OK(g.launch(st));
   }
   Product d(p->ctx, kOpDown, p->dt, T, D, F, 1);
+  d.p.b_early = 1;   // Wd does not come from the gate kernel
   FUSED_OK(d.a_k(p->h, F, T, 1, p->ldf, 0));
   FUSED_OK(d.b_k(0, wd, F, D, 1, ldd, 0));
   FUSED_OK(d.output(0, io->y.ptr, 1, io->y.ld, 0, bf16));
@@ -227,6 +228,7 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     FUSED_OK(w.launch(st));
   }
   Product g(p->ctx, kOpDx, p->dt, T, D, F, 1);
+  g.p.b_early = 1;   // Wg and Wu do not come from the kernel before
   FUSED_OK(g.a_k(p->dgu, F, T, 2, p->ldf, zs));
   FUSED_OK(g.b_mn(0, wg, D, F, 1, ldg, 0));
   FUSED_OK(g.b_mn(1, wu, D, F, 1, ldu, 0));

@@ -16,9 +16,9 @@ const FusedVariant* table(int i, int* n) {
 struct TileCost {
   int cta_group, block_n;
   double kb_us;    // one k-block of one tile while every SM works
-  double tile_us;  // what a tile costs besides (first accumulator's epilogue, fill)
+  double tile_us;  // fill and the last tile's epilogue
 };
-constexpr TileCost kTiles[] = {{2, 256, 0.40, 3.0}, {1, 256, 0.40, 3.0}, {1, 128, 0.24, 2.0}};
+constexpr TileCost kTiles[] = {{2, 256, 0.31, 7.0}, {1, 256, 0.36, 6.0}, {1, 128, 0.24, 5.0}};
 
 }  // namespace
 
@@ -33,40 +33,57 @@ const FusedVariant* fused_find(int op, int cta_group, int block_n, int dt) {
   return nullptr;
 }
 
-// Raises the kernels' shared-memory limits on the current device and asks how many CTA pairs it
-// can hold at once.
-static cudaError_t bind_device(int* max_pairs) {
-  *max_pairs = 0;
+// Raises the kernels' shared-memory limits on the current device and asks how many clusters of
+// their CTAs it can hold at once.
+static cudaError_t bind_device(FusedDevice* d) {
+  int largest[2] = {0, 0};
+  const void* func[2] = {nullptr, nullptr};
+  int threads = 0;
   for (int i = 0; i < 3; ++i) {
     int n = 0;
     const FusedVariant* t = table(i, &n);
     for (int j = 0; j < n; ++j) {
-      cudaError_t e = cudaFuncSetAttribute(t[j].func, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           t[j].smem_bytes);
+      const cudaError_t e = cudaFuncSetAttribute(t[j].func, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 t[j].smem_bytes);
       if (e != cudaSuccess) return e;
-      if (t[j].cta_group != 2 || *max_pairs > 0) continue;
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(148, 1, 1);
-      cfg.blockDim = dim3(static_cast<unsigned>(t[j].threads), 1, 1);
-      cfg.dynamicSmemBytes = static_cast<size_t>(t[j].smem_bytes);
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = 2;
-      attr[0].val.clusterDim.y = 1;
-      attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      e = cudaOccupancyMaxActiveClusters(max_pairs, t[j].func, &cfg);
-      if (e != cudaSuccess) return e;
+      const int pair = t[j].cta_group == 2;
+      if (t[j].smem_bytes > largest[pair]) {
+        largest[pair] = t[j].smem_bytes;
+        func[pair] = t[j].func;
+        threads = t[j].threads;
+      }
     }
   }
+  d->clusters[0] = d->sm_count;
+  for (int i = 1; i < 4; ++i) {
+    const int pair = i == 1;     // (a pair and a splitting cluster of two occupy SMs alike)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(d->sm_count >> i << i), 1, 1);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+    cfg.dynamicSmemBytes = static_cast<size_t>(largest[pair]);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << i;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&d->clusters[i], func[pair], &cfg);
+    if (e != cudaSuccess) return e;
+    if (d->clusters[i] > d->sm_count >> i) d->clusters[i] = d->sm_count >> i;
+  }
+  if (d->clusters[1] > kFusedMaxPairs) d->clusters[1] = kFusedMaxPairs;
   return cudaSuccess;
 }
 
-// The kernels have the same inner loop, so a launch takes about (k-blocks and tiles the busiest
-// worker gets) x (their costs); the smallest estimate wins. Parts of a reduction cost a trip of
-// the fp32 sums through L2 each.
-FusedChoice fused_choose(const FusedShape& s, int sm_count, int max_pairs) {
+// The kernels have the same inner loop, so a launch takes about (k-blocks the busiest worker gets)
+// x (their cost) + the fill and drain; the smallest estimate wins.
+//   * CTA pairs, whole tiles: the busiest worker gets ceil(tiles / workers) of them;
+//   * CTA pairs, the leftover tiles dealt out along k: an even share of all k-blocks, and the
+//     exchange of the pieces' sums, which hides behind whole tiles where there are any;
+//   * single CTAs, a cluster per tile: 1 / split of a tile's k-blocks per wave of clusters, and the
+//     exchange inside the cluster.
+FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
   FusedChoice best = {};
   double best_us = 0.0;
   const bool sym = s.op == kOpGramWide || s.op == kOpGramTall || s.op == kOpPoly;
@@ -82,20 +99,39 @@ FusedChoice fused_choose(const FusedShape& s, int sm_count, int max_pairs) {
     f.num_kb = static_cast<int>((s.K + 63) / 64);
     const int kbs = f.num_kb * (s.op == kOpDx ? 2 : 1);
     const long long tiles = static_cast<long long>(f.tiles_per_z) * s.zcount;
-    const int workers = c.cta_group == 2 ? max_pairs : sm_count;
-    if (workers < 1) continue;
-    for (int split = 1; split <= 32 && split <= kbs; ++split) {
-      const long long units = tiles * split;
-      if (split > 1 && (units * c.cta_group > kFusedMaxUnits || kbs / split < 4)) break;
-      const long long waves = (units + workers - 1) / workers;
-      const int part = (kbs + split - 1) / split;
-      double us = static_cast<double>(waves) * (part * c.kb_us) + c.tile_us;
-      if (split > 1) us += 2.0 + 0.6 * split;
-      if (best.kv && us >= best_us) continue;
+    auto consider = [&](int split, int sk_tiles, long long grid, double us) {
+      if (best.kv && us >= best_us) return;
       best_us = us;
       best = f;
-      best.nsplit = split;
-      best.grid = static_cast<int>(units < workers ? units : workers) * c.cta_group;
+      best.split = split;
+      best.sk_tiles = sk_tiles;
+      best.grid = static_cast<int>(grid);
+    };
+    if (c.cta_group == 2) {
+      const int workers = d.clusters[1];
+      if (workers < 1) continue;
+      const long long waves = (tiles + workers - 1) / workers;
+      consider(1, 0, 2 * (tiles < workers ? tiles : workers), waves * kbs * c.kb_us + c.tile_us);
+      const int left = static_cast<int>(tiles % workers);
+      const long long groups = (kbs + kSkGroup - 1) / kSkGroup;
+      if (left && left * groups >= workers) {
+        const long long whole = tiles / workers;
+        const double share = static_cast<double>(left * groups) / workers * kSkGroup;
+        consider(1, left, 2 * workers, (whole * kbs + share) * c.kb_us + c.tile_us + (whole ? 2.0 : 6.0));
+      }
+      continue;
+    }
+    for (int i = 0, split = 1; i < 4 && split <= kv->max_split && split <= kbs; ++i, split *= 2) {
+      const long long at_once = d.clusters[i];
+      if (at_once < 1) break;
+      const long long waves = (tiles + at_once - 1) / at_once;
+      const int part = (kbs + split - 1) / split;
+      if (split == 1) {
+        consider(1, 0, tiles < at_once ? tiles : at_once, waves * part * c.kb_us + c.tile_us);
+      } else {
+        // a cluster has one tile: from the second wave on every tile pays for its own fill and drain
+        consider(split, 0, tiles * split, waves * (part * c.kb_us + c.tile_us) + 1.5 + 0.2 * split);
+      }
     }
   }
   return best;
@@ -107,12 +143,11 @@ int fused_context_create(FusedContext* c) {
   cudaDeviceProp prop;
   FUSED_CUDA(cudaGetDeviceProperties(&prop, c->device));
   if (prop.major != 10) return ROLLER_ERR_DEVICE;
-  c->sm_count = prop.multiProcessorCount;
-  cudaError_t e = bind_device(&c->max_pairs);
-  if (c->max_pairs > c->sm_count / 2) c->max_pairs = c->sm_count / 2;
+  c->dev.sm_count = prop.multiProcessorCount;
+  cudaError_t e = bind_device(&c->dev);
   if (e == cudaSuccess) e = cudaMalloc(&c->ws, kFusedWsBytes);
-  if (e == cudaSuccess) e = cudaMalloc(&c->counters, kFusedMaxUnits * sizeof(uint32_t));
-  if (e == cudaSuccess) e = cudaMemset(c->counters, 0, kFusedMaxUnits * sizeof(uint32_t));
+  if (e == cudaSuccess) e = cudaMalloc(&c->counters, kFusedCounters * sizeof(uint32_t));
+  if (e == cudaSuccess) e = cudaMemset(c->counters, 0, kFusedCounters * sizeof(uint32_t));
   if (e == cudaSuccess) e = cudaMalloc(&c->status, sizeof(uint32_t));
   if (e == cudaSuccess) e = cudaMemset(c->status, 0, sizeof(uint32_t));
   if (e == cudaSuccess) return ROLLER_OK;
@@ -138,7 +173,7 @@ int fused_context_status(FusedContext* c, uint32_t* device_status) {
   if (h == 0) return ROLLER_OK;
   // a launch that gave up may have left a split reduction half counted
   FUSED_CUDA(cudaMemset(c->status, 0, sizeof(uint32_t)));
-  FUSED_CUDA(cudaMemset(c->counters, 0, kFusedMaxUnits * sizeof(uint32_t)));
+  FUSED_CUDA(cudaMemset(c->counters, 0, kFusedCounters * sizeof(uint32_t)));
   return ROLLER_ERR_TIMEOUT;
 }
 

@@ -21,6 +21,8 @@ struct IntTag {
   static constexpr int value = V;
 };
 
+constexpr int kSkGroup = 4;     // k-blocks that stay together when a tile is cut along k
+
 constexpr int kFusedSave = 1;   // kOpGate: g and u are written too
 constexpr int kFusedLast = 2;   // kOpUpdate*: the result leaves as bf16, divided by the scale
 
@@ -45,9 +47,11 @@ struct FusedParams {
   int num_kb;           // k-blocks of 64 (of each half in kOpDx)
   int a_bytes;          // bytes one TMA load of A brings (fewer rows than 128 on single CTAs)
   int tiles_m, tiles_n, tiles_per_z, zcount;
-  int nsplit;           // parts each tile's reduction is cut into (at most its k-blocks)
-  float* ws;            // partial tiles, tiles * cta_group * nsplit * 128 * block_n floats
-  uint32_t* counters;   // one per tile and CTA of a pair; zero between launches
+  int split;            // single CTAs: cluster size, CTAs that share a tile's k (1 = none)
+  int sk_tiles;         // CTA pairs: tiles cut along k and dealt out to all workers (0 = none)
+  float* ws;            // their sums: two slots per worker and CTA, 128 * block_n floats each
+  uint32_t* counters;   // one per such tile and CTA of a pair; zero between launches
+  int b_early;          // the second operand may be read before the previous kernel is done
   int act;
   int flags;
   float coef_a, coef_b, coef_c, inv_scale;
@@ -57,7 +61,7 @@ struct FusedParams {
 
 struct FusedVariant {
   int op, cta_group, block_n, dt;   // dt: 1 = bf16, 2 = fp16
-  int threads, smem_bytes;
+  int threads, smem_bytes, max_split;
   const void* func;
   cudaError_t (*launch)(const FusedParams& p, int grid, cudaStream_t stream);
 };
@@ -78,10 +82,15 @@ struct FusedShape {
 };
 struct FusedChoice {
   const FusedVariant* kv;
-  int tiles_m, tiles_n, tiles_per_z, num_kb, nsplit, grid;
+  int tiles_m, tiles_n, tiles_per_z, num_kb, split, sk_tiles, grid;
 };
-// Workspace that every choice fits in.
-constexpr int kFusedMaxUnits = 2 * 160;                   // units of a split launch
-constexpr size_t kFusedWsBytes = static_cast<size_t>(160) * 2 * 128 * 256 * 4;
-FusedChoice fused_choose(const FusedShape& s, int sm_count, int max_pairs);
+// What the current device holds at once: CTAs of one per SM, and clusters of 2, 4 and 8.
+struct FusedDevice {
+  int sm_count;
+  int clusters[4];     // [i]: clusters of 2^i CTAs
+};
+constexpr int kFusedMaxPairs = 80;
+constexpr int kFusedCounters = 2 * kFusedMaxPairs;
+constexpr size_t kFusedWsBytes = static_cast<size_t>(kFusedMaxPairs) * 2 * 2 * 128 * 256 * 4;
+FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d);
 }  // namespace rb200

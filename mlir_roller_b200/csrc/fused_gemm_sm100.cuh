@@ -19,14 +19,25 @@
 // operands may be contiguous along k or along m / n, maps are 3-D (a batch of matrices, the two
 // halves [dg du]), the reduction may run over two pairs of matrices (kOpDx), a tile's columns
 // may come from two matrices (kOpGate: each half of the tile from one weight, so the thread
-// that holds g[i,j] also holds u[i,j] and neither reaches memory unless it is asked for), only one
-// triangle of a symmetric product is computed, and a tile's reduction may be cut into `nsplit`
-// parts.
+// that holds g[i,j] also holds u[i,j] and neither reaches memory unless it is asked for), and only
+// one triangle of a symmetric product is computed.
 //
-// Split reductions: with few rows there are few tiles, and a weight has to be streamed by all SMs
-// to come at the memory's rate. Each part leaves its fp32 sums in a workspace and counts itself
-// in; the part that arrives last adds all of them in the parts' order (so the result does not
-// depend on who was last) and runs the epilogue. Nobody waits for anybody.
+// Reductions are cut in two ways, neither of which makes a CTA wait for one that may not run:
+//   * single CTAs (few rows or columns, hence few tiles, and a weight that has to be streamed by
+//     all SMs to come at the memory's rate): a cluster of 2, 4 or 8 CTAs shares one tile, each
+//     takes a part of k, and at the end each collects the others' sums of its share of the
+//     columns through distributed shared memory (the ring's, which is free by then);
+//   * CTA pairs: the tiles that do not fill a last wave (sk_tiles of them) are dealt out along k in
+//     equal runs to all workers, before the whole tiles. Each piece leaves its fp32 sums in a
+//     workspace and counts itself in; the one that arrives last adds all of them and runs the
+//     epilogue. Nobody waits for anybody.
+// Both add the parts in the order of k, so results do not depend on timing.
+//
+// A launch may be scheduled while the previous one of its stream still runs (programmatic
+// dependent launch). It touches memory only behind griddepcontrol.wait, with one exception
+// (p.b_early): weights may be fetched before, when the previous kernel is one of this library
+// that does not write them. That is safe because a kernel here lets its successor start only
+// after its own wait has returned, so everything before the previous kernel is complete.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -50,14 +61,15 @@ struct FusedCfg {
   static constexpr bool UPDATE = (OP == kOpUpdateWide || OP == kOpUpdateTall);
   static constexpr int A_BYTES = BM * 128, B_BYTES = BNL * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  // columns of D one epilogue warp owns, and columns of one box it hands to the TMA unit
+  // columns of the result one epilogue warp owns; they leave in boxes of 32 rows x 32 columns
   static constexpr int OUT_COLS = (OP == kOpGate ? BN / 4 : BN / 2);
-  static constexpr int BOX_COLS = (OP == kOpDact || OUT_COLS < 64) ? 32 : 64;
-  static constexpr int BOX_BYTES = BOX_COLS * 2 * 32;
-  static constexpr int SET_BOXES = OP == kOpDact ? 3 : (SYM || UPDATE) ? 2 : 1;
-  static constexpr int SET_BYTES = SET_BOXES * BOX_BYTES;
+  static constexpr int INPUTS = (OP == kOpDact || UPDATE) ? 2 : OP == kOpPoly ? 1 : 0;
+  static constexpr int BOX_BYTES = 32 * 64;
   static constexpr int EPI_WARPS = 8;
-  static constexpr int STAGING_BYTES = EPI_WARPS * SET_BYTES;
+  // boxes a warp has under way at once: two beside a ring of six stages, four where an epilogue
+  // writes several matrices (five stages)
+  static constexpr int RING = (CG == 1 && BN == 256) || OP == kOpDown || OP == kOpDx || OP == kOpDw ? 2 : 4;
+  static constexpr int STAGING_BYTES = EPI_WARPS * RING * BOX_BYTES;
   static constexpr int CTRL_BYTES = 256;
   static constexpr int SMEM_LIMIT = 232448;      // 227 KiB opt-in maximum per CTA
   static constexpr int STAGES_FIT = (SMEM_LIMIT - 1024 - CTRL_BYTES - STAGING_BYTES) / STAGE_BYTES;
@@ -68,6 +80,9 @@ struct FusedCfg {
   static constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
   static_assert(BN == 256 || BN == 128, "tile widths");
   static_assert(!SYM || TILE_M == BN, "one triangle of square tiles");
+  // a cluster's exchange of partial sums: at most 128 rows x BN columns, in the ring's memory
+  static constexpr int MAX_SPLIT = CG == 2 ? 1 : (OP == kOpGate ? BN / 64 : BN / 32);
+  static_assert(CG == 2 || STAGES * STAGE_BYTES >= 128 * BN * 4, "exchange area");
   static_assert(STAGES >= 3 && SMEM_BYTES <= SMEM_LIMIT, "shared memory");
 };
 
@@ -154,6 +169,62 @@ __device__ __forceinline__ FusedTile fused_tile(int t, int tiles_m, int tiles_n,
   return c;
 }
 
+// One piece of work: k-blocks [kb0, kb1) of a tile.
+struct FusedPiece {
+  int tile, kb0, kb1;
+  bool whole;
+};
+
+// The pieces of one worker. The first `sk_tiles` tiles are cut into groups of kSkGroup k-blocks, dealt
+// out evenly; the other tiles follow whole, round-robin. (A run spans at most two tiles: there
+// are fewer sk_tiles than workers.)
+struct FusedWalk {
+  int tiles, sk_tiles, total_kb, groups, workers, worker;
+  int g, g_end, next_tile;
+  __device__ FusedWalk(const FusedParams& p, int total_kb_, int workers_, int worker_)
+      : tiles(p.tiles_per_z * p.zcount), sk_tiles(p.sk_tiles), total_kb(total_kb_),
+        groups((total_kb_ + kSkGroup - 1) / kSkGroup), workers(workers_), worker(worker_) {
+    g = sk_tiles ? begin(worker) : 0;
+    g_end = sk_tiles ? begin(worker + 1) : 0;
+    next_tile = sk_tiles + worker;
+  }
+  __device__ int begin(int w) const {
+    return static_cast<int>(static_cast<long long>(sk_tiles) * groups * w / workers);
+  }
+  __device__ bool next(FusedPiece& s) {
+    if (g < g_end) {
+      s.tile = g / groups;
+      const int t0 = s.tile * groups;
+      const int e = min(g_end, t0 + groups);
+      s.kb0 = (g - t0) * kSkGroup;
+      s.kb1 = min((e - t0) * kSkGroup, total_kb);
+      s.whole = (g == t0 && e == t0 + groups);
+      g = e;
+      return true;
+    }
+    if (next_tile >= tiles) return false;
+    s.tile = next_tile;
+    s.kb0 = 0;
+    s.kb1 = total_kb;
+    s.whole = true;
+    next_tile += workers;
+    return true;
+  }
+  // The workers [first, last] that hold pieces of sk tile `t`.
+  __device__ void holders(int t, int& first, int& last) const {
+    const long long all = static_cast<long long>(sk_tiles) * groups;
+    const int g0 = t * groups, g1 = g0 + groups;
+    first = static_cast<int>(static_cast<long long>(g0) * workers / all);
+    while (first > 0 && begin(first) > g0) --first;
+    while (begin(first + 1) <= g0) ++first;
+    last = static_cast<int>(static_cast<long long>(g1 - 1) * workers / all);
+    while (begin(last) >= g1) --last;
+    while (begin(last + 1) < g1) ++last;
+  }
+  // A worker's pieces have a slot each: 0 for the tile its run begins in, 1 for the next.
+  __device__ int slot(int w, int t) const { return 2 * w + (begin(w) / groups == t ? 0 : 1); }
+};
+
 // Loads `ROWS` m/n values x 64 k of an operand at (row0, k0, z) into shared memory.
 template <int ROWS, bool MN, bool PAIR>
 __device__ __forceinline__ void fused_load(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int row0,
@@ -190,12 +261,15 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   auto tmem_empty_bar = [&](int a) { return ctrl + 144u + 8u * a; };
   const uint32_t mma_done_bar = ctrl + 160u;
   const uint32_t tmem_slot = ctrl + 176u;
-  const uint32_t last_slot = ctrl + 180u;   // outcome of the count of a split reduction
+  const uint32_t last_slot = ctrl + 180u;   // whether this CTA's piece was the tile's last
   const WaitCtx wc{p.status, p.spin_limit};
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t cta_rank = (CG == 2) ? cluster_ctarank() : 0u;
+  // a cluster is either a CTA pair (one tile of 256 rows) or `split` CTAs sharing one tile's k
+  const int split = CG == 2 ? 1 : p.split;
+  const uint32_t cluster_rank = (CG == 2 || split > 1) ? cluster_ctarank() : 0u;
+  const uint32_t cta_rank = CG == 2 ? cluster_rank : 0u;
   const bool is_leader = (cta_rank == 0);
 
   if (threadIdx.x == 0) {
@@ -215,65 +289,102 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     tma_prefetch_desc(&p.a);
     tma_prefetch_desc(&p.b[0]);
     if (OP == kOpGate || OP == kOpDx) tma_prefetch_desc(&p.b[1]);
+    tma_prefetch_desc(&p.o[0]);
   }
-  grid_launch_dependents();
   tcgen05_fence_before_sync();
   if constexpr (CG == 2) cluster_sync(); else __syncthreads();
   tcgen05_fence_after_sync();
-  grid_dependency_wait();   // everything below touches memory that the previous kernel may have
 
   uint32_t tmem_base;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
 
-  const int workers = static_cast<int>(gridDim.x) / CG;
-  const int worker = static_cast<int>(blockIdx.x) / CG;
   const int per_z = p.tiles_per_z;
-  const int units = per_z * p.zcount * p.nsplit;
   const int total_kb = p.num_kb * (OP == kOpDx ? 2 : 1);
+  const int per_worker = CG == 2 ? 2 : split;
+  FusedWalk walk(p, total_kb, static_cast<int>(gridDim.x) / per_worker, static_cast<int>(blockIdx.x) / per_worker);
+  // the part of each tile's k that this CTA of a splitting cluster takes (the cluster then has
+  // exactly one tile)
+  const int part_kb0 = static_cast<int>(static_cast<long long>(total_kb) * cluster_rank / split);
+  const int part_kb1 = static_cast<int>(static_cast<long long>(total_kb) * (cluster_rank + 1) / split);
+  auto next_piece = [&](FusedPiece& s) {
+    if (!walk.next(s)) return false;
+    if (split > 1) {
+      s.kb0 = part_kb0;
+      s.kb1 = part_kb1;
+    }
+    return true;
+  };
+
+  bool epi_ok = true;
 
   if (warp == 0 && lane == 0) {
     // ---------------------------------------------------------------- TMA producer
+    auto load_a = [&](int s, uint32_t bar, const FusedTile& c, int kb) {
+      const int phase = (OP == kOpDx && kb >= p.num_kb) ? 1 : 0;
+      const int m0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM;
+      fused_load<Cfg::BM, Cfg::A_MN, CG == 2>(smem_base + s * Cfg::STAGE_BYTES, &p.a, bar, m0,
+                                              (kb - phase * p.num_kb) * Cfg::BK, OP == kOpDx ? phase : c.z);
+    };
+    auto load_b = [&](int s, uint32_t bar, const FusedTile& c, int kb) {
+      const uint32_t b_dst = smem_base + s * Cfg::STAGE_BYTES + Cfg::A_BYTES;
+      const int phase = (OP == kOpDx && kb >= p.num_kb) ? 1 : 0;
+      const int k0 = (kb - phase * p.num_kb) * Cfg::BK;
+      if constexpr (OP == kOpGate) {
+        // tile columns: BN/2 rows of Wg, then the same BN/2 rows of Wu
+        const int f0 = c.nb * (BN / 2);
+        if constexpr (CG == 2) {
+          fused_load<Cfg::BNL, false, true>(b_dst, &p.b[cta_rank], bar, f0, k0, 0);
+        } else {
+          fused_load<BN / 2, false, false>(b_dst, &p.b[0], bar, f0, k0, 0);
+          fused_load<BN / 2, false, false>(b_dst + Cfg::B_BYTES / 2, &p.b[1], bar, f0, k0, 0);
+        }
+      } else {
+        const int bz = (OP == kOpDw || OP == kOpDx) ? 0 : c.z;
+        const int n0 = c.nb * BN + static_cast<int>(cta_rank) * Cfg::BNL;
+        fused_load<Cfg::BNL, Cfg::B_MN, CG == 2>(b_dst, &p.b[phase], bar, n0, k0, bz);
+      }
+    };
+    // The barrier counts the bytes of both operands (for a pair: of both CTAs, on the leader's,
+    // which alone arms it).
+    auto arm = [&](int s) {
+      if constexpr (CG == 2) {
+        if (is_leader) mbar_expect_tx(full_bar(s), 2 * (Cfg::A_BYTES + Cfg::B_BYTES));
+        return map_to_cta(full_bar(s), 0);
+      } else {
+        mbar_expect_tx(full_bar(s), p.a_bytes + Cfg::B_BYTES);
+        return full_bar(s);
+      }
+    };
     int s = 0;
     uint32_t ph = 0;
-    bool ok = true;
-    for (int u = worker; ok && u < units; u += workers) {
-      const int t = u / p.nsplit, part = u - t * p.nsplit;
-      const FusedTile c = fused_tile<Cfg::SYM>(t, p.tiles_m, p.tiles_n, per_z);
-      const int kb0 = static_cast<int>(static_cast<long long>(total_kb) * part / p.nsplit);
-      const int kb1 = static_cast<int>(static_cast<long long>(total_kb) * (part + 1) / p.nsplit);
-      const int m0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM;
-      for (int kb = kb0; kb < kb1; ++kb) {
+    bool ok = true, first = true;
+    FusedPiece w;
+    while (ok && next_piece(w)) {
+      const FusedTile c = fused_tile<Cfg::SYM>(w.tile, p.tiles_m, p.tiles_n, per_z);
+      int kb = w.kb0;
+      if (first) {
+        first = false;
+        const int early = p.b_early ? min(STAGES, w.kb1 - w.kb0) : 0;
+        for (int i = 0; i < early; ++i) load_b(i, arm(i), c, kb + i);
+        grid_dependency_wait();
+        grid_launch_dependents();
+        for (int i = 0; i < early; ++i)
+          load_a(i, CG == 2 ? map_to_cta(full_bar(i), 0) : full_bar(i), c, kb + i);
+        kb += early;
+        s = early;
+        if (s == STAGES) { s = 0; ph ^= 1u; }
+      }
+      for (; kb < w.kb1; ++kb) {
         if (!mbar_wait(empty_bar(s), ph ^ 1u, wc, kDevTimeoutEmpty)) { ok = false; break; }
-        const uint32_t a_dst = smem_base + s * Cfg::STAGE_BYTES;
-        const uint32_t b_dst = a_dst + Cfg::A_BYTES;
-        uint32_t bar = full_bar(s);
-        if constexpr (CG == 2) {
-          // the leader's barrier counts the bytes of both CTAs; only the leader arms it
-          if (is_leader) mbar_expect_tx(bar, 2 * (Cfg::A_BYTES + Cfg::B_BYTES));
-          bar = map_to_cta(bar, 0);
-        } else {
-          mbar_expect_tx(bar, p.a_bytes + Cfg::B_BYTES);
-        }
-        const int phase = (OP == kOpDx && kb >= p.num_kb) ? 1 : 0;
-        const int k0 = (kb - phase * p.num_kb) * Cfg::BK;
-        const int az = OP == kOpDx ? phase : c.z;
-        const int bz = (OP == kOpDw || OP == kOpDx) ? 0 : c.z;
-        fused_load<Cfg::BM, Cfg::A_MN, CG == 2>(a_dst, &p.a, bar, m0, k0, az);
-        if constexpr (OP == kOpGate) {
-          // tile columns: BN/2 rows of Wg, then the same BN/2 rows of Wu
-          const int f0 = c.nb * (BN / 2);
-          if constexpr (CG == 2) {
-            fused_load<Cfg::BNL, false, true>(b_dst, &p.b[cta_rank], bar, f0, k0, 0);
-          } else {
-            fused_load<BN / 2, false, false>(b_dst, &p.b[0], bar, f0, k0, 0);
-            fused_load<BN / 2, false, false>(b_dst + Cfg::B_BYTES / 2, &p.b[1], bar, f0, k0, 0);
-          }
-        } else {
-          const int n0 = c.nb * BN + static_cast<int>(cta_rank) * Cfg::BNL;
-          fused_load<Cfg::BNL, Cfg::B_MN, CG == 2>(b_dst, &p.b[phase], bar, n0, k0, bz);
-        }
+        const uint32_t bar = arm(s);
+        load_a(s, bar, c, kb);
+        load_b(s, bar, c, kb);
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
+    }
+    if (first) {   // (no work: a pair's grid may hold more CTAs than pieces)
+      grid_dependency_wait();
+      grid_launch_dependents();
     }
     // the MMA issuer's last releases must land in this CTA before it may exit
     for (int i = 0; i < STAGES && ok; ++i) {
@@ -287,17 +398,16 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
                                               DT == 1 ? 1u : 0u);
     // one MMA covers 16 k: 32 bytes along a k-contiguous row, or 16 rows of 128 bytes
     constexpr uint64_t a_step = Cfg::A_MN ? 128 : 2, b_step = Cfg::B_MN ? 128 : 2;
+    grid_dependency_wait();
     int s = 0, acc = 0;
     uint32_t ph = 0, acc_ph = 0;
     bool ok = true;
-    for (int u = worker; ok && u < units; u += workers) {
-      const int part = u % p.nsplit;
-      const int kb0 = static_cast<int>(static_cast<long long>(total_kb) * part / p.nsplit);
-      const int kb1 = static_cast<int>(static_cast<long long>(total_kb) * (part + 1) / p.nsplit);
+    FusedPiece w;
+    while (ok && next_piece(w)) {
       if (!mbar_wait(tmem_empty_bar(acc), acc_ph ^ 1u, wc, kDevTimeoutTmemEmpty)) break;
       tcgen05_fence_after_sync();
       const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = w.kb0; kb < w.kb1; ++kb) {
         if (!mbar_wait(full_bar(s), ph, wc, kDevTimeoutReady)) { ok = false; break; }
         tcgen05_fence_after_sync();
         const uint32_t stage = smem_base + s * Cfg::STAGE_BYTES;
@@ -305,7 +415,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
         const uint64_t b = fused_desc<Cfg::B_MN>(stage + Cfg::A_BYTES);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_f16<CG>(d_tmem, a + kk * a_step, b + kk * b_step, idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
+          umma_f16<CG>(d_tmem, a + kk * a_step, b + kk * b_step, idesc, (kb != w.kb0 || kk != 0) ? 1u : 0u);
         umma_commit<CG>(empty_bar(s));
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
@@ -316,53 +426,306 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     // whatever was issued has to complete before tensor and shared memory are given up
     umma_commit<CG>(mma_done_bar);
     mbar_wait_drain(mma_done_bar, 0u, p.spin_limit);
-  } else if (warp >= Cfg::FIRST_EPI_WARP) {
-    // ---------------------------------------------------------------- epilogue
-    const int quarter = warp & 3;                     // TMEM lanes 32 * (warp id mod 4)
-    const int half = (warp - Cfg::FIRST_EPI_WARP) >> 2;
-    const int et = static_cast<int>(threadIdx.x) - Cfg::FIRST_EPI_WARP * 32;
-    const uint32_t boxes = staging + static_cast<uint32_t>(warp - Cfg::FIRST_EPI_WARP) * Cfg::SET_BYTES;
-    const uint32_t tmem_lane = static_cast<uint32_t>(quarter * 32) << 16;
-    int acc = 0;
-    uint32_t acc_ph = 0;
-    bool ok = true;
-    for (int u = worker; ok && u < units; u += workers) {
-      const int t = u / p.nsplit, part = u - t * p.nsplit;
-      const FusedTile c = fused_tile<Cfg::SYM>(t, p.tiles_m, p.tiles_n, per_z);
-      const int row0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32;
-      const int row = row0 + lane;
-      const bool row_ok = row < p.M;
-      // a tile row of CTA rank `cta_rank` that lies wholly below the matrix has nothing to do but
-      // to hand its accumulator back
-      ok = __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(acc), acc_ph, wc, kDevTimeoutTmemFull));
-      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN) + tmem_lane;
-      bool finish = ok;
-      // ---- split reduction: leave this part's sums, count in, go on only as the last one
-      const size_t slot4 = static_cast<size_t>(32 * BN);   // float4 per CTA's partial tile
-      const float4* parts4 = nullptr;
-      if (p.nsplit > 1) {
-        if (fused_bar_any(!ok)) { ok = false; break; }
-        tcgen05_fence_after_sync();
-        float4* tile4 = reinterpret_cast<float4*>(p.ws) + (static_cast<size_t>(t) * CG + cta_rank) * p.nsplit * slot4;
-        float4* mine4 = tile4 + part * slot4 + quarter * 32 + lane;
-        for (int c32 = half * (BN / 2); c32 < (half + 1) * (BN / 2); c32 += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32(d_tmem + c32, r);
-          tmem_ld_wait();
-          if (row_ok) {
+  }
+
+  // ------------------------------------------------------------------ epilogue (warps 4 .. 11)
+  const bool epi = warp >= Cfg::FIRST_EPI_WARP;
+  const int quarter = warp & 3;                     // TMEM lanes 32 * (warp id mod 4)
+  const int half = (warp - Cfg::FIRST_EPI_WARP) >> 2;
+  const int et = static_cast<int>(threadIdx.x) - Cfg::FIRST_EPI_WARP * 32;
+  const uint32_t boxes = staging + static_cast<uint32_t>(warp - Cfg::FIRST_EPI_WARP) * (Cfg::RING * Cfg::BOX_BYTES);
+  const uint32_t tmem_lane = static_cast<uint32_t>(quarter * 32) << 16;
+  int box_at = 0;      // ring of staging boxes
+
+  auto load_d = [&](uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    tmem_ld_32x32(taddr, r);
+    tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              __stcg(mine4 + (c32 / 4 + j) * 128,
-                     make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
-                                 __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])));
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+  };
+  // 32 16-bit elements of this thread's row of epilogue input `which`
+  auto fetch = [&](int which, const FusedTile& c, int row, int col, uint4 (&raw)[4]) {
+    const uint16_t* src = static_cast<const uint16_t*>(p.in[which]) + c.z * p.in_zstride +
+                          static_cast<long long>(row) * p.in_ld[which] + col;
+    if (p.in_vec && col + 32 <= p.in_cols) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        raw[j] = row < p.M ? __ldg(reinterpret_cast<const uint4*>(src) + j) : make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = j * 8 + i * 2;
+          uint32_t lo = 0, hi = 0;
+          if (row < p.M && col + k < p.in_cols) lo = __ldg(src + k);
+          if (row < p.M && col + k + 1 < p.in_cols) hi = __ldg(src + k + 1);
+          w[i] = lo | (hi << 16);
+        }
+        raw[j] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  };
+  auto expand = [&](const uint4 (&raw)[4], float (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float2 f;
+      f = fused_unpack<DT>(raw[j].x); v[8 * j] = f.x; v[8 * j + 1] = f.y;
+      f = fused_unpack<DT>(raw[j].y); v[8 * j + 2] = f.x; v[8 * j + 3] = f.y;
+      f = fused_unpack<DT>(raw[j].z); v[8 * j + 4] = f.x; v[8 * j + 5] = f.y;
+      f = fused_unpack<DT>(raw[j].w); v[8 * j + 6] = f.x; v[8 * j + 7] = f.y;
+    }
+  };
+  // A staging box that the TMA unit has read (the one handed out RING boxes ago).
+  auto free_box = [&]() {
+    if (lane == 0) bulk_wait_read<Cfg::RING - 1>();
+    __syncwarp();
+    const uint32_t b = boxes + static_cast<uint32_t>(box_at) * Cfg::BOX_BYTES;
+    box_at = box_at + 1 == Cfg::RING ? 0 : box_at + 1;
+    return b;
+  };
+  // 32 columns of this warp's 32 rows, as 16-bit values, to columns col.. of output `o`
+  auto emit = [&](int o, const FusedTile& c, int row0, int col, const float (&v)[32], bool as_bf16) {
+    const uint32_t box = free_box();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = (as_bf16 && DT != 1) ? fused_pack<1>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1])
+                                    : fused_pack<DT>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
+      // 64-byte swizzle: 16-byte chunks of a 64-byte row, exchanged by bits 1..2 of the row
+      const int chunk = j ^ ((lane >> 1) & 3);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 64 + chunk * 16),
+                   "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                   : "memory");
+    }
+    const int oz = OP == kOpDw ? 0 : c.z;
+    if (p.out_tma & (1 << o)) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (row0 < p.M) tma_store_3d(&p.o[o], box, col, row0, oz);
+        bulk_commit_group();
+      }
+    } else {
+      // rows that start anywhere: a warp writes 32 consecutive elements per instruction
+      __syncwarp();
+      uint16_t* dst = static_cast<uint16_t*>(p.out[o]) + oz * p.out_zstride + col + lane;
+      const bool in = col + lane < p.out_cols;
+      for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
+        uint16_t x;
+        asm volatile("ld.shared.u16 %0, [%1];"
+                     : "=h"(x)
+                     : "r"(box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16) + (lane & 7) * 2)
+                     : "memory");
+        if (in) dst[static_cast<long long>(row0 + r) * p.out_ld[o]] = x;
+      }
+      if (lane == 0) bulk_commit_group();   // (an empty group keeps the ring's count)
+    }
+  };
+  // The mirror image of 32 x 32 elements of a symmetric fp16 matrix (its own box has no swizzle).
+  // Neighbouring lanes exchange halves, so that each word holds two neighbouring columns.
+  auto emit_mirror = [&](const FusedTile& c, int row0, int col, const float (&v)[32]) {
+    const uint32_t box = free_box();
+    const bool odd = lane & 1;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t ab = fused_pack<DT>(v[2 * j], v[2 * j + 1]);
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, ab, 1);
+      const uint32_t word = odd ? __byte_perm(got, ab, 0x7632) : __byte_perm(ab, got, 0x5410);
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(box + (2 * j + odd) * 64 + (lane >> 1) * 4), "r"(word) : "memory");
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (row0 < p.M) tma_store_3d(&p.o[1], box, row0, col, c.z);
+      bulk_commit_group();
+    }
+  };
+
+  // The epilogue of this warp's slabs `first`, first + step, .. < count of tile `c`. Slab i is the 32
+  // result columns from tile column 32 i on; `sums(tile_col, v)` gives 32 columns of D.
+  // `raw` holds the first slab's inputs already when `fetched`.
+  auto epilogue = [&](const FusedTile& c, int slab0, int step, int slab_end, auto sums, bool fetched,
+                      uint4 (&raw)[Cfg::INPUTS ? Cfg::INPUTS : 1][4]) {
+    const int row0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32;
+    const int row = row0 + lane;
+    const int col_base = c.nb * (OP == kOpGate ? BN / 2 : BN);
+    auto run = [&](auto act_tag) {
+      constexpr int ACT = decltype(act_tag)::value;
+#pragma unroll 1
+      for (int i = slab0; i < slab_end; i += step) {
+        const int tc = i * 32, col = col_base + tc;
+        if (col >= p.out_cols) break;     // (uniform over the warp)
+        float v[32];
+        if constexpr (Cfg::INPUTS > 0) {
+          if (!fetched) {
+#pragma unroll
+            for (int q = 0; q < Cfg::INPUTS; ++q) fetch(q, c, row, col, raw[q]);
           }
         }
+        // the next slab's inputs are on their way while this one is worked on
+        auto refill = [&]() {
+          if constexpr (Cfg::INPUTS > 0) {
+            fetched = i + step < slab_end && col + step * 32 < p.out_cols;
+            if (fetched) {
+#pragma unroll
+              for (int q = 0; q < Cfg::INPUTS; ++q) fetch(q, c, row, col + step * 32, raw[q]);
+            }
+          }
+        };
+        if constexpr (OP == kOpGate) {
+          float w[32];
+          sums(tc, v);
+          sums(tc + BN / 2, w);
+          if (p.flags & kFusedSave) {
+            emit(1, c, row0, col, v, false);
+            emit(2, c, row0, col, w, false);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float y, slope;
+            activation<ACT>(v[j], y, slope);
+            v[j] = y * w[j];
+          }
+          emit(0, c, row0, col, v, false);
+        } else if constexpr (OP == kOpDact) {
+          float g[32], w[32];
+          expand(raw[0], g);
+          expand(raw[1], w);
+          refill();
+          sums(tc, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float y, slope;
+            activation<ACT>(g[j], y, slope);
+            const float dh = v[j], uu = w[j];
+            g[j] = dh * uu * slope;    // dg
+            v[j] = dh * y;             // du
+            w[j] = y * uu;             // h
+          }
+          emit(0, c, row0, col, g, false);
+          emit(1, c, row0, col, v, false);
+          emit(2, c, row0, col, w, false);
+        } else if constexpr (OP == kOpDown || OP == kOpDx || OP == kOpDw) {
+          sums(tc, v);
+          emit(OP == kOpDw ? c.z : 0, c, row0, col, v, false);
+        } else if constexpr (Cfg::SYM) {
+          if constexpr (OP == kOpPoly) {
+            float pin[32];
+            expand(raw[0], pin);
+            refill();
+            sums(tc, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = p.coef_b * pin[j] + p.coef_c * v[j];
+            // what rounding q's diagonal to 16 bits loses is as large as the rest of that
+            // rounding together: it goes into the vector that scales x instead
+            const int dj = row - col;
+            if (row < p.M && dj >= 0 && dj < 32) {
+              float x = 0.0f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x = (j == dj) ? v[j] : x;
+              p.vec[c.z * p.vec_ld + row] = p.coef_a + (x - __half2float(__float2half_rn(x))) * p.inv_scale;
+            }
+          } else {
+            sums(tc, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
+          }
+          emit(0, c, row0, col, v, false);
+          if (c.mb != c.nb) emit_mirror(c, row0, col, v);
+        } else {
+          float hi[32], lo[32];
+          expand(raw[0], hi);
+          expand(raw[1], lo);
+          refill();
+          sums(tc, v);
+          const float dr = (OP == kOpUpdateWide && row < p.M) ? p.vec[c.z * p.vec_ld + row] : 0.0f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float dv = dr;
+            if constexpr (OP == kOpUpdateTall) dv = (col + j < p.out_cols) ? __ldg(p.vec + c.z * p.vec_ld + col + j) : 0.0f;
+            v[j] = dv * (hi[j] + lo[j]) + v[j] * p.inv_scale;
+          }
+          if (p.flags & kFusedLast) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
+            emit(0, c, row0, col, v, true);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) lo[j] = v[j] - __half2float(__float2half_rn(v[j]));
+            emit(0, c, row0, col, v, false);
+            emit(1, c, row0, col, lo, false);
+          }
+        }
+      }
+    };
+    if constexpr (OP == kOpGate || OP == kOpDact) {
+      if (p.act == kActSilu) run(IntTag<kActSilu>{});
+      else if (p.act == kActGelu) run(IntTag<kActGelu>{});
+      else run(IntTag<kActGeluTanh>{});
+    } else {
+      run(IntTag<0>{});
+    }
+  };
+
+  constexpr int kSlabs = Cfg::OUT_COLS / 32;     // slabs of one warp of a whole tile
+  uint4 raw[Cfg::INPUTS ? Cfg::INPUTS : 1][4];
+
+  if (epi && split == 1) {
+    grid_dependency_wait();
+    int acc = 0;
+    uint32_t acc_ph = 0;
+    FusedPiece w;
+    while (epi_ok && next_piece(w)) {
+      const FusedTile c = fused_tile<Cfg::SYM>(w.tile, p.tiles_m, p.tiles_n, per_z);
+      const int row = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32 + lane;
+      bool fetched = false;
+      if constexpr (Cfg::INPUTS > 0) {
+        // the first slab's inputs do not depend on the product
+        const int col = c.nb * BN + half * Cfg::OUT_COLS;
+        fetched = w.whole && col < p.out_cols;
+        if (fetched) {
+#pragma unroll
+          for (int q = 0; q < Cfg::INPUTS; ++q) fetch(q, c, row, col, raw[q]);
+        }
+      }
+      epi_ok = __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(acc), acc_ph, wc, kDevTimeoutTmemFull));
+      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN) + tmem_lane;
+      if (w.whole) {
+        if (!epi_ok) break;
+        tcgen05_fence_after_sync();
+        epilogue(c, half * kSlabs, 1, (half + 1) * kSlabs,
+                 [&](int tc, float (&v)[32]) { load_d(d_tmem + tc, v); }, fetched, raw);
+      } else if constexpr (CG == 2) {
+        // ---- a piece: leave its sums, count in, go on only as the tile's last one
+        if (fused_bar_any(!epi_ok)) { epi_ok = false; break; }
+        tcgen05_fence_after_sync();
+        constexpr size_t kSlot4 = 32 * BN;     // float4 per CTA and piece
+        float4* const ws4 = reinterpret_cast<float4*>(p.ws) + quarter * 32 + lane;
+        auto slot4 = [&](int worker) {
+          return ws4 + (static_cast<size_t>(walk.slot(worker, w.tile)) * CG + cta_rank) * kSlot4;
+        };
+        float4* const mine4 = slot4(walk.worker);
+        for (int c32 = half * (BN / 2); c32 < (half + 1) * (BN / 2); c32 += 32) {
+          float v[32];
+          load_d(d_tmem + c32, v);
+          if (row < p.M) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              __stcg(mine4 + (c32 / 4 + j) * 128, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+          }
+        }
+        int h0, h1;
+        walk.holders(w.tile, h0, h1);
         __threadfence();
         fused_bar_any(false);
         if (et == 0) {
-          uint32_t* counter = p.counters + static_cast<size_t>(t) * CG + cta_rank;
-          const uint32_t before = atomicAdd(counter, 1u);
-          const bool last = before == static_cast<uint32_t>(p.nsplit) - 1u;
+          uint32_t* counter = p.counters + w.tile * CG + cta_rank;
+          const bool last = atomicAdd(counter, 1u) == static_cast<uint32_t>(h1 - h0);
           if (last) *counter = 0;    // ready for the next launch
           asm volatile("st.shared.u32 [%0], %1;" ::"r"(last_slot), "r"(static_cast<uint32_t>(last)) : "memory");
           __threadfence();
@@ -370,269 +733,25 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
         fused_bar_any(false);
         uint32_t last;
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(last) : "r"(last_slot) : "memory");
-        finish = last != 0;
-        __threadfence();
-        parts4 = tile4 + quarter * 32 + lane;
-      }
-      if (!ok) break;
-      tcgen05_fence_after_sync();
-
-      // the 32 columns of D from tile column `col` on
-      auto slab = [&](int col, float (&v)[32]) {
-        if (p.nsplit == 1) {
-          uint32_t r[32];
-          tmem_ld_32x32(d_tmem + col, r);
-          tmem_ld_wait();
+        if (last) {
+          __threadfence();
+          epilogue(c, half * kSlabs, 1, (half + 1) * kSlabs,
+                   [&](int tc, float (&v)[32]) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-        } else {
+                     for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                     if (row >= p.M) return;
+                     for (int h = h0; h <= h1; ++h) {
+                       const float4* src = slot4(h) + (tc / 4) * 128;
+                       float4 x[8];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-          if (row_ok) {
-            for (int q = 0; q < p.nsplit; ++q) {
-              const float4* src = parts4 + q * slot4 + (col / 4) * 128;
+                       for (int j = 0; j < 8; ++j) x[j] = __ldcg(src + j * 128);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float4 x = __ldcg(src + j * 128);
-                v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
-              }
-            }
-          }
-        }
-      };
-      // 32 elements of this thread's row of an epilogue input
-      auto input = [&](int which, int col, float (&v)[32]) {
-        const uint16_t* src = static_cast<const uint16_t*>(p.in[which]) + c.z * p.in_zstride +
-                              static_cast<long long>(row) * p.in_ld[which] + col;
-        if (row_ok && p.in_vec && col + 32 <= p.in_cols) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(src) + j);
-            float2 f;
-            f = fused_unpack<DT>(w.x); v[8 * j] = f.x; v[8 * j + 1] = f.y;
-            f = fused_unpack<DT>(w.y); v[8 * j + 2] = f.x; v[8 * j + 3] = f.y;
-            f = fused_unpack<DT>(w.z); v[8 * j + 4] = f.x; v[8 * j + 5] = f.y;
-            f = fused_unpack<DT>(w.w); v[8 * j + 6] = f.x; v[8 * j + 7] = f.y;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            uint32_t w = 0;
-            if (row_ok && col + j < p.in_cols) w = __ldg(src + j);
-            v[j] = fused_unpack<DT>(w).x;
-          }
-        }
-      };
-      // 32 columns as 16-bit values into half `s` of box `b` of the staging area
-      auto put = [&](int b, int s, const float (&v)[32], bool as_bf16) {
-        const uint32_t box = boxes + b * Cfg::BOX_BYTES;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i] = (as_bf16 && DT != 1) ? fused_pack<1>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1])
-                                        : fused_pack<DT>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
-          const int chunk = Cfg::BOX_COLS == 64 ? ((s * 4 + j) ^ (lane & 7)) : (j ^ ((lane >> 1) & 3));
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                           box + lane * (Cfg::BOX_COLS * 2) + chunk * 16),
-                       "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                       : "memory");
-        }
-      };
-      // the staging boxes may be written again once the TMA unit has read them
-      auto boxes_free = [&]() {
-        if (lane == 0) bulk_wait_read_all();
-        __syncwarp();
-      };
-      auto boxes_written = [&]() {
-        fence_proxy_async_smem();
-        __syncwarp();
-      };
-      // box `b` to columns col0.. of output `o`
-      auto emit = [&](int o, int b, int col0) {
-        if (col0 >= p.out_cols || row0 >= p.M) return;
-        const uint32_t box = boxes + b * Cfg::BOX_BYTES;
-        const int oz = OP == kOpDw ? 0 : c.z;
-        if (p.out_tma & (1 << o)) {
-          if (lane == 0) tma_store_3d(&p.o[o], box, col0, row0, oz);
-        } else {
-          // rows that start anywhere: a warp writes 32 consecutive elements per instruction
-          uint16_t* dst = static_cast<uint16_t*>(p.out[o]) + oz * p.out_zstride + col0;
-          for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
-#pragma unroll
-            for (int h = 0; h < Cfg::BOX_COLS / 32; ++h) {
-              const int j = h * 32 + lane;
-              const int chunk = Cfg::BOX_COLS == 64 ? ((j >> 3) ^ (r & 7)) : ((j >> 3) ^ ((r >> 1) & 3));
-              uint16_t w;
-              asm volatile("ld.shared.u16 %0, [%1];"
-                           : "=h"(w)
-                           : "r"(box + r * (Cfg::BOX_COLS * 2) + chunk * 16 + (j & 7) * 2)
-                           : "memory");
-              if (col0 + j < p.out_cols) dst[static_cast<long long>(row0 + r) * p.out_ld[o] + j] = w;
-            }
-          }
-        }
-      };
-      auto emitted = [&]() {
-        if (lane == 0) bulk_commit_group();
-      };
-
-      if (finish) {
-        constexpr int SL = Cfg::BOX_COLS / 32;
-        const int tcol0 = half * Cfg::OUT_COLS;                   // first column in the tile
-        const int col_base = c.nb * (OP == kOpGate ? BN / 2 : BN) + tcol0;
-        if constexpr (OP == kOpGate) {
-          auto gate = [&](auto act_tag) {
-            constexpr int ACT = decltype(act_tag)::value;
-            const int outs = (p.flags & kFusedSave) ? 3 : 1;
-            for (int o = 0; o < outs; ++o) {
-#pragma unroll 1
-              for (int cc = 0; cc < Cfg::OUT_COLS; cc += Cfg::BOX_COLS) {
-                boxes_free();
-#pragma unroll 1
-                for (int s = 0; s < SL; ++s) {
-                  const int tc = tcol0 + cc + s * 32;
-                  float v[32];
-                  if (o == 2) {
-                    slab(tc + BN / 2, v);
-                  } else {
-                    slab(tc, v);
-                    if (o == 0) {
-                      float w[32];
-                      slab(tc + BN / 2, w);
-#pragma unroll
-                      for (int j = 0; j < 32; ++j) {
-                        float y, slope;
-                        activation<ACT>(v[j], y, slope);
-                        v[j] = y * w[j];
-                      }
-                    }
-                  }
-                  put(0, s, v, false);
-                }
-                boxes_written();
-                emit(o, 0, col_base + cc);
-                emitted();
-              }
-            }
-          };
-          if (p.act == kActSilu) gate(IntTag<kActSilu>{});
-          else if (p.act == kActGelu) gate(IntTag<kActGelu>{});
-          else gate(IntTag<kActGeluTanh>{});
-        } else if constexpr (OP == kOpDact) {
-          auto dact = [&](auto act_tag) {
-            constexpr int ACT = decltype(act_tag)::value;
-#pragma unroll 1
-            for (int cc = 0; cc < Cfg::OUT_COLS; cc += 32) {
-              const int col = col_base + cc;
-              if (col >= p.out_cols) break;     // (uniform over the warp)
-              float g[32], w[32], d[32];
-              input(0, col, g);
-              input(1, col, w);
-              slab(tcol0 + cc, d);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                float y, slope;
-                activation<ACT>(g[j], y, slope);
-                const float dh = d[j], uu = w[j];
-                g[j] = dh * uu * slope;    // dg
-                d[j] = dh * y;             // du
-                w[j] = y * uu;             // h
-              }
-              boxes_free();
-              put(0, 0, g, false);
-              put(1, 0, d, false);
-              put(2, 0, w, false);
-              boxes_written();
-              emit(0, 0, col);
-              emit(1, 1, col);
-              emit(2, 2, col);
-              emitted();
-            }
-          };
-          if (p.act == kActSilu) dact(IntTag<kActSilu>{});
-          else if (p.act == kActGelu) dact(IntTag<kActGelu>{});
-          else dact(IntTag<kActGeluTanh>{});
-        } else {
-#pragma unroll 1
-          for (int cc = 0; cc < Cfg::OUT_COLS; cc += 64) {
-            const int col0 = col_base + cc;
-            if (col0 >= p.out_cols) break;      // (uniform over the warp)
-            boxes_free();
-#pragma unroll 1
-            for (int s = 0; s < 2; ++s) {
-              const int col = col0 + s * 32;
-              float v[32];
-              slab(tcol0 + cc + s * 32, v);
-              if constexpr (OP == kOpDown || OP == kOpDx || OP == kOpDw) {
-                put(0, s, v, false);
-              } else if constexpr (Cfg::SYM) {
-                if constexpr (OP == kOpPoly) {
-                  float pin[32];
-                  input(0, col, pin);
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) v[j] = p.coef_b * pin[j] + p.coef_c * v[j];
-                  // what rounding q's diagonal to 16 bits loses is as large as the rest of
-                  // that rounding together: it goes into the vector that scales x instead
-                  const int dj = row - col;
-                  if (row_ok && dj >= 0 && dj < 32) {
-                    float x = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) x = (j == dj) ? v[j] : x;
-                    p.vec[c.z * p.vec_ld + row] = p.coef_a + (x - __half2float(__float2half_rn(x))) * p.inv_scale;
-                  }
-                } else {
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
-                }
-                put(0, s, v, false);
-                if (c.mb != c.nb) {
-                  // the mirror image: 64 rows (this tile's columns) of 32 elements, unswizzled
-                  const uint32_t box = boxes + Cfg::BOX_BYTES + s * 32 * 64 + lane * 2;
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) {
-                    const __half h = __float2half_rn(v[j]);
-                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(box + j * 64), "h"(__half_as_ushort(h)) : "memory");
-                  }
-                }
-              } else {
-                float hi[32], lo[32];
-                input(0, col, hi);
-                input(1, col, lo);
-                const float dr = (OP == kOpUpdateWide && row_ok) ? p.vec[c.z * p.vec_ld + row] : 0.0f;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  float dv = dr;
-                  if constexpr (OP == kOpUpdateTall) dv = (col + j < p.out_cols) ? __ldg(p.vec + c.z * p.vec_ld + col + j) : 0.0f;
-                  v[j] = dv * (hi[j] + lo[j]) + v[j] * p.inv_scale;
-                }
-                if (p.flags & kFusedLast) {
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
-                  put(0, s, v, true);
-                } else {
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) lo[j] = v[j] - __half2float(__float2half_rn(v[j]));
-                  put(0, s, v, false);
-                  put(1, s, lo, false);
-                }
-              }
-            }
-            boxes_written();
-            if constexpr (OP == kOpDw) {
-              emit(c.z, 0, col0);
-            } else {
-              emit(0, 0, col0);
-              if constexpr (Cfg::SYM) {
-                // (rows of the mirror image that lie outside the matrix are clipped)
-                if (c.mb != c.nb && row0 < p.M && lane == 0) tma_store_3d(&p.o[1], boxes + Cfg::BOX_BYTES, row0, col0, c.z);
-              } else if constexpr (Cfg::UPDATE) {
-                if (!(p.flags & kFusedLast)) emit(1, 1, col0);
-              }
-            }
-            emitted();
-          }
+                       for (int j = 0; j < 8; ++j) {
+                         v[4 * j] += x[j].x; v[4 * j + 1] += x[j].y; v[4 * j + 2] += x[j].z; v[4 * j + 3] += x[j].w;
+                       }
+                     }
+                   },
+                   false, raw);
         }
       }
       tcgen05_fence_before_sync();
@@ -644,11 +763,99 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
       acc ^= 1;
       if (acc == 0) acc_ph ^= 1u;
     }
-    // stores handed to the TMA unit have to be performed before the CTA may go
-    if (lane == 0) bulk_wait_all();
+  }
+
+  if constexpr (CG == 1) {
+    if (split > 1) {
+      // ---- the cluster's CTAs hold the tile's parts: each takes 1 / split of the result columns
+      FusedPiece w;
+      w.tile = static_cast<int>(blockIdx.x) / split;
+      const FusedTile c = fused_tile<Cfg::SYM>(w.tile, p.tiles_m, p.tiles_n, per_z);
+      const int row = c.mb * Cfg::BM + quarter * 32 + lane;
+      constexpr int kTileSlabs = (OP == kOpGate ? BN / 2 : BN) / 32;
+      const int share = kTileSlabs / split;            // slabs of each CTA
+      bool fetched = false;
+      const int my_first = static_cast<int>(cluster_rank) * share + half;
+      if (epi) {
+        grid_dependency_wait();
+        if constexpr (Cfg::INPUTS > 0) {
+          const int col = c.nb * BN + my_first * 32;
+          fetched = half < share && col < p.out_cols;
+          if (fetched) {
+#pragma unroll
+            for (int q = 0; q < Cfg::INPUTS; ++q) fetch(q, c, row, col, raw[q]);
+          }
+        }
+        epi_ok = __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(0), 0u, wc, kDevTimeoutTmemFull));
+      }
+      __syncwarp();
+      cluster_sync();      // all MMAs of the cluster are done: the rings' memory is free
+      // Exchange area of a CTA: [sender][32-column group][4 columns][row] float4. A share of the gate's
+      // columns has two groups per slab (g, then u).
+      constexpr int kGroups = OP == kOpGate ? 2 : 1;
+      const uint32_t sender_bytes = static_cast<uint32_t>(share * kGroups) * 16384u;
+      const uint32_t lane_at = static_cast<uint32_t>(quarter * 32 + lane) * 16u;
+      if (epi && epi_ok) {
+        tcgen05_fence_after_sync();
+        for (int i = half; i < kTileSlabs; i += 2) {
+          const uint32_t to = static_cast<uint32_t>(i / share);
+          if (to == cluster_rank) continue;
+          // senders in the order of k, the receiver itself left out
+          const uint32_t place = cluster_rank - (cluster_rank > to ? 1u : 0u);
+#pragma unroll
+          for (int q = 0; q < kGroups; ++q) {
+            float v[32];
+            load_d(tmem_base + tmem_lane + i * 32 + q * (BN / 2), v);
+            if (row < p.M) {
+              const uint32_t dst = map_to_cta(
+                  smem_base + place * sender_bytes + static_cast<uint32_t>((i % share) * kGroups + q) * 16384u + lane_at, to);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + j * 2048u),
+                             "f"(v[4 * j]), "f"(v[4 * j + 1]), "f"(v[4 * j + 2]), "f"(v[4 * j + 3])
+                             : "memory");
+            }
+          }
+        }
+      }
+      __syncwarp();
+      cluster_sync();
+      if (epi && epi_ok && half < share) {
+        epilogue(c, my_first, 2, (static_cast<int>(cluster_rank) + 1) * share,
+                 [&](int tc, float (&v)[32]) {
+                   const int q = (OP == kOpGate && tc >= BN / 2) ? 1 : 0;
+                   const int i = (tc - q * (BN / 2)) / 32 - static_cast<int>(cluster_rank) * share;
+                   float own[32];
+                   load_d(tmem_base + tmem_lane + tc, own);
+#pragma unroll
+                   for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                   for (int r = 0; r < split; ++r) {
+                     if (r == static_cast<int>(cluster_rank)) {
+#pragma unroll
+                       for (int j = 0; j < 32; ++j) v[j] += own[j];
+                     } else if (row < p.M) {
+                       const uint32_t src = smem_base + static_cast<uint32_t>(r - (r > static_cast<int>(cluster_rank) ? 1 : 0)) * sender_bytes +
+                                            static_cast<uint32_t>(i * kGroups + q) * 16384u + lane_at;
+#pragma unroll
+                       for (int j = 0; j < 8; ++j) {
+                         float4 x;
+                         asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                      : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                                      : "r"(src + j * 2048u)
+                                      : "memory");
+                         v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
+                       }
+                     }
+                   }
+                 },
+                 fetched, raw);
+      }
+    }
   }
 
   // ------------------------------------------------------------------ teardown
+  // stores handed to the TMA unit have to be performed before the CTA may go
+  if (epi && lane == 0) bulk_wait_all();
   __syncwarp();
   // after a failed wait some role left its loop early: let bulk copies on their way land
   if (*reinterpret_cast<volatile uint32_t*>(p.status) != kDevOk) abort_grace_period();

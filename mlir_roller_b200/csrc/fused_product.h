@@ -29,7 +29,8 @@ inline bool aligned16(const void* p, long long ld) {
 
 // What the products of one plan share.
 struct FusedContext {
-  int device, sm_count, max_pairs;
+  int device;
+  FusedDevice dev;
   float* ws;            // partial tiles
   uint32_t* counters;
   uint32_t* status;
@@ -48,7 +49,7 @@ struct Product {
   Product(const FusedContext& x, int op_, int dt, long long M, long long N, long long K, int z)
       : op(op_), bf16(dt == 1) {
     memset(&p, 0, sizeof(p));
-    c = fused_choose(FusedShape{op, dt, M, N, K, z}, x.sm_count, x.max_pairs);
+    c = fused_choose(FusedShape{op, dt, M, N, K, z}, x.dev);
     p.M = static_cast<int>(M);
     p.out_cols = static_cast<int>(N);
     p.num_kb = c.num_kb;
@@ -56,7 +57,8 @@ struct Product {
     p.tiles_n = c.tiles_n;
     p.tiles_per_z = c.tiles_per_z;
     p.zcount = z;
-    p.nsplit = c.nsplit;
+    p.split = c.split;
+    p.sk_tiles = c.sk_tiles;
     p.ws = x.ws;
     p.counters = x.counters;
     p.status = x.status;
@@ -88,14 +90,11 @@ struct Product {
     p.out_zstride = zs;
     if (!aligned16(base, ld) || (z > 1 && (zs % 8 != 0 || zs < ld * p.M))) return ROLLER_OK;
     p.out_tma |= 1 << i;
-    // the box that one epilogue warp hands over (FusedCfg::BOX_COLS)
-    const bool narrow = op == kOpDact || (op == kOpGate && c.kv->block_n == 128);
-    return encode_batch16(&p.o[i], base, p.out_cols, p.M, z, ld, zs, narrow ? 32 : 64, 32,
-                          narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, as_bf16);
+    return encode_batch16(&p.o[i], base, p.out_cols, p.M, z, ld, zs, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, as_bf16);
   }
   // The mirror image of a symmetric output (always the library's own, aligned memory).
   int mirror(void* base, long long z, long long ld, long long zs) {
-    return encode_batch16(&p.o[1], base, p.out_cols, p.M, z, ld, zs, 32, 64, CU_TENSOR_MAP_SWIZZLE_NONE, bf16);
+    return encode_batch16(&p.o[1], base, p.out_cols, p.M, z, ld, zs, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE, bf16);
   }
   int launch(cudaStream_t st) {
     FUSED_CUDA(c.kv->launch(p, c.grid, st));

@@ -14,7 +14,7 @@ static cudaError_t fused_launch(const FusedParams& p, int grid, cudaStream_t str
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = Cfg::CG;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(Cfg::CG == 2 ? 2 : p.split);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   // scheduled while the previous kernel of the stream winds down; the kernel waits for that
@@ -35,6 +35,7 @@ static FusedVariant fused_make() {
   v.block_n = BN;
   v.dt = DT;
   v.threads = Cfg::THREADS;
+  v.max_split = Cfg::MAX_SPLIT < 8 ? Cfg::MAX_SPLIT : 8;
   v.smem_bytes = Cfg::SMEM_BYTES;
   v.func = reinterpret_cast<const void*>(&fused_gemm_kernel<Cfg>);
   v.launch = &fused_launch<Cfg>;
