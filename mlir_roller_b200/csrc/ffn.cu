@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kMaxExtent = 1 << 20;
 
-enum Operand { kX = 0, kWg, kWu, kWd, kDy, kOperands };
+enum Operand { kX = 0, kWg, kWu, kWd, kDy, kG, kU, kOperands };
 
 }  // namespace
 
@@ -36,9 +36,11 @@ struct roller_ffn_plan {
 namespace {
 
 int rows_of(const roller_ffn_plan* p, int which) {
-  return which == kX || which == kDy ? p->max_tokens : which == kWd ? p->d : p->f;
+  return which == kWd ? p->d : (which == kWg || which == kWu) ? p->f : p->max_tokens;
 }
-int cols_of(const roller_ffn_plan* p, int which) { return which == kWd ? p->f : p->d; }
+int cols_of(const roller_ffn_plan* p, int which) {
+  return which == kWd || which == kG || which == kU ? p->f : p->d;
+}
 
 size_t pad_bytes(const roller_ffn_plan* p, int which) {
   return static_cast<size_t>(rows_of(p, which)) * up64(cols_of(p, which)) * 2;
@@ -113,7 +115,7 @@ int roller_b200_ffn_create(int max_tokens, int d_model, int d_ff, int mode, int 
   cudaError_t e = cudaMalloc(&p->h, h_bytes);
   if (e == cudaSuccess && p->training) e = cudaMalloc(&p->dgu, 2 * h_bytes);
   for (int i = 0; i < kOperands && e == cudaSuccess; ++i)
-    if (cols_of(p, i) % 8 != 0 && (i != kDy || p->training)) e = cudaMalloc(&p->pad[i], pad_bytes(p, i));
+    if (cols_of(p, i) % 8 != 0 && (i < kDy || p->training)) e = cudaMalloc(&p->pad[i], pad_bytes(p, i));
   if (e != cudaSuccess) {
     const int failed = e == cudaErrorMemoryAllocation ? ROLLER_ERR_NOMEM : report_cuda_error(e, "ffn plan setup");
     cudaGetLastError();
@@ -188,13 +190,15 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     for (int j = 0; j < i; ++j)
       if (all[i] == all[j]) return ROLLER_ERR_INVALID;
   const bool bf16 = p->dt == 1;
-  const void *x, *wg, *wu, *wd, *dy;
-  long long ldx, ldg, ldu, ldd, ldy;
+  const void *x, *wg, *wu, *wd, *dy, *g, *u;
+  long long ldx, ldg, ldu, ldd, ldy, ldsg, ldsu;
   FUSED_OK(usable(p, kX, io->x, T, st, &x, &ldx));
   FUSED_OK(usable(p, kWg, io->wg, F, st, &wg, &ldg));
   FUSED_OK(usable(p, kWu, io->wu, F, st, &wu, &ldu));
   FUSED_OK(usable(p, kWd, io->wd, D, st, &wd, &ldd));
   FUSED_OK(usable(p, kDy, io->dy, T, st, &dy, &ldy));
+  FUSED_OK(usable(p, kG, io->g, T, st, &g, &ldsg));
+  FUSED_OK(usable(p, kU, io->u, T, st, &u, &ldsu));
   const long long zs = static_cast<long long>(p->max_tokens) * p->ldf;   // dg to du
   {
     Product a(p->ctx, kOpDact, p->dt, T, F, D, 1);
@@ -204,12 +208,8 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     FUSED_OK(a.output(0, p->dgu, 1, p->ldf, 0, bf16));
     FUSED_OK(a.output(1, static_cast<uint16_t*>(p->dgu) + zs, 1, p->ldf, 0, bf16));
     FUSED_OK(a.output(2, p->h, 1, p->ldf, 0, bf16));
-    a.p.in[0] = io->g.ptr;
-    a.p.in[1] = io->u.ptr;
-    a.p.in_ld[0] = io->g.ld;
-    a.p.in_ld[1] = io->u.ld;
-    a.p.in_cols = F;
-    a.p.in_vec = aligned16(io->g.ptr, io->g.ld) && aligned16(io->u.ptr, io->u.ld);
+    FUSED_OK(a.input(0, g, 1, ldsg, 0));
+    FUSED_OK(a.input(1, u, 1, ldsu, 0));
     FUSED_OK(a.launch(st));
   }
   {
@@ -227,13 +227,13 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     FUSED_OK(w.output(0, io->dwd.ptr, 1, io->dwd.ld, 0, bf16));
     FUSED_OK(w.launch(st));
   }
-  Product g(p->ctx, kOpDx, p->dt, T, D, F, 1);
-  g.p.b_early = 1;   // Wg and Wu do not come from the kernel before
-  FUSED_OK(g.a_k(p->dgu, F, T, 2, p->ldf, zs));
-  FUSED_OK(g.b_mn(0, wg, D, F, 1, ldg, 0));
-  FUSED_OK(g.b_mn(1, wu, D, F, 1, ldu, 0));
-  FUSED_OK(g.output(0, io->dx.ptr, 1, io->dx.ld, 0, bf16));
-  return g.launch(st);
+  Product r(p->ctx, kOpDx, p->dt, T, D, F, 1);
+  r.p.b_early = 1;   // Wg and Wu do not come from the kernel before
+  FUSED_OK(r.a_k(p->dgu, F, T, 2, p->ldf, zs));
+  FUSED_OK(r.b_mn(0, wg, D, F, 1, ldg, 0));
+  FUSED_OK(r.b_mn(1, wu, D, F, 1, ldu, 0));
+  FUSED_OK(r.output(0, io->dx.ptr, 1, io->dx.ld, 0, bf16));
+  return r.launch(st);
 }
 
 int roller_b200_ffn_status(roller_ffn_plan* p, uint32_t* device_status) {

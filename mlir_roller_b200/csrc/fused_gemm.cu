@@ -18,7 +18,7 @@ struct TileCost {
   double kb_us;    // one k-block of one tile while every SM works
   double tile_us;  // fill and the last tile's epilogue
 };
-constexpr TileCost kTiles[] = {{2, 256, 0.31, 7.0}, {1, 256, 0.36, 6.0}, {1, 128, 0.24, 5.0}};
+constexpr TileCost kTiles[] = {{2, 256, 0.36, 7.0}, {1, 256, 0.40, 6.0}, {1, 128, 0.28, 5.0}};
 
 }  // namespace
 
@@ -72,15 +72,15 @@ static cudaError_t bind_device(FusedDevice* d) {
     if (e != cudaSuccess) return e;
     if (d->clusters[i] > d->sm_count >> i) d->clusters[i] = d->sm_count >> i;
   }
-  if (d->clusters[1] > kFusedMaxPairs) d->clusters[1] = kFusedMaxPairs;
   return cudaSuccess;
 }
 
 // The kernels have the same inner loop, so a launch takes about (k-blocks the busiest worker gets)
 // x (their cost) + the fill and drain; the smallest estimate wins.
-//   * CTA pairs, whole tiles: the busiest worker gets ceil(tiles / workers) of them;
-//   * CTA pairs, the leftover tiles dealt out along k: an even share of all k-blocks, and the
-//     exchange of the pieces' sums, which hides behind whole tiles where there are any;
+//   * CTA pairs: the busiest worker gets ceil(tiles / workers) whole tiles. (Dealing the tiles that
+//     do not fill a last wave out along k was built and measured: writing and reading back the
+//     fp32 sums of 256 x 256 tiles costs 15-25 us, more than an even share of k saves up to
+//     K = 8192.)
 //   * single CTAs, a cluster per tile: 1 / split of a tile's k-blocks per wave of clusters, and the
 //     exchange inside the cluster.
 FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
@@ -99,26 +99,18 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
     f.num_kb = static_cast<int>((s.K + 63) / 64);
     const int kbs = f.num_kb * (s.op == kOpDx ? 2 : 1);
     const long long tiles = static_cast<long long>(f.tiles_per_z) * s.zcount;
-    auto consider = [&](int split, int sk_tiles, long long grid, double us) {
+    auto consider = [&](int split, long long grid, double us) {
       if (best.kv && us >= best_us) return;
       best_us = us;
       best = f;
       best.split = split;
-      best.sk_tiles = sk_tiles;
       best.grid = static_cast<int>(grid);
     };
     if (c.cta_group == 2) {
       const int workers = d.clusters[1];
       if (workers < 1) continue;
       const long long waves = (tiles + workers - 1) / workers;
-      consider(1, 0, 2 * (tiles < workers ? tiles : workers), waves * kbs * c.kb_us + c.tile_us);
-      const int left = static_cast<int>(tiles % workers);
-      const long long groups = (kbs + kSkGroup - 1) / kSkGroup;
-      if (left && left * groups >= workers) {
-        const long long whole = tiles / workers;
-        const double share = static_cast<double>(left * groups) / workers * kSkGroup;
-        consider(1, left, 2 * workers, (whole * kbs + share) * c.kb_us + c.tile_us + (whole ? 2.0 : 6.0));
-      }
+      consider(1, 2 * (tiles < workers ? tiles : workers), waves * kbs * c.kb_us + c.tile_us);
       continue;
     }
     for (int i = 0, split = 1; i < 4 && split <= kv->max_split && split <= kbs; ++i, split *= 2) {
@@ -127,10 +119,10 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
       const long long waves = (tiles + at_once - 1) / at_once;
       const int part = (kbs + split - 1) / split;
       if (split == 1) {
-        consider(1, 0, tiles < at_once ? tiles : at_once, waves * part * c.kb_us + c.tile_us);
+        consider(1, tiles < at_once ? tiles : at_once, waves * part * c.kb_us + c.tile_us);
       } else {
         // a cluster has one tile: from the second wave on every tile pays for its own fill and drain
-        consider(split, 0, tiles * split, waves * (part * c.kb_us + c.tile_us) + 1.5 + 0.2 * split);
+        consider(split, tiles * split, waves * (part * c.kb_us + c.tile_us) + 1.5 + 0.2 * split);
       }
     }
   }
@@ -145,9 +137,6 @@ int fused_context_create(FusedContext* c) {
   if (prop.major != 10) return ROLLER_ERR_DEVICE;
   c->dev.sm_count = prop.multiProcessorCount;
   cudaError_t e = bind_device(&c->dev);
-  if (e == cudaSuccess) e = cudaMalloc(&c->ws, kFusedWsBytes);
-  if (e == cudaSuccess) e = cudaMalloc(&c->counters, kFusedCounters * sizeof(uint32_t));
-  if (e == cudaSuccess) e = cudaMemset(c->counters, 0, kFusedCounters * sizeof(uint32_t));
   if (e == cudaSuccess) e = cudaMalloc(&c->status, sizeof(uint32_t));
   if (e == cudaSuccess) e = cudaMemset(c->status, 0, sizeof(uint32_t));
   if (e == cudaSuccess) return ROLLER_OK;
@@ -158,11 +147,8 @@ int fused_context_create(FusedContext* c) {
 }
 
 void fused_context_destroy(FusedContext* c) {
-  cudaFree(c->ws);
-  cudaFree(c->counters);
   cudaFree(c->status);
-  c->ws = nullptr;
-  c->counters = c->status = nullptr;
+  c->status = nullptr;
 }
 
 int fused_context_status(FusedContext* c, uint32_t* device_status) {
@@ -171,9 +157,7 @@ int fused_context_status(FusedContext* c, uint32_t* device_status) {
   FUSED_CUDA(cudaMemcpy(&h, c->status, sizeof(h), cudaMemcpyDeviceToHost));
   if (device_status) *device_status = h;
   if (h == 0) return ROLLER_OK;
-  // a launch that gave up may have left a split reduction half counted
   FUSED_CUDA(cudaMemset(c->status, 0, sizeof(uint32_t)));
-  FUSED_CUDA(cudaMemset(c->counters, 0, kFusedCounters * sizeof(uint32_t)));
   return ROLLER_ERR_TIMEOUT;
 }
 

@@ -21,8 +21,6 @@ struct IntTag {
   static constexpr int value = V;
 };
 
-constexpr int kSkGroup = 4;     // k-blocks that stay together when a tile is cut along k
-
 constexpr int kFusedSave = 1;   // kOpGate: g and u are written too
 constexpr int kFusedLast = 2;   // kOpUpdate*: the result leaves as bf16, divided by the scale
 
@@ -36,11 +34,7 @@ struct FusedParams {
   long long out_zstride;
   int out_cols;         // columns of the outputs (those beyond are not written)
   int out_tma;          // bit o: output o leaves through o[o] (16-byte aligned base and rows)
-  const void* in[2];    // element-wise inputs of the epilogue
-  long long in_ld[2];
-  long long in_zstride;
-  int in_cols;          // columns that may be read
-  int in_vec;           // their rows are 16-byte aligned
+  CUtensorMap i[2];     // element-wise inputs of the epilogue
   float* vec;           // kOpPoly writes, kOpUpdate* reads: one value per row of q, [z][vec_ld]
   int vec_ld;
   int M;                // rows of D
@@ -48,9 +42,6 @@ struct FusedParams {
   int a_bytes;          // bytes one TMA load of A brings (fewer rows than 128 on single CTAs)
   int tiles_m, tiles_n, tiles_per_z, zcount;
   int split;            // single CTAs: cluster size, CTAs that share a tile's k (1 = none)
-  int sk_tiles;         // CTA pairs: tiles cut along k and dealt out to all workers (0 = none)
-  float* ws;            // their sums: two slots per worker and CTA, 128 * block_n floats each
-  uint32_t* counters;   // one per such tile and CTA of a pair; zero between launches
   int b_early;          // the second operand may be read before the previous kernel is done
   int act;
   int flags;
@@ -82,15 +73,12 @@ struct FusedShape {
 };
 struct FusedChoice {
   const FusedVariant* kv;
-  int tiles_m, tiles_n, tiles_per_z, num_kb, split, sk_tiles, grid;
+  int tiles_m, tiles_n, tiles_per_z, num_kb, split, grid;
 };
 // What the current device holds at once: CTAs of one per SM, and clusters of 2, 4 and 8.
 struct FusedDevice {
   int sm_count;
   int clusters[4];     // [i]: clusters of 2^i CTAs
 };
-constexpr int kFusedMaxPairs = 80;
-constexpr int kFusedCounters = 2 * kFusedMaxPairs;
-constexpr size_t kFusedWsBytes = static_cast<size_t>(kFusedMaxPairs) * 2 * 2 * 128 * 256 * 4;
 FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d);
 }  // namespace rb200

@@ -22,16 +22,16 @@
 // that holds g[i,j] also holds u[i,j] and neither reaches memory unless it is asked for), and only
 // one triangle of a symmetric product is computed.
 //
-// Reductions are cut in two ways, neither of which makes a CTA wait for one that may not run:
-//   * single CTAs (few rows or columns, hence few tiles, and a weight that has to be streamed by
-//     all SMs to come at the memory's rate): a cluster of 2, 4 or 8 CTAs shares one tile, each
-//     takes a part of k, and at the end each collects the others' sums of its share of the
-//     columns through distributed shared memory (the ring's, which is free by then);
-//   * CTA pairs: the tiles that do not fill a last wave (sk_tiles of them) are dealt out along k in
-//     equal runs to all workers, before the whole tiles. Each piece leaves its fp32 sums in a
-//     workspace and counts itself in; the one that arrives last adds all of them and runs the
-//     epilogue. Nobody waits for anybody.
-// Both add the parts in the order of k, so results do not depend on timing.
+// With few rows or columns there are few tiles, and a weight has to be streamed by all SMs to come
+// at the memory's rate. Single CTAs therefore also run in clusters of 2, 4 or 8 that share one
+// tile: each takes a part of k, and at the end each collects the others' sums of its share of
+// the columns through distributed shared memory (the ring's, which is free by then), adds them in the
+// order of k and runs the epilogue on its share. Results do not depend on timing.
+//
+// Epilogue inputs come and results go through the TMA unit in boxes of 32 rows x 32 columns, one
+// warp's slab. Loads and stores from registers, a thread per row, were measured beside it (whole
+// 32-byte sectors): the pair kernels got a third slower with kOpDact and kOpUpdate*, because
+// every access of a warp touches 32 lines.
 //
 // A launch may be scheduled while the previous one of its stream still runs (programmatic
 // dependent launch). It touches memory only behind griddepcontrol.wait, with one exception
@@ -66,10 +66,11 @@ struct FusedCfg {
   static constexpr int INPUTS = (OP == kOpDact || UPDATE) ? 2 : OP == kOpPoly ? 1 : 0;
   static constexpr int BOX_BYTES = 32 * 64;
   static constexpr int EPI_WARPS = 8;
-  // boxes a warp has under way at once: two beside a ring of six stages, four where an epilogue
-  // writes several matrices (five stages)
-  static constexpr int RING = (CG == 1 && BN == 256) || OP == kOpDown || OP == kOpDx || OP == kOpDw ? 2 : 4;
-  static constexpr int STAGING_BYTES = EPI_WARPS * RING * BOX_BYTES;
+  // boxes of one warp: its inputs, and the results it has under way (those of one slab where an
+  // epilogue writes several matrices)
+  static constexpr int RING = OP == kOpDact ? 3 : 2;
+  static constexpr int WARP_BOXES = INPUTS + RING;
+  static constexpr int STAGING_BYTES = EPI_WARPS * WARP_BOXES * BOX_BYTES;
   static constexpr int CTRL_BYTES = 256;
   static constexpr int SMEM_LIMIT = 232448;      // 227 KiB opt-in maximum per CTA
   static constexpr int STAGES_FIT = (SMEM_LIMIT - 1024 - CTRL_BYTES - STAGING_BYTES) / STAGE_BYTES;
@@ -125,20 +126,6 @@ __device__ __forceinline__ void activation(float v, float& y, float& slope) {
   }
 }
 
-// Barrier among the 256 epilogue threads carrying a vote.
-__device__ __forceinline__ bool fused_bar_any(bool mine) {
-  uint32_t out;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 q, %1, 0;\n\t"
-      "bar.red.or.pred p, 1, 256, q;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(out)
-      : "r"(static_cast<uint32_t>(mine))
-      : "memory");
-  return out != 0;
-}
-
 struct FusedTile {
   int z, mb, nb;
 };
@@ -168,62 +155,6 @@ __device__ __forceinline__ FusedTile fused_tile(int t, int tiles_m, int tiles_n,
   }
   return c;
 }
-
-// One piece of work: k-blocks [kb0, kb1) of a tile.
-struct FusedPiece {
-  int tile, kb0, kb1;
-  bool whole;
-};
-
-// The pieces of one worker. The first `sk_tiles` tiles are cut into groups of kSkGroup k-blocks, dealt
-// out evenly; the other tiles follow whole, round-robin. (A run spans at most two tiles: there
-// are fewer sk_tiles than workers.)
-struct FusedWalk {
-  int tiles, sk_tiles, total_kb, groups, workers, worker;
-  int g, g_end, next_tile;
-  __device__ FusedWalk(const FusedParams& p, int total_kb_, int workers_, int worker_)
-      : tiles(p.tiles_per_z * p.zcount), sk_tiles(p.sk_tiles), total_kb(total_kb_),
-        groups((total_kb_ + kSkGroup - 1) / kSkGroup), workers(workers_), worker(worker_) {
-    g = sk_tiles ? begin(worker) : 0;
-    g_end = sk_tiles ? begin(worker + 1) : 0;
-    next_tile = sk_tiles + worker;
-  }
-  __device__ int begin(int w) const {
-    return static_cast<int>(static_cast<long long>(sk_tiles) * groups * w / workers);
-  }
-  __device__ bool next(FusedPiece& s) {
-    if (g < g_end) {
-      s.tile = g / groups;
-      const int t0 = s.tile * groups;
-      const int e = min(g_end, t0 + groups);
-      s.kb0 = (g - t0) * kSkGroup;
-      s.kb1 = min((e - t0) * kSkGroup, total_kb);
-      s.whole = (g == t0 && e == t0 + groups);
-      g = e;
-      return true;
-    }
-    if (next_tile >= tiles) return false;
-    s.tile = next_tile;
-    s.kb0 = 0;
-    s.kb1 = total_kb;
-    s.whole = true;
-    next_tile += workers;
-    return true;
-  }
-  // The workers [first, last] that hold pieces of sk tile `t`.
-  __device__ void holders(int t, int& first, int& last) const {
-    const long long all = static_cast<long long>(sk_tiles) * groups;
-    const int g0 = t * groups, g1 = g0 + groups;
-    first = static_cast<int>(static_cast<long long>(g0) * workers / all);
-    while (first > 0 && begin(first) > g0) --first;
-    while (begin(first + 1) <= g0) ++first;
-    last = static_cast<int>(static_cast<long long>(g1 - 1) * workers / all);
-    while (begin(last) >= g1) --last;
-    while (begin(last + 1) < g1) ++last;
-  }
-  // A worker's pieces have a slot each: 0 for the tile its run begins in, 1 for the next.
-  __device__ int slot(int w, int t) const { return 2 * w + (begin(w) / groups == t ? 0 : 1); }
-};
 
 // Loads `ROWS` m/n values x 64 k of an operand at (row0, k0, z) into shared memory.
 template <int ROWS, bool MN, bool PAIR>
@@ -261,7 +192,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   auto tmem_empty_bar = [&](int a) { return ctrl + 144u + 8u * a; };
   const uint32_t mma_done_bar = ctrl + 160u;
   const uint32_t tmem_slot = ctrl + 176u;
-  const uint32_t last_slot = ctrl + 180u;   // whether this CTA's piece was the tile's last
+  auto in_bar = [&](int w) { return ctrl + 184u + 8u * w; };   // a warp's inputs have landed
   const WaitCtx wc{p.status, p.spin_limit};
 
   const int warp = threadIdx.x >> 5;
@@ -282,6 +213,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
       mbar_init(tmem_empty_bar(a), CG * Cfg::EPI_WARPS);
     }
     mbar_init(mma_done_bar, 1);
+    for (int w = 0; w < Cfg::EPI_WARPS; ++w) mbar_init(in_bar(w), 1);
     fence_barrier_init();
   }
   if (warp == 1) tmem_alloc<CG>(tmem_slot, Cfg::TMEM_COLS);
@@ -299,21 +231,15 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
 
   const int per_z = p.tiles_per_z;
+  const int tiles = per_z * p.zcount;
   const int total_kb = p.num_kb * (OP == kOpDx ? 2 : 1);
+  // Tiles go round-robin to the CTAs, pairs or clusters; a CTA of a splitting cluster takes its part
+  // of k, and its cluster has exactly one tile.
   const int per_worker = CG == 2 ? 2 : split;
-  FusedWalk walk(p, total_kb, static_cast<int>(gridDim.x) / per_worker, static_cast<int>(blockIdx.x) / per_worker);
-  // the part of each tile's k that this CTA of a splitting cluster takes (the cluster then has
-  // exactly one tile)
-  const int part_kb0 = static_cast<int>(static_cast<long long>(total_kb) * cluster_rank / split);
-  const int part_kb1 = static_cast<int>(static_cast<long long>(total_kb) * (cluster_rank + 1) / split);
-  auto next_piece = [&](FusedPiece& s) {
-    if (!walk.next(s)) return false;
-    if (split > 1) {
-      s.kb0 = part_kb0;
-      s.kb1 = part_kb1;
-    }
-    return true;
-  };
+  const int workers = static_cast<int>(gridDim.x) / per_worker;
+  const int worker = static_cast<int>(blockIdx.x) / per_worker;
+  const int kb0 = static_cast<int>(static_cast<long long>(total_kb) * (cluster_rank - cta_rank) / split);
+  const int kb1 = static_cast<int>(static_cast<long long>(total_kb) * (cluster_rank - cta_rank + 1) / split);
 
   bool epi_ok = true;
 
@@ -357,14 +283,12 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     };
     int s = 0;
     uint32_t ph = 0;
-    bool ok = true, first = true;
-    FusedPiece w;
-    while (ok && next_piece(w)) {
-      const FusedTile c = fused_tile<Cfg::SYM>(w.tile, p.tiles_m, p.tiles_n, per_z);
-      int kb = w.kb0;
-      if (first) {
-        first = false;
-        const int early = p.b_early ? min(STAGES, w.kb1 - w.kb0) : 0;
+    bool ok = true;
+    for (int t = worker; ok && t < tiles; t += workers) {
+      const FusedTile c = fused_tile<Cfg::SYM>(t, p.tiles_m, p.tiles_n, per_z);
+      int kb = kb0;
+      if (t == worker) {
+        const int early = p.b_early ? min(STAGES, kb1 - kb0) : 0;
         for (int i = 0; i < early; ++i) load_b(i, arm(i), c, kb + i);
         grid_dependency_wait();
         grid_launch_dependents();
@@ -374,17 +298,13 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
         s = early;
         if (s == STAGES) { s = 0; ph ^= 1u; }
       }
-      for (; kb < w.kb1; ++kb) {
+      for (; kb < kb1; ++kb) {
         if (!mbar_wait(empty_bar(s), ph ^ 1u, wc, kDevTimeoutEmpty)) { ok = false; break; }
         const uint32_t bar = arm(s);
         load_a(s, bar, c, kb);
         load_b(s, bar, c, kb);
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
-    }
-    if (first) {   // (no work: a pair's grid may hold more CTAs than pieces)
-      grid_dependency_wait();
-      grid_launch_dependents();
     }
     // the MMA issuer's last releases must land in this CTA before it may exit
     for (int i = 0; i < STAGES && ok; ++i) {
@@ -402,12 +322,11 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     int s = 0, acc = 0;
     uint32_t ph = 0, acc_ph = 0;
     bool ok = true;
-    FusedPiece w;
-    while (ok && next_piece(w)) {
+    for (int t = worker; ok && t < tiles; t += workers) {
       if (!mbar_wait(tmem_empty_bar(acc), acc_ph ^ 1u, wc, kDevTimeoutTmemEmpty)) break;
       tcgen05_fence_after_sync();
       const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-      for (int kb = w.kb0; kb < w.kb1; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait(full_bar(s), ph, wc, kDevTimeoutReady)) { ok = false; break; }
         tcgen05_fence_after_sync();
         const uint32_t stage = smem_base + s * Cfg::STAGE_BYTES;
@@ -415,7 +334,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
         const uint64_t b = fused_desc<Cfg::B_MN>(stage + Cfg::A_BYTES);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_f16<CG>(d_tmem, a + kk * a_step, b + kk * b_step, idesc, (kb != w.kb0 || kk != 0) ? 1u : 0u);
+          umma_f16<CG>(d_tmem, a + kk * a_step, b + kk * b_step, idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
         umma_commit<CG>(empty_bar(s));
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
@@ -432,10 +351,11 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   const bool epi = warp >= Cfg::FIRST_EPI_WARP;
   const int quarter = warp & 3;                     // TMEM lanes 32 * (warp id mod 4)
   const int half = (warp - Cfg::FIRST_EPI_WARP) >> 2;
-  const int et = static_cast<int>(threadIdx.x) - Cfg::FIRST_EPI_WARP * 32;
-  const uint32_t boxes = staging + static_cast<uint32_t>(warp - Cfg::FIRST_EPI_WARP) * (Cfg::RING * Cfg::BOX_BYTES);
+  const uint32_t in_boxes = staging + static_cast<uint32_t>(warp - Cfg::FIRST_EPI_WARP) * (Cfg::WARP_BOXES * Cfg::BOX_BYTES);
+  const uint32_t boxes = in_boxes + Cfg::INPUTS * Cfg::BOX_BYTES;
   const uint32_t tmem_lane = static_cast<uint32_t>(quarter * 32) << 16;
-  int box_at = 0;      // ring of staging boxes
+  int box_at = 0;      // ring of result boxes
+  uint32_t in_ph = 0;
 
   auto load_d = [&](uint32_t taddr, float (&v)[32]) {
     uint32_t r[32];
@@ -444,39 +364,28 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
   };
-  // 32 16-bit elements of this thread's row of epilogue input `which`
-  auto fetch = [&](int which, const FusedTile& c, int row, int col, uint4 (&raw)[4]) {
-    const uint16_t* src = static_cast<const uint16_t*>(p.in[which]) + c.z * p.in_zstride +
-                          static_cast<long long>(row) * p.in_ld[which] + col;
-    if (p.in_vec && col + 32 <= p.in_cols) {
+  // The inputs of one slab are sent for, and later taken into registers (16-bit pairs).
+  auto fetch = [&](const FusedTile& c, int row0, int col) {
+    __syncwarp();      // (every lane has taken the previous slab's)
+    if (lane == 0) {
+      const uint32_t bar = in_bar(warp - Cfg::FIRST_EPI_WARP);
+      mbar_expect_tx(bar, Cfg::INPUTS * Cfg::BOX_BYTES);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        raw[j] = row < p.M ? __ldg(reinterpret_cast<const uint4*>(src) + j) : make_uint4(0, 0, 0, 0);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int k = j * 8 + i * 2;
-          uint32_t lo = 0, hi = 0;
-          if (row < p.M && col + k < p.in_cols) lo = __ldg(src + k);
-          if (row < p.M && col + k + 1 < p.in_cols) hi = __ldg(src + k + 1);
-          w[i] = lo | (hi << 16);
-        }
-        raw[j] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+      for (int q = 0; q < Cfg::INPUTS; ++q) tma_load_3d(in_boxes + q * Cfg::BOX_BYTES, &p.i[q], bar, col, row0, c.z);
     }
   };
-  auto expand = [&](const uint4 (&raw)[4], float (&v)[32]) {
+  auto take = [&](uint32_t (&raw)[Cfg::INPUTS ? Cfg::INPUTS : 1][16]) {
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(in_bar(warp - Cfg::FIRST_EPI_WARP), in_ph, wc, kDevTimeoutFull));
+    in_ph ^= 1u;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float2 f;
-      f = fused_unpack<DT>(raw[j].x); v[8 * j] = f.x; v[8 * j + 1] = f.y;
-      f = fused_unpack<DT>(raw[j].y); v[8 * j + 2] = f.x; v[8 * j + 3] = f.y;
-      f = fused_unpack<DT>(raw[j].z); v[8 * j + 4] = f.x; v[8 * j + 5] = f.y;
-      f = fused_unpack<DT>(raw[j].w); v[8 * j + 6] = f.x; v[8 * j + 7] = f.y;
-    }
+    for (int q = 0; q < Cfg::INPUTS; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(raw[q][4 * j]), "=r"(raw[q][4 * j + 1]), "=r"(raw[q][4 * j + 2]), "=r"(raw[q][4 * j + 3])
+                     : "r"(in_boxes + q * Cfg::BOX_BYTES + lane * 64 + (j ^ ((lane >> 1) & 3)) * 16)
+                     : "memory");
+    return ok;
   };
   // A staging box that the TMA unit has read (the one handed out RING boxes ago).
   auto free_box = [&]() {
@@ -486,9 +395,8 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     box_at = box_at + 1 == Cfg::RING ? 0 : box_at + 1;
     return b;
   };
-  // 32 columns of this warp's 32 rows, as 16-bit values, to columns col.. of output `o`
-  auto emit = [&](int o, const FusedTile& c, int row0, int col, const float (&v)[32], bool as_bf16) {
-    const uint32_t box = free_box();
+  // 32 columns of this warp's 32 rows, as 16-bit values, into a box ...
+  auto put = [&](uint32_t box, const float (&v)[32], bool as_bf16) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t w[4];
@@ -502,6 +410,11 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
                    "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                    : "memory");
     }
+  };
+  // ... and from there to columns col.. of output `o`.
+  auto emit = [&](int o, const FusedTile& c, int row0, int col, const float (&v)[32], bool as_bf16) {
+    const uint32_t box = free_box();
+    put(box, v, as_bf16);
     const int oz = OP == kOpDw ? 0 : c.z;
     if (p.out_tma & (1 << o)) {
       fence_proxy_async_smem();
@@ -546,11 +459,10 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     }
   };
 
-  // The epilogue of this warp's slabs `first`, first + step, .. < count of tile `c`. Slab i is the 32
+  // The epilogue of this warp's slabs slab0, slab0 + step, .. < slab_end of tile `c`. Slab i is the 32
   // result columns from tile column 32 i on; `sums(tile_col, v)` gives 32 columns of D.
-  // `raw` holds the first slab's inputs already when `fetched`.
-  auto epilogue = [&](const FusedTile& c, int slab0, int step, int slab_end, auto sums, bool fetched,
-                      uint4 (&raw)[Cfg::INPUTS ? Cfg::INPUTS : 1][4]) {
+  // The first slab's inputs have been sent for.
+  auto epilogue = [&](const FusedTile& c, int slab0, int step, int slab_end, auto sums) {
     const int row0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32;
     const int row = row0 + lane;
     const int col_base = c.nb * (OP == kOpGate ? BN / 2 : BN);
@@ -561,21 +473,15 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
         const int tc = i * 32, col = col_base + tc;
         if (col >= p.out_cols) break;     // (uniform over the warp)
         float v[32];
+        uint32_t raw[Cfg::INPUTS ? Cfg::INPUTS : 1][16];
         if constexpr (Cfg::INPUTS > 0) {
-          if (!fetched) {
-#pragma unroll
-            for (int q = 0; q < Cfg::INPUTS; ++q) fetch(q, c, row, col, raw[q]);
-          }
+          epi_ok = take(raw) && epi_ok;
+          // the next slab's inputs are on their way while this one is worked on
+          if (i + step < slab_end && col + step * 32 < p.out_cols) fetch(c, row0, col + step * 32);
         }
-        // the next slab's inputs are on their way while this one is worked on
-        auto refill = [&]() {
-          if constexpr (Cfg::INPUTS > 0) {
-            fetched = i + step < slab_end && col + step * 32 < p.out_cols;
-            if (fetched) {
-#pragma unroll
-              for (int q = 0; q < Cfg::INPUTS; ++q) fetch(q, c, row, col + step * 32, raw[q]);
-            }
-          }
+        auto input = [&](int q, int k) {      // element k of input q
+          const float2 f = fused_unpack<DT>(raw[q][k / 2]);
+          return k & 1 ? f.y : f.x;
         };
         if constexpr (OP == kOpGate) {
           float w[32];
@@ -593,34 +499,40 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
           }
           emit(0, c, row0, col, v, false);
         } else if constexpr (OP == kOpDact) {
-          float g[32], w[32];
-          expand(raw[0], g);
-          expand(raw[1], w);
-          refill();
+          float du[32], h[32];
           sums(tc, v);
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             float y, slope;
-            activation<ACT>(g[j], y, slope);
-            const float dh = v[j], uu = w[j];
-            g[j] = dh * uu * slope;    // dg
-            v[j] = dh * y;             // du
-            w[j] = y * uu;             // h
+            activation<ACT>(input(0, j), y, slope);
+            const float dh = v[j], uu = input(1, j);
+            v[j] = dh * uu * slope;    // dg
+            du[j] = dh * y;
+            h[j] = y * uu;
           }
-          emit(0, c, row0, col, g, false);
-          emit(1, c, row0, col, v, false);
-          emit(2, c, row0, col, w, false);
+          // three matrices, one hand-over (all three are the library's own, aligned memory)
+          if (lane == 0) bulk_wait_read_all();
+          __syncwarp();
+          put(boxes, v, false);
+          put(boxes + Cfg::BOX_BYTES, du, false);
+          put(boxes + 2 * Cfg::BOX_BYTES, h, false);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (row0 < p.M) {
+#pragma unroll
+              for (int o = 0; o < 3; ++o) tma_store_3d(&p.o[o], boxes + o * Cfg::BOX_BYTES, col, row0, 0);
+            }
+            bulk_commit_group();
+          }
         } else if constexpr (OP == kOpDown || OP == kOpDx || OP == kOpDw) {
           sums(tc, v);
           emit(OP == kOpDw ? c.z : 0, c, row0, col, v, false);
         } else if constexpr (Cfg::SYM) {
           if constexpr (OP == kOpPoly) {
-            float pin[32];
-            expand(raw[0], pin);
-            refill();
             sums(tc, v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = p.coef_b * pin[j] + p.coef_c * v[j];
+            for (int j = 0; j < 32; ++j) v[j] = p.coef_b * input(0, j) + p.coef_c * v[j];
             // what rounding q's diagonal to 16 bits loses is as large as the rest of that
             // rounding together: it goes into the vector that scales x instead
             const int dj = row - col;
@@ -638,27 +550,23 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
           emit(0, c, row0, col, v, false);
           if (c.mb != c.nb) emit_mirror(c, row0, col, v);
         } else {
-          float hi[32], lo[32];
-          expand(raw[0], hi);
-          expand(raw[1], lo);
-          refill();
           sums(tc, v);
           const float dr = (OP == kOpUpdateWide && row < p.M) ? p.vec[c.z * p.vec_ld + row] : 0.0f;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             float dv = dr;
             if constexpr (OP == kOpUpdateTall) dv = (col + j < p.out_cols) ? __ldg(p.vec + c.z * p.vec_ld + col + j) : 0.0f;
-            v[j] = dv * (hi[j] + lo[j]) + v[j] * p.inv_scale;
+            v[j] = dv * (input(0, j) + input(1, j)) + v[j] * p.inv_scale;
           }
           if (p.flags & kFusedLast) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
             emit(0, c, row0, col, v, true);
           } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) lo[j] = v[j] - __half2float(__float2half_rn(v[j]));
             emit(0, c, row0, col, v, false);
-            emit(1, c, row0, col, lo, false);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
+            emit(1, c, row0, col, v, false);
           }
         }
       }
@@ -673,87 +581,23 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   };
 
   constexpr int kSlabs = Cfg::OUT_COLS / 32;     // slabs of one warp of a whole tile
-  uint4 raw[Cfg::INPUTS ? Cfg::INPUTS : 1][4];
 
   if (epi && split == 1) {
     grid_dependency_wait();
     int acc = 0;
     uint32_t acc_ph = 0;
-    FusedPiece w;
-    while (epi_ok && next_piece(w)) {
-      const FusedTile c = fused_tile<Cfg::SYM>(w.tile, p.tiles_m, p.tiles_n, per_z);
-      const int row = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32 + lane;
-      bool fetched = false;
-      if constexpr (Cfg::INPUTS > 0) {
-        // the first slab's inputs do not depend on the product
+    for (int t = worker; epi_ok && t < tiles; t += workers) {
+      const FusedTile c = fused_tile<Cfg::SYM>(t, p.tiles_m, p.tiles_n, per_z);
+      if constexpr (Cfg::INPUTS > 0) {     // they do not depend on the product
         const int col = c.nb * BN + half * Cfg::OUT_COLS;
-        fetched = w.whole && col < p.out_cols;
-        if (fetched) {
-#pragma unroll
-          for (int q = 0; q < Cfg::INPUTS; ++q) fetch(q, c, row, col, raw[q]);
-        }
+        if (col < p.out_cols) fetch(c, (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32, col);
       }
       epi_ok = __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(acc), acc_ph, wc, kDevTimeoutTmemFull));
+      if (!epi_ok) break;
+      tcgen05_fence_after_sync();
       const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN) + tmem_lane;
-      if (w.whole) {
-        if (!epi_ok) break;
-        tcgen05_fence_after_sync();
-        epilogue(c, half * kSlabs, 1, (half + 1) * kSlabs,
-                 [&](int tc, float (&v)[32]) { load_d(d_tmem + tc, v); }, fetched, raw);
-      } else if constexpr (CG == 2) {
-        // ---- a piece: leave its sums, count in, go on only as the tile's last one
-        if (fused_bar_any(!epi_ok)) { epi_ok = false; break; }
-        tcgen05_fence_after_sync();
-        constexpr size_t kSlot4 = 32 * BN;     // float4 per CTA and piece
-        float4* const ws4 = reinterpret_cast<float4*>(p.ws) + quarter * 32 + lane;
-        auto slot4 = [&](int worker) {
-          return ws4 + (static_cast<size_t>(walk.slot(worker, w.tile)) * CG + cta_rank) * kSlot4;
-        };
-        float4* const mine4 = slot4(walk.worker);
-        for (int c32 = half * (BN / 2); c32 < (half + 1) * (BN / 2); c32 += 32) {
-          float v[32];
-          load_d(d_tmem + c32, v);
-          if (row < p.M) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              __stcg(mine4 + (c32 / 4 + j) * 128, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
-          }
-        }
-        int h0, h1;
-        walk.holders(w.tile, h0, h1);
-        __threadfence();
-        fused_bar_any(false);
-        if (et == 0) {
-          uint32_t* counter = p.counters + w.tile * CG + cta_rank;
-          const bool last = atomicAdd(counter, 1u) == static_cast<uint32_t>(h1 - h0);
-          if (last) *counter = 0;    // ready for the next launch
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(last_slot), "r"(static_cast<uint32_t>(last)) : "memory");
-          __threadfence();
-        }
-        fused_bar_any(false);
-        uint32_t last;
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(last) : "r"(last_slot) : "memory");
-        if (last) {
-          __threadfence();
-          epilogue(c, half * kSlabs, 1, (half + 1) * kSlabs,
-                   [&](int tc, float (&v)[32]) {
-#pragma unroll
-                     for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-                     if (row >= p.M) return;
-                     for (int h = h0; h <= h1; ++h) {
-                       const float4* src = slot4(h) + (tc / 4) * 128;
-                       float4 x[8];
-#pragma unroll
-                       for (int j = 0; j < 8; ++j) x[j] = __ldcg(src + j * 128);
-#pragma unroll
-                       for (int j = 0; j < 8; ++j) {
-                         v[4 * j] += x[j].x; v[4 * j + 1] += x[j].y; v[4 * j + 2] += x[j].z; v[4 * j + 3] += x[j].w;
-                       }
-                     }
-                   },
-                   false, raw);
-        }
-      }
+      epilogue(c, half * kSlabs, 1, (half + 1) * kSlabs,
+               [&](int tc, float (&v)[32]) { load_d(d_tmem + tc, v); });
       tcgen05_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
@@ -768,23 +612,16 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   if constexpr (CG == 1) {
     if (split > 1) {
       // ---- the cluster's CTAs hold the tile's parts: each takes 1 / split of the result columns
-      FusedPiece w;
-      w.tile = static_cast<int>(blockIdx.x) / split;
-      const FusedTile c = fused_tile<Cfg::SYM>(w.tile, p.tiles_m, p.tiles_n, per_z);
+      const FusedTile c = fused_tile<Cfg::SYM>(worker, p.tiles_m, p.tiles_n, per_z);
       const int row = c.mb * Cfg::BM + quarter * 32 + lane;
       constexpr int kTileSlabs = (OP == kOpGate ? BN / 2 : BN) / 32;
       const int share = kTileSlabs / split;            // slabs of each CTA
-      bool fetched = false;
       const int my_first = static_cast<int>(cluster_rank) * share + half;
       if (epi) {
         grid_dependency_wait();
         if constexpr (Cfg::INPUTS > 0) {
           const int col = c.nb * BN + my_first * 32;
-          fetched = half < share && col < p.out_cols;
-          if (fetched) {
-#pragma unroll
-            for (int q = 0; q < Cfg::INPUTS; ++q) fetch(q, c, row, col, raw[q]);
-          }
+          if (half < share && col < p.out_cols) fetch(c, c.mb * Cfg::BM + quarter * 32, col);
         }
         epi_ok = __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(0), 0u, wc, kDevTimeoutTmemFull));
       }
@@ -847,8 +684,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
                        }
                      }
                    }
-                 },
-                 fetched, raw);
+                 });
       }
     }
   }

@@ -31,9 +31,7 @@ inline bool aligned16(const void* p, long long ld) {
 struct FusedContext {
   int device;
   FusedDevice dev;
-  float* ws;            // partial tiles
-  uint32_t* counters;
-  uint32_t* status;
+  uint32_t* status;     // device status word
 };
 int fused_context_create(FusedContext* c);    // on the current device; a roller_status
 void fused_context_destroy(FusedContext* c);
@@ -58,9 +56,6 @@ struct Product {
     p.tiles_per_z = c.tiles_per_z;
     p.zcount = z;
     p.split = c.split;
-    p.sk_tiles = c.sk_tiles;
-    p.ws = x.ws;
-    p.counters = x.counters;
     p.status = x.status;
     p.spin_limit = kSpinLimitCycles;
   }
@@ -91,6 +86,10 @@ struct Product {
     if (!aligned16(base, ld) || (z > 1 && (zs % 8 != 0 || zs < ld * p.M))) return ROLLER_OK;
     p.out_tma |= 1 << i;
     return encode_batch16(&p.o[i], base, p.out_cols, p.M, z, ld, zs, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, as_bf16);
+  }
+  // A matrix that the epilogue reads beside D.
+  int input(int i, const void* base, long long z, long long ld, long long zs) {
+    return encode_batch16(&p.i[i], base, p.out_cols, p.M, z, ld, zs, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, bf16);
   }
   // The mirror image of a symmetric output (always the library's own, aligned memory).
   int mirror(void* base, long long z, long long ld, long long zs) {

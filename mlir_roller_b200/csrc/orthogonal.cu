@@ -285,11 +285,7 @@ int roller_b200_ortho_run(roller_ortho_plan* p, const void* g, long long ld_g, l
       FUSED_OK(q.b_k(0, p->pm, m, m, Z, p->ldm, p->zsm));
       FUSED_OK(q.output(0, p->qm, Z, p->ldm, p->zsm, false));
       FUSED_OK(q.mirror(p->qm, Z, p->ldm, p->zsm));
-      q.p.in[0] = p->pm;
-      q.p.in_ld[0] = p->ldm;
-      q.p.in_zstride = p->zsm;
-      q.p.in_cols = static_cast<int>(p->ldm);
-      q.p.in_vec = 1;
+      FUSED_OK(q.input(0, p->pm, Z, p->ldm, p->zsm));
       q.p.vec = p->vec;
       q.p.vec_ld = static_cast<int>(p->ldm);
       q.p.coef_a = p->a;
@@ -306,12 +302,8 @@ int roller_b200_ortho_run(roller_ortho_plan* p, const void* g, long long ld_g, l
       FUSED_OK(u.a_k(p->qm, m, m, Z, p->ldm, p->zsm));
       FUSED_OK(u.b_mn(0, hi, C, R, Z, p->ldx, p->zsx));
     }
-    u.p.in[0] = hi;
-    u.p.in[1] = lo;
-    u.p.in_ld[0] = u.p.in_ld[1] = p->ldx;
-    u.p.in_zstride = p->zsx;
-    u.p.in_cols = static_cast<int>(p->ldx);
-    u.p.in_vec = 1;
+    FUSED_OK(u.input(0, hi, Z, p->ldx, p->zsx));
+    FUSED_OK(u.input(1, lo, Z, p->ldx, p->zsx));
     u.p.vec = p->vec;
     u.p.vec_ld = static_cast<int>(p->ldm);
     u.p.inv_scale = 1.0f / kScale;

@@ -68,9 +68,9 @@ class GatedFfnPlan:
         self._io = _lib.FfnIo()
 
     def new_saved(self, tokens: int):
-        """Two tensors for g and u, with rows that start on 16 bytes (the fast layout for odd d_ff)."""
+        """Two tensors for g and u, with rows that start on 32 bytes (the fast layout for any d_ff)."""
         import torch
-        ld = (self.d_ff + 7) // 8 * 8
+        ld = (self.d_ff + 15) // 16 * 16
         return tuple(torch.empty(tokens, ld, dtype=self.dtype, device=self.device)[:, :self.d_ff]
                      for _ in range(2))
 
