@@ -220,6 +220,18 @@ def _stream_ptr(stream) -> C.c_void_p:
     return C.c_void_p(getattr(stream, "cuda_stream", stream))
 
 
+def on_device(device, stream, fn, *args) -> int:
+    """fn(*args, stream) with `device` current; `stream` None is its current stream."""
+    import torch
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    ptr = C.c_void_p(getattr(stream, "cuda_stream", stream))
+    if torch.cuda.current_device() == device.index:
+        return fn(*args, ptr)
+    with torch.cuda.device(device):
+        return fn(*args, ptr)
+
+
 def gemm_static_scratch(tile: KTile, mode: int, M: int, N: int, K: int, lda: int, ldb: int,
                         ldc: int, a_ptr: int, b_ptr: int, c_ptr: int, status_ptr: int = 0,
                         stream=None) -> None:

@@ -18,7 +18,7 @@ struct TileCost {
   double kb_us;    // one k-block of one tile while every SM works
   double tile_us;  // fill and the last tile's epilogue
 };
-constexpr TileCost kTiles[] = {{2, 256, 0.36, 7.0}, {1, 256, 0.40, 6.0}, {1, 128, 0.28, 5.0}};
+constexpr TileCost kTiles[] = {{2, 256, 0.36, 7.0}, {1, 256, 0.40, 6.0}, {1, 128, 0.28, 4.5}};
 
 }  // namespace
 
@@ -77,16 +77,20 @@ static cudaError_t bind_device(FusedDevice* d) {
 
 // The kernels have the same inner loop, so a launch takes about (k-blocks the busiest worker gets)
 // x (their cost) + the fill and drain; the smallest estimate wins.
-//   * CTA pairs: the busiest worker gets ceil(tiles / workers) whole tiles. (Dealing the tiles that
-//     do not fill a last wave out along k was built and measured: writing and reading back the
+//   * whole tiles: the busiest CTA (or pair) gets ceil(tiles / workers) of them. (Dealing the tiles
+//     that do not fill a last wave out along k was built and measured: writing and reading back the
 //     fp32 sums of 256 x 256 tiles costs 15-25 us, more than an even share of k saves up to
 //     K = 8192.)
-//   * single CTAs, a cluster per tile: 1 / split of a tile's k-blocks per wave of clusters, and the
-//     exchange inside the cluster.
+//   * a cluster per tile: 1 / split of a tile's k-blocks per wave of clusters, and the exchange.
+// No launch is shorter than its operands' way from memory: with few rows this decides, and the
+// kernel with the smallest fixed cost that still has enough CTAs on the way wins.
 FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
   FusedChoice best = {};
   double best_us = 0.0;
   const bool sym = s.op == kOpGramWide || s.op == kOpGramTall || s.op == kOpPoly;
+  const double halves = s.op == kOpGate || s.op == kOpDx ? 2.0 : 1.0;
+  const double stream_us = halves * s.K * (s.op == kOpGate ? s.M / 2.0 + s.N : sym ? s.N : s.M + s.N) *
+                           (s.op == kOpDw ? 1 : s.zcount) * 2.0 / 6.2e6;
   for (const TileCost& c : kTiles) {
     const FusedVariant* kv = fused_find(s.op, c.cta_group, c.block_n, s.dt);
     if (!kv) continue;
@@ -95,35 +99,29 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
     const int bm = 128 * c.cta_group, bn = s.op == kOpGate ? c.block_n / 2 : c.block_n;
     f.tiles_m = static_cast<int>((s.M + bm - 1) / bm);
     f.tiles_n = static_cast<int>((s.N + bn - 1) / bn);
-    f.tiles_per_z = sym ? f.tiles_m * (f.tiles_m + 1) / 2 : f.tiles_m * f.tiles_n;
+    f.tiles_per_z = f.tiles_m * f.tiles_n;
+    if (sym) {   // `ratio` tile rows each have 1, 2, 3 .. tiles (fused_tile)
+      const int ratio = bn / bm, q = f.tiles_m / ratio;
+      f.tiles_per_z = ratio * q * (q + 1) / 2 + f.tiles_m % ratio * (q + 1);
+    }
     f.num_kb = static_cast<int>((s.K + 63) / 64);
     const int kbs = f.num_kb * (s.op == kOpDx ? 2 : 1);
     const long long tiles = static_cast<long long>(f.tiles_per_z) * s.zcount;
-    auto consider = [&](int split, long long grid, double us) {
-      if (best.kv && us >= best_us) return;
-      best_us = us;
-      best = f;
-      best.split = split;
-      best.grid = static_cast<int>(grid);
-    };
-    if (c.cta_group == 2) {
-      const int workers = d.clusters[1];
-      if (workers < 1) continue;
-      const long long waves = (tiles + workers - 1) / workers;
-      consider(1, 2 * (tiles < workers ? tiles : workers), waves * kbs * c.kb_us + c.tile_us);
-      continue;
-    }
-    for (int i = 0, split = 1; i < 4 && split <= kv->max_split && split <= kbs; ++i, split *= 2) {
-      const long long at_once = d.clusters[i];
+    for (int split = 1; split <= kv->max_split && split <= kbs; split *= 2) {
+      const int ctas = c.cta_group * split;                       // of a cluster
+      const long long at_once = d.clusters[ctas == 1 ? 0 : ctas == 2 ? 1 : ctas == 4 ? 2 : 3];
       if (at_once < 1) break;
       const long long waves = (tiles + at_once - 1) / at_once;
       const int part = (kbs + split - 1) / split;
-      if (split == 1) {
-        consider(1, tiles < at_once ? tiles : at_once, waves * part * c.kb_us + c.tile_us);
-      } else {
-        // a cluster has one tile: from the second wave on every tile pays for its own fill and drain
-        consider(split, tiles * split, waves * (part * c.kb_us + c.tile_us) + 1.5 + 0.2 * split);
-      }
+      // a cluster has one tile: from the second wave on every tile pays for its own fill and drain
+      const double fixed = c.tile_us + (split == 1 ? 0.0 : split == 2 ? 2.0 : split == 4 ? 2.5 : 5.0);
+      double us = split == 1 ? waves * part * c.kb_us + fixed : waves * (part * c.kb_us + fixed);
+      if (us < stream_us + fixed) us = stream_us + fixed;
+      if (best.kv && us >= best_us) continue;
+      best_us = us;
+      best = f;
+      best.split = split;
+      best.grid = static_cast<int>(split > 1 ? tiles : tiles < at_once ? tiles : at_once) * ctas;
     }
   }
   return best;

@@ -41,7 +41,7 @@ struct FusedParams {
   int num_kb;           // k-blocks of 64 (of each half in kOpDx)
   int a_bytes;          // bytes one TMA load of A brings (fewer rows than 128 on single CTAs)
   int tiles_m, tiles_n, tiles_per_z, zcount;
-  int split;            // single CTAs: cluster size, CTAs that share a tile's k (1 = none)
+  int split;            // parts of a cluster that share a tile's k (1 = none)
   int b_early;          // the second operand may be read before the previous kernel is done
   int act;
   int flags;

@@ -23,8 +23,8 @@
 // one triangle of a symmetric product is computed.
 //
 // With few rows or columns there are few tiles, and a weight has to be streamed by all SMs to come
-// at the memory's rate. Single CTAs therefore also run in clusters of 2, 4 or 8 that share one
-// tile: each takes a part of k, and at the end each collects the others' sums of its share of
+// at the memory's rate. CTAs (or pairs) therefore also run in clusters of up to 8 CTAs that share
+// one tile: each takes a part of k, and at the end each collects the others' sums of its share of
 // the columns through distributed shared memory (the ring's, which is free by then), adds them in the
 // order of k and runs the epilogue on its share. Results do not depend on timing.
 //
@@ -80,10 +80,18 @@ struct FusedCfg {
   static constexpr int FIRST_EPI_WARP = 4;
   static constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
   static_assert(BN == 256 || BN == 128, "tile widths");
-  static_assert(!SYM || TILE_M == BN, "one triangle of square tiles");
-  // a cluster's exchange of partial sums: at most 128 rows x BN columns, in the ring's memory
-  static constexpr int MAX_SPLIT = CG == 2 ? 1 : (OP == kOpGate ? BN / 64 : BN / 32);
-  static_assert(CG == 2 || STAGES * STAGE_BYTES >= 128 * BN * 4, "exchange area");
+  static constexpr int SYM_RATIO = BN / TILE_M;      // tile rows per tile column of a triangle
+  static_assert(!SYM || SYM_RATIO == 1 || SYM_RATIO == 2, "triangle of tiles");
+  // The exchange of partial sums in a splitting cluster goes through the ring's memory: each CTA
+  // receives its share of the columns of 128 rows from every other part. (With more parts than
+  // slabs of 32 columns, some only give.)
+  static constexpr int SLABS = (OP == kOpGate ? BN / 2 : BN) / 32;
+  static constexpr int MAX_SPLIT = CG == 2 ? (OP == kOpGate ? 2 : 4) : OP == kOpGate ? 4 : 8;
+  static constexpr int exchange_bytes(int split) {
+    return (split - 1) * (SLABS > split ? SLABS / split : 1) * (OP == kOpGate ? 2 : 1) * 16384;
+  }
+  static_assert(exchange_bytes(MAX_SPLIT) <= STAGES * STAGE_BYTES && exchange_bytes(2) <= STAGES * STAGE_BYTES,
+                "exchange area");
   static_assert(STAGES >= 3 && SMEM_BYTES <= SMEM_LIMIT, "shared memory");
 };
 
@@ -131,18 +139,21 @@ struct FusedTile {
 };
 
 // Tile order. Rectangular problems: panels of 8 tile rows, so that the tiles in flight share
-// operand rows and columns in L2. Symmetric ones: the lower triangle, row by row.
-template <bool SYM>
+// operand rows and columns in L2. Symmetric ones: the tiles that touch the lower triangle, row by
+// row (RATIO tile rows to a tile column; 0 = not symmetric).
+template <int RATIO>
 __device__ __forceinline__ FusedTile fused_tile(int t, int tiles_m, int tiles_n, int per_z) {
   FusedTile c;
   c.z = t / per_z;
   int r = t - c.z * per_z;
-  if constexpr (SYM) {
-    int i = static_cast<int>((sqrtf(8.0f * static_cast<float>(r) + 1.0f) - 1.0f) * 0.5f);
-    while (i * (i + 1) / 2 > r) --i;
-    while ((i + 1) * (i + 2) / 2 <= r) ++i;
-    c.mb = i;
-    c.nb = r - i * (i + 1) / 2;
+  if constexpr (RATIO > 0) {
+    // RATIO rows have q + 1 tiles each, RATIO q (q + 1) / 2 tiles come before them
+    int q = static_cast<int>((sqrtf(8.0f / RATIO * static_cast<float>(r) + 1.0f) - 1.0f) * 0.5f);
+    while (RATIO * q * (q + 1) / 2 > r) --q;
+    while (RATIO * (q + 1) * (q + 2) / 2 <= r) ++q;
+    r -= RATIO * q * (q + 1) / 2;
+    c.mb = RATIO * q + r / (q + 1);
+    c.nb = r % (q + 1);
   } else {
     constexpr int kPanel = 8;
     const int per_panel = kPanel * tiles_n;
@@ -197,10 +208,12 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  // a cluster is either a CTA pair (one tile of 256 rows) or `split` CTAs sharing one tile's k
-  const int split = CG == 2 ? 1 : p.split;
+  // a cluster holds the `split` parts of one tile's k, each a CTA or a pair (ranks 2i and 2i + 1)
+  const int split = p.split;
   const uint32_t cluster_rank = (CG == 2 || split > 1) ? cluster_ctarank() : 0u;
-  const uint32_t cta_rank = CG == 2 ? cluster_rank : 0u;
+  const uint32_t cta_rank = CG == 2 ? (cluster_rank & 1u) : 0u;
+  const uint32_t part = cluster_rank / CG;
+  const uint32_t leader_rank = cluster_rank - cta_rank;
   const bool is_leader = (cta_rank == 0);
 
   if (threadIdx.x == 0) {
@@ -235,11 +248,10 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   const int total_kb = p.num_kb * (OP == kOpDx ? 2 : 1);
   // Tiles go round-robin to the CTAs, pairs or clusters; a CTA of a splitting cluster takes its part
   // of k, and its cluster has exactly one tile.
-  const int per_worker = CG == 2 ? 2 : split;
-  const int workers = static_cast<int>(gridDim.x) / per_worker;
-  const int worker = static_cast<int>(blockIdx.x) / per_worker;
-  const int kb0 = static_cast<int>(static_cast<long long>(total_kb) * (cluster_rank - cta_rank) / split);
-  const int kb1 = static_cast<int>(static_cast<long long>(total_kb) * (cluster_rank - cta_rank + 1) / split);
+  const int workers = static_cast<int>(gridDim.x) / (CG * split);
+  const int worker = static_cast<int>(blockIdx.x) / (CG * split);
+  const int kb0 = static_cast<int>(static_cast<long long>(total_kb) * part / split);
+  const int kb1 = static_cast<int>(static_cast<long long>(total_kb) * (part + 1) / split);
 
   bool epi_ok = true;
 
@@ -275,7 +287,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     auto arm = [&](int s) {
       if constexpr (CG == 2) {
         if (is_leader) mbar_expect_tx(full_bar(s), 2 * (Cfg::A_BYTES + Cfg::B_BYTES));
-        return map_to_cta(full_bar(s), 0);
+        return map_to_cta(full_bar(s), leader_rank);
       } else {
         mbar_expect_tx(full_bar(s), p.a_bytes + Cfg::B_BYTES);
         return full_bar(s);
@@ -285,7 +297,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     uint32_t ph = 0;
     bool ok = true;
     for (int t = worker; ok && t < tiles; t += workers) {
-      const FusedTile c = fused_tile<Cfg::SYM>(t, p.tiles_m, p.tiles_n, per_z);
+      const FusedTile c = fused_tile<Cfg::SYM ? Cfg::SYM_RATIO : 0>(t, p.tiles_m, p.tiles_n, per_z);
       int kb = kb0;
       if (t == worker) {
         const int early = p.b_early ? min(STAGES, kb1 - kb0) : 0;
@@ -293,7 +305,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
         grid_dependency_wait();
         grid_launch_dependents();
         for (int i = 0; i < early; ++i)
-          load_a(i, CG == 2 ? map_to_cta(full_bar(i), 0) : full_bar(i), c, kb + i);
+          load_a(i, CG == 2 ? map_to_cta(full_bar(i), leader_rank) : full_bar(i), c, kb + i);
         kb += early;
         s = early;
         if (s == STAGES) { s = 0; ph ^= 1u; }
@@ -335,15 +347,15 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
           umma_f16<CG>(d_tmem, a + kk * a_step, b + kk * b_step, idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
-        umma_commit<CG>(empty_bar(s));
+        umma_commit_to<CG>(empty_bar(s), leader_rank);
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
-      if (ok) umma_commit<CG>(tmem_full_bar(acc));
+      if (ok) umma_commit_to<CG>(tmem_full_bar(acc), leader_rank);
       acc ^= 1;
       if (acc == 0) acc_ph ^= 1u;
     }
     // whatever was issued has to complete before tensor and shared memory are given up
-    umma_commit<CG>(mma_done_bar);
+    umma_commit_to<CG>(mma_done_bar, leader_rank);
     mbar_wait_drain(mma_done_bar, 0u, p.spin_limit);
   }
 
@@ -459,6 +471,9 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     }
   };
 
+  // Whether a slab has anything to do (it decides whether inputs are sent for).
+  auto wanted = [&](int row0, int col) { return col < p.out_cols && (!Cfg::SYM || col <= row0); };
+
   // The epilogue of this warp's slabs slab0, slab0 + step, .. < slab_end of tile `c`. Slab i is the 32
   // result columns from tile column 32 i on; `sums(tile_col, v)` gives 32 columns of D.
   // The first slab's inputs have been sent for.
@@ -471,13 +486,14 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
 #pragma unroll 1
       for (int i = slab0; i < slab_end; i += step) {
         const int tc = i * 32, col = col_base + tc;
-        if (col >= p.out_cols) break;     // (uniform over the warp)
+        // (uniform over the warp; above the diagonal a slab is the mirror image of another one)
+        if (!wanted(row0, col)) break;
         float v[32];
         uint32_t raw[Cfg::INPUTS ? Cfg::INPUTS : 1][16];
         if constexpr (Cfg::INPUTS > 0) {
           epi_ok = take(raw) && epi_ok;
           // the next slab's inputs are on their way while this one is worked on
-          if (i + step < slab_end && col + step * 32 < p.out_cols) fetch(c, row0, col + step * 32);
+          if (i + step < slab_end && wanted(row0, col + step * 32)) fetch(c, row0, col + step * 32);
         }
         auto input = [&](int q, int k) {      // element k of input q
           const float2 f = fused_unpack<DT>(raw[q][k / 2]);
@@ -548,7 +564,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
             for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
           }
           emit(0, c, row0, col, v, false);
-          if (c.mb != c.nb) emit_mirror(c, row0, col, v);
+          if (col < row0) emit_mirror(c, row0, col, v);
         } else {
           sums(tc, v);
           const float dr = (OP == kOpUpdateWide && row < p.M) ? p.vec[c.z * p.vec_ld + row] : 0.0f;
@@ -587,10 +603,11 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     int acc = 0;
     uint32_t acc_ph = 0;
     for (int t = worker; epi_ok && t < tiles; t += workers) {
-      const FusedTile c = fused_tile<Cfg::SYM>(t, p.tiles_m, p.tiles_n, per_z);
+      const FusedTile c = fused_tile<Cfg::SYM ? Cfg::SYM_RATIO : 0>(t, p.tiles_m, p.tiles_n, per_z);
       if constexpr (Cfg::INPUTS > 0) {     // they do not depend on the product
         const int col = c.nb * BN + half * Cfg::OUT_COLS;
-        if (col < p.out_cols) fetch(c, (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32, col);
+        const int row0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32;
+        if (wanted(row0, col)) fetch(c, row0, col);
       }
       epi_ok = __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(acc), acc_ph, wc, kDevTimeoutTmemFull));
       if (!epi_ok) break;
@@ -601,7 +618,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
       tcgen05_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CG == 2) mbar_arrive_cluster(tmem_empty_bar(acc), 0);
+        if constexpr (CG == 2) mbar_arrive_cluster(tmem_empty_bar(acc), leader_rank);
         else mbar_arrive(tmem_empty_bar(acc));
       }
       acc ^= 1;
@@ -609,83 +626,83 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     }
   }
 
-  if constexpr (CG == 1) {
-    if (split > 1) {
-      // ---- the cluster's CTAs hold the tile's parts: each takes 1 / split of the result columns
-      const FusedTile c = fused_tile<Cfg::SYM>(worker, p.tiles_m, p.tiles_n, per_z);
-      const int row = c.mb * Cfg::BM + quarter * 32 + lane;
-      constexpr int kTileSlabs = (OP == kOpGate ? BN / 2 : BN) / 32;
-      const int share = kTileSlabs / split;            // slabs of each CTA
-      const int my_first = static_cast<int>(cluster_rank) * share + half;
-      if (epi) {
-        grid_dependency_wait();
-        if constexpr (Cfg::INPUTS > 0) {
-          const int col = c.nb * BN + my_first * 32;
-          if (half < share && col < p.out_cols) fetch(c, c.mb * Cfg::BM + quarter * 32, col);
-        }
-        epi_ok = __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(0), 0u, wc, kDevTimeoutTmemFull));
+  if (split > 1) {
+    // ---- the cluster holds the tile's parts: their sums are put together, each CTA taking a share
+    // of the slabs: slab i is received by part i / share, or by every `apart`-th part
+    const FusedTile c = fused_tile<Cfg::SYM ? Cfg::SYM_RATIO : 0>(worker, p.tiles_m, p.tiles_n, per_z);
+    const int row0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32;
+    const bool row_ok = row0 + lane < p.M;
+    const int share = max(Cfg::SLABS / split, 1), apart = max(split / Cfg::SLABS, 1);
+    const int my_slab = static_cast<int>(part) / apart * share;
+    const bool receives = static_cast<int>(part) % apart == 0 && half < share;
+    if (epi) {
+      grid_dependency_wait();
+      if constexpr (Cfg::INPUTS > 0) {
+        const int col = c.nb * BN + (my_slab + half) * 32;
+        if (receives && wanted(row0, col)) fetch(c, row0, col);
       }
-      __syncwarp();
-      cluster_sync();      // all MMAs of the cluster are done: the rings' memory is free
-      // Exchange area of a CTA: [sender][32-column group][4 columns][row] float4. A share of the gate's
-      // columns has two groups per slab (g, then u).
-      constexpr int kGroups = OP == kOpGate ? 2 : 1;
-      const uint32_t sender_bytes = static_cast<uint32_t>(share * kGroups) * 16384u;
-      const uint32_t lane_at = static_cast<uint32_t>(quarter * 32 + lane) * 16u;
-      if (epi && epi_ok) {
-        tcgen05_fence_after_sync();
-        for (int i = half; i < kTileSlabs; i += 2) {
-          const uint32_t to = static_cast<uint32_t>(i / share);
-          if (to == cluster_rank) continue;
-          // senders in the order of k, the receiver itself left out
-          const uint32_t place = cluster_rank - (cluster_rank > to ? 1u : 0u);
+      epi_ok = __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(0), 0u, wc, kDevTimeoutTmemFull));
+    }
+    __syncwarp();
+    cluster_sync();      // all MMAs of the cluster are done: the rings' memory is free
+    // Exchange area of a CTA: [sender][32-column group][4 columns][row] float4. The gate has two
+    // groups per slab (g, then u).
+    constexpr int kGroups = OP == kOpGate ? 2 : 1;
+    const uint32_t sender_bytes = static_cast<uint32_t>(share * kGroups) * 16384u;
+    const uint32_t lane_at = static_cast<uint32_t>(quarter * 32 + lane) * 16u;
+    if (epi && epi_ok) {
+      tcgen05_fence_after_sync();
+      for (int i = half; i < Cfg::SLABS; i += 2) {
+        const uint32_t to = static_cast<uint32_t>(i / share * apart);
+        if (to == part) continue;
+        // senders in the order of k, the receiver itself left out
+        const uint32_t place = part - (part > to ? 1u : 0u);
 #pragma unroll
-          for (int q = 0; q < kGroups; ++q) {
-            float v[32];
-            load_d(tmem_base + tmem_lane + i * 32 + q * (BN / 2), v);
-            if (row < p.M) {
-              const uint32_t dst = map_to_cta(
-                  smem_base + place * sender_bytes + static_cast<uint32_t>((i % share) * kGroups + q) * 16384u + lane_at, to);
+        for (int q = 0; q < kGroups; ++q) {
+          float v[32];
+          load_d(tmem_base + tmem_lane + i * 32 + q * (BN / 2), v);
+          if (row_ok) {
+            const uint32_t dst = map_to_cta(
+                smem_base + place * sender_bytes + static_cast<uint32_t>((i % share) * kGroups + q) * 16384u + lane_at,
+                to * CG + cta_rank);
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + j * 2048u),
-                             "f"(v[4 * j]), "f"(v[4 * j + 1]), "f"(v[4 * j + 2]), "f"(v[4 * j + 3])
-                             : "memory");
-            }
+            for (int j = 0; j < 8; ++j)
+              asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + j * 2048u),
+                           "f"(v[4 * j]), "f"(v[4 * j + 1]), "f"(v[4 * j + 2]), "f"(v[4 * j + 3])
+                           : "memory");
           }
         }
       }
-      __syncwarp();
-      cluster_sync();
-      if (epi && epi_ok && half < share) {
-        epilogue(c, my_first, 2, (static_cast<int>(cluster_rank) + 1) * share,
-                 [&](int tc, float (&v)[32]) {
-                   const int q = (OP == kOpGate && tc >= BN / 2) ? 1 : 0;
-                   const int i = (tc - q * (BN / 2)) / 32 - static_cast<int>(cluster_rank) * share;
-                   float own[32];
-                   load_d(tmem_base + tmem_lane + tc, own);
+    }
+    __syncwarp();
+    cluster_sync();
+    if (epi && epi_ok && receives) {
+      epilogue(c, my_slab + half, 2, my_slab + share, [&](int tc, float (&v)[32]) {
+        const int q = (OP == kOpGate && tc >= BN / 2) ? 1 : 0;
+        const int i = (tc - q * (BN / 2)) / 32 - my_slab;
+        float own[32];
+        load_d(tmem_base + tmem_lane + tc, own);
 #pragma unroll
-                   for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-                   for (int r = 0; r < split; ++r) {
-                     if (r == static_cast<int>(cluster_rank)) {
+        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+        for (int r = 0; r < split; ++r) {
+          if (r == static_cast<int>(part)) {
 #pragma unroll
-                       for (int j = 0; j < 32; ++j) v[j] += own[j];
-                     } else if (row < p.M) {
-                       const uint32_t src = smem_base + static_cast<uint32_t>(r - (r > static_cast<int>(cluster_rank) ? 1 : 0)) * sender_bytes +
-                                            static_cast<uint32_t>(i * kGroups + q) * 16384u + lane_at;
+            for (int j = 0; j < 32; ++j) v[j] += own[j];
+          } else if (row_ok) {
+            const uint32_t src = smem_base + static_cast<uint32_t>(r - (r > static_cast<int>(part) ? 1 : 0)) * sender_bytes +
+                                 static_cast<uint32_t>(i * kGroups + q) * 16384u + lane_at;
 #pragma unroll
-                       for (int j = 0; j < 8; ++j) {
-                         float4 x;
-                         asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                      : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
-                                      : "r"(src + j * 2048u)
-                                      : "memory");
-                         v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
-                       }
-                     }
-                   }
-                 });
-      }
+            for (int j = 0; j < 8; ++j) {
+              float4 x;
+              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                           : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                           : "r"(src + j * 2048u)
+                           : "memory");
+              v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
+            }
+          }
+        }
+      });
     }
   }
 

@@ -14,7 +14,7 @@ static cudaError_t fused_launch(const FusedParams& p, int grid, cudaStream_t str
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(Cfg::CG == 2 ? 2 : p.split);
+  attr[0].val.clusterDim.x = static_cast<unsigned>(Cfg::CG * p.split);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   // scheduled while the previous kernel of the stream winds down; the kernel waits for that
@@ -35,7 +35,7 @@ static FusedVariant fused_make() {
   v.block_n = BN;
   v.dt = DT;
   v.threads = Cfg::THREADS;
-  v.max_split = Cfg::MAX_SPLIT < 8 ? Cfg::MAX_SPLIT : 8;
+  v.max_split = Cfg::MAX_SPLIT;
   v.smem_bytes = Cfg::SMEM_BYTES;
   v.func = reinterpret_cast<const void*>(&fused_gemm_kernel<Cfg>);
   v.launch = &fused_launch<Cfg>;
@@ -50,7 +50,7 @@ static const FusedVariant* fused_ffn_table(int* n) {
       fused_make<kOpGate, 2, 256, DT>(), fused_make<kOpGate, 1, 256, DT>(), fused_make<kOpGate, 1, 128, DT>(),
       fused_make<kOpDown, 2, 256, DT>(), fused_make<kOpDown, 1, 256, DT>(), fused_make<kOpDown, 1, 128, DT>(),
       fused_make<kOpDact, 2, 256, DT>(), fused_make<kOpDact, 1, 128, DT>(),
-      fused_make<kOpDx, 2, 256, DT>(),   fused_make<kOpDx, 1, 128, DT>(),
+      fused_make<kOpDx, 2, 256, DT>(),   fused_make<kOpDx, 1, 256, DT>(), fused_make<kOpDx, 1, 128, DT>(),
       fused_make<kOpDw, 2, 256, DT>(),   fused_make<kOpDw, 1, 128, DT>(),
   };
   *n = static_cast<int>(sizeof(t) / sizeof(t[0]));

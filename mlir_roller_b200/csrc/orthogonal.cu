@@ -27,7 +27,7 @@ using namespace rb200;
 namespace {
 
 constexpr float kScale = 1024.0f;   // S
-constexpr int kSumBlocks = 296;     // blocks of the norm per matrix, at most
+constexpr int kSumBlocks = 1184;    // blocks of the norm per matrix, at most
 constexpr int kMaxSide = 65536, kMaxShort = 16384, kMaxBatch = 4096;
 
 template <typename T>
@@ -72,6 +72,7 @@ __global__ void __launch_bounds__(256) ortho_sumsq(Source s, double* __restrict_
   double sum = 0.0;
   for (long long r = static_cast<long long>(blockIdx.x) * ty + y; r < s.rows; r += static_cast<long long>(gridDim.x) * ty) {
     const T* row = g + r * s.ld;
+#pragma unroll 4
     for (int c = x * 8; c < s.cols; c += s.tx * 8) {
       float v[8];
       load8(row, c, s.cols, s.vec, v);
@@ -112,6 +113,7 @@ ortho_scale(Source s, const double* __restrict__ part, int parts, double eps, __
   for (long long r = static_cast<long long>(blockIdx.x) * ty + y; r < s.rows; r += static_cast<long long>(gridDim.x) * ty) {
     const T* row = g + r * s.ld;
     const long long at = blockIdx.y * zsx + r * ldx;
+#pragma unroll 2
     for (int c = x * 8; c < s.cols; c += s.tx * 8) {
       float v[8];
       load8(row, c, s.cols, s.vec, v);
@@ -134,7 +136,7 @@ int convert(const Source& s, int batch, int blocks, double* part, double eps, __
   const dim3 sums(static_cast<unsigned>(blocks < kSumBlocks ? blocks : kSumBlocks), static_cast<unsigned>(batch));
   ortho_sumsq<T><<<sums, 256, 0, st>>>(s, part);
   FUSED_CUDA(cudaGetLastError());
-  const dim3 grid(static_cast<unsigned>(blocks < 4 * kSumBlocks ? blocks : 4 * kSumBlocks), static_cast<unsigned>(batch));
+  const dim3 grid(static_cast<unsigned>(blocks < kSumBlocks ? blocks : kSumBlocks), static_cast<unsigned>(batch));
   ortho_scale<T><<<grid, 256, 0, st>>>(s, part, static_cast<int>(sums.x), eps, hi, lo, ldx, zsx);
   FUSED_CUDA(cudaGetLastError());
   return ROLLER_OK;
@@ -163,7 +165,74 @@ struct roller_ortho_plan {
   __half* x[2][2];         // [which][hi, lo], [batch][rows][ldx]
   __half *pm, *qm;         // p and q, [batch][m][ldm]
   float* vec;              // [batch][ldm]
+  // The launches of a step, built once: everything they touch is the plan's own, but for the last
+  // step's output. [which x] reads x[which] and writes the other.
+  Product *gram[2], *poly, *update[2], *last[2];
 };
+
+namespace {
+
+// Tensor maps and parameters of the plan's launches.
+int build_products(roller_ortho_plan* p) {
+  const int R = p->rows, C = p->cols, Z = p->batch, m = p->m, n = p->n;
+  for (int w = 0; w < 2; ++w) {
+    __half *hi = p->x[w][0], *lo = p->x[w][1];
+    p->gram[w] = new (std::nothrow) Product(p->ctx, p->tall ? kOpGramTall : kOpGramWide, 2, m, m, n, Z);
+    if (!p->gram[w]) return ROLLER_ERR_NOMEM;
+    Product& g = *p->gram[w];
+    if (p->tall) {
+      FUSED_OK(g.a_mn(hi, C, R, Z, p->ldx, p->zsx));
+      FUSED_OK(g.b_mn(0, hi, C, R, Z, p->ldx, p->zsx));
+    } else {
+      FUSED_OK(g.a_k(hi, C, R, Z, p->ldx, p->zsx));
+      FUSED_OK(g.b_k(0, hi, C, R, Z, p->ldx, p->zsx));
+    }
+    FUSED_OK(g.output(0, p->pm, Z, p->ldm, p->zsm, false));
+    FUSED_OK(g.mirror(p->pm, Z, p->ldm, p->zsm));
+    g.p.inv_scale = 1.0f / kScale;
+    for (int final_step = 0; final_step < 2; ++final_step) {
+      Product*& slot = final_step ? p->last[w] : p->update[w];
+      slot = new (std::nothrow) Product(p->ctx, p->tall ? kOpUpdateTall : kOpUpdateWide, 2, R, C, m, Z);
+      if (!slot) return ROLLER_ERR_NOMEM;
+      Product& u = *slot;
+      if (p->tall) {
+        FUSED_OK(u.a_k(hi, C, R, Z, p->ldx, p->zsx));
+        FUSED_OK(u.b_k(0, p->qm, m, m, Z, p->ldm, p->zsm));
+      } else {
+        FUSED_OK(u.a_k(p->qm, m, m, Z, p->ldm, p->zsm));
+        FUSED_OK(u.b_mn(0, hi, C, R, Z, p->ldx, p->zsx));
+      }
+      FUSED_OK(u.input(0, hi, Z, p->ldx, p->zsx));
+      FUSED_OK(u.input(1, lo, Z, p->ldx, p->zsx));
+      u.p.vec = p->vec;
+      u.p.vec_ld = static_cast<int>(p->ldm);
+      u.p.inv_scale = 1.0f / kScale;
+      if (final_step) {
+        u.p.flags |= kFusedLast;      // (its output is set by each call)
+      } else {
+        FUSED_OK(u.output(0, p->x[1 - w][0], Z, p->ldx, p->zsx, false));
+        FUSED_OK(u.output(1, p->x[1 - w][1], Z, p->ldx, p->zsx, false));
+      }
+    }
+  }
+  p->poly = new (std::nothrow) Product(p->ctx, kOpPoly, 2, m, m, m, Z);
+  if (!p->poly) return ROLLER_ERR_NOMEM;
+  Product& q = *p->poly;
+  FUSED_OK(q.a_k(p->pm, m, m, Z, p->ldm, p->zsm));
+  FUSED_OK(q.b_k(0, p->pm, m, m, Z, p->ldm, p->zsm));
+  FUSED_OK(q.input(0, p->pm, Z, p->ldm, p->zsm));
+  FUSED_OK(q.output(0, p->qm, Z, p->ldm, p->zsm, false));
+  FUSED_OK(q.mirror(p->qm, Z, p->ldm, p->zsm));
+  q.p.vec = p->vec;
+  q.p.vec_ld = static_cast<int>(p->ldm);
+  q.p.coef_a = p->a;
+  q.p.coef_b = p->b;
+  q.p.coef_c = p->c / kScale;
+  q.p.inv_scale = 1.0f / kScale;
+  return ROLLER_OK;
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -221,6 +290,11 @@ int roller_b200_ortho_create(int batch, int rows, int cols, int in_type, int ste
     roller_b200_ortho_destroy(p);
     return failed;
   }
+  const int built = build_products(p);
+  if (built != ROLLER_OK) {
+    roller_b200_ortho_destroy(p);
+    return built;
+  }
   *out = p;
   return ROLLER_OK;
 }
@@ -262,58 +336,16 @@ int roller_b200_ortho_run(roller_ortho_plan* p, const void* g, long long ld_g, l
   else
     FUSED_OK(convert<__half>(s, p->batch, blocks, p->part, p->eps, p->x[0][0], p->x[0][1], p->ldx, p->zsx, st));
 
-  const int R = p->rows, C = p->cols, Z = p->batch, m = p->m, n = p->n;
   for (int i = 0; i < p->steps; ++i) {
-    __half *hi = p->x[i & 1][0], *lo = p->x[i & 1][1];
-    {
-      Product q(p->ctx, p->tall ? kOpGramTall : kOpGramWide, 2, m, m, n, Z);
-      if (p->tall) {
-        FUSED_OK(q.a_mn(hi, C, R, Z, p->ldx, p->zsx));
-        FUSED_OK(q.b_mn(0, hi, C, R, Z, p->ldx, p->zsx));
-      } else {
-        FUSED_OK(q.a_k(hi, C, R, Z, p->ldx, p->zsx));
-        FUSED_OK(q.b_k(0, hi, C, R, Z, p->ldx, p->zsx));
-      }
-      FUSED_OK(q.output(0, p->pm, Z, p->ldm, p->zsm, false));
-      FUSED_OK(q.mirror(p->pm, Z, p->ldm, p->zsm));
-      q.p.inv_scale = 1.0f / kScale;
-      FUSED_OK(q.launch(st));
+    const int w = i & 1;
+    FUSED_OK(p->gram[w]->launch(st));
+    FUSED_OK(p->poly->launch(st));
+    if (i + 1 < p->steps) {
+      FUSED_OK(p->update[w]->launch(st));
+      continue;
     }
-    {
-      Product q(p->ctx, kOpPoly, 2, m, m, m, Z);
-      FUSED_OK(q.a_k(p->pm, m, m, Z, p->ldm, p->zsm));
-      FUSED_OK(q.b_k(0, p->pm, m, m, Z, p->ldm, p->zsm));
-      FUSED_OK(q.output(0, p->qm, Z, p->ldm, p->zsm, false));
-      FUSED_OK(q.mirror(p->qm, Z, p->ldm, p->zsm));
-      FUSED_OK(q.input(0, p->pm, Z, p->ldm, p->zsm));
-      q.p.vec = p->vec;
-      q.p.vec_ld = static_cast<int>(p->ldm);
-      q.p.coef_a = p->a;
-      q.p.coef_b = p->b;
-      q.p.coef_c = p->c / kScale;
-      q.p.inv_scale = 1.0f / kScale;
-      FUSED_OK(q.launch(st));
-    }
-    Product u(p->ctx, p->tall ? kOpUpdateTall : kOpUpdateWide, 2, R, C, m, Z);
-    if (p->tall) {
-      FUSED_OK(u.a_k(hi, C, R, Z, p->ldx, p->zsx));
-      FUSED_OK(u.b_k(0, p->qm, m, m, Z, p->ldm, p->zsm));
-    } else {
-      FUSED_OK(u.a_k(p->qm, m, m, Z, p->ldm, p->zsm));
-      FUSED_OK(u.b_mn(0, hi, C, R, Z, p->ldx, p->zsx));
-    }
-    FUSED_OK(u.input(0, hi, Z, p->ldx, p->zsx));
-    FUSED_OK(u.input(1, lo, Z, p->ldx, p->zsx));
-    u.p.vec = p->vec;
-    u.p.vec_ld = static_cast<int>(p->ldm);
-    u.p.inv_scale = 1.0f / kScale;
-    if (i + 1 == p->steps) {
-      u.p.flags |= kFusedLast;
-      FUSED_OK(u.output(0, out, Z, ld_out, zs_out, true));
-    } else {
-      FUSED_OK(u.output(0, p->x[~i & 1][0], Z, p->ldx, p->zsx, false));
-      FUSED_OK(u.output(1, p->x[~i & 1][1], Z, p->ldx, p->zsx, false));
-    }
+    Product u = *p->last[w];
+    FUSED_OK(u.output(0, out, p->batch, ld_out, zs_out, true));
     FUSED_OK(u.launch(st));
   }
   return ROLLER_OK;
@@ -326,6 +358,7 @@ int roller_b200_ortho_status(roller_ortho_plan* p, uint32_t* device_status) {
 
 int roller_b200_ortho_destroy(roller_ortho_plan* p) {
   if (!p) return ROLLER_OK;
+  for (Product* q : {p->gram[0], p->gram[1], p->poly, p->update[0], p->update[1], p->last[0], p->last[1]}) delete q;
   cudaFree(p->part);
   for (auto& pair : p->x)
     for (__half* b : pair) cudaFree(b);

@@ -406,4 +406,20 @@ __device__ __forceinline__ void umma_commit(uint32_t bar) {
   }
 }
 
+// The same for a pair anywhere in its cluster: the arrival goes to the barrier at the same offset in
+// the CTAs leader_rank and leader_rank + 1.
+template <int kCtaGroup>
+__device__ __forceinline__ void umma_commit_to(uint32_t bar, uint32_t leader_rank) {
+  if constexpr (kCtaGroup == 1) {
+    umma_commit<1>(bar);
+  } else {
+    const uint16_t mask = static_cast<uint16_t>(0x3u << leader_rank);
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(bar),
+        "h"(mask)
+        : "memory");
+  }
+}
+
 }  // namespace rb200

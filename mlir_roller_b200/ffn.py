@@ -20,19 +20,24 @@ epilogue (src/roller.py:47-68).
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import _lib
+
+# roller_ffn_io: the number of tokens (padded to eight bytes), then twelve bases and row strides
+_IO = struct.Struct("@i4x" + 12 * "Pq")
+_NONE = 12 * (("", None, 0, 0),)
 
 ACTIVATIONS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
 
 
 def check_matrix(t, name: str, dtype, device, rows: int, cols: int) -> int:
     """Row stride of a 2-D tensor after checking its type, device, shape and order."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} is {t.dtype}, this plan needs {dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, this plan is bound to {device}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+    if t.shape != (rows, cols):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({rows}, {cols})")
     ld, step = t.stride()
     if cols > 1 and step != 1:
@@ -74,58 +79,43 @@ class GatedFfnPlan:
         return tuple(torch.empty(tokens, ld, dtype=self.dtype, device=self.device)[:, :self.d_ff]
                      for _ in range(2))
 
-    def _set(self, t, name: str, rows: int, cols: int) -> None:
-        m = getattr(self._io, name)
-        if t is None:
-            m.ptr, m.ld = None, 0
-            return
-        m.ld = check_matrix(t, name, self.dtype, self.device, rows, cols)
-        m.ptr = t.data_ptr()
-
-    def _call(self, fn, name: str, stream) -> None:
-        import torch
+    def _call(self, fn, name: str, tokens: int, mats, stream) -> None:
+        """`mats`: (name, tensor or None, rows, cols) in the order of roller_ffn_io."""
         if not self._h:
             raise RuntimeError("the plan has been destroyed")
-        with torch.cuda.device(self.device):
-            if stream is None:
-                stream = torch.cuda.current_stream()
-            _lib.check(fn(self._h, C.byref(self._io), C.c_void_p(getattr(stream, "cuda_stream", stream))), name)
+        words = [tokens]
+        for what, t, rows, cols in mats:
+            if t is None:
+                words += (0, 0)
+                continue
+            ld = check_matrix(t, what, self.dtype, self.device, rows, cols)
+            words += (t.data_ptr(), ld)
+        _IO.pack_into(self._io, 0, *words)
+        _lib.check(_lib.on_device(self.device, stream, fn, self._h, C.byref(self._io)), name)
 
-    def _operands(self, x, wg, wu, wd) -> int:
+    def _tokens(self, x) -> int:
         tokens = x.shape[0]
         if tokens > self.max_tokens:
             raise _lib.RollerError(_lib.ERR_TOO_LARGE, f"{tokens} tokens, the plan was made for {self.max_tokens}")
-        d, f = self.d_model, self.d_ff
-        self._io.tokens = tokens
-        self._set(x, "x", tokens, d)
-        self._set(wg, "wg", f, d)
-        self._set(wu, "wu", f, d)
-        self._set(wd, "wd", d, f)
         return tokens
 
     def forward(self, x, wg, wu, wd, y, g=None, u=None, stream=None) -> None:
         """Writes y, and g and u when they are given (both or neither)."""
         if (g is None) != (u is None):
             raise ValueError("g and u are written together: give both or neither")
-        tokens = self._operands(x, wg, wu, wd)
-        self._set(y, "y", tokens, self.d_model)
-        self._set(g, "g", tokens, self.d_ff)
-        self._set(u, "u", tokens, self.d_ff)
-        self._call(self._lib.roller_b200_ffn_forward, "roller_b200_ffn_forward", stream)
+        n, d, f = self._tokens(x), self.d_model, self.d_ff
+        self._call(self._lib.roller_b200_ffn_forward, "roller_b200_ffn_forward", n,
+                   (("x", x, n, d), ("wg", wg, f, d), ("wu", wu, f, d), ("wd", wd, d, f), ("y", y, n, d),
+                    ("g", g, n, f), ("u", u, n, f)) + _NONE[:5], stream)
 
     def backward(self, x, wg, wu, wd, g, u, dy, dx, dwg, dwu, dwd, stream=None) -> None:
         """Writes dx, dwg, dwu and dwd (not added to) for the gradient dy of y. g and u are what
         `forward` wrote for the same x and weights. The plan has to be made with training=True."""
-        d, f = self.d_model, self.d_ff
-        tokens = self._operands(x, wg, wu, wd)
-        self._set(g, "g", tokens, f)
-        self._set(u, "u", tokens, f)
-        self._set(dy, "dy", tokens, d)
-        self._set(dx, "dx", tokens, d)
-        self._set(dwg, "dwg", f, d)
-        self._set(dwu, "dwu", f, d)
-        self._set(dwd, "dwd", d, f)
-        self._call(self._lib.roller_b200_ffn_backward, "roller_b200_ffn_backward", stream)
+        n, d, f = self._tokens(x), self.d_model, self.d_ff
+        self._call(self._lib.roller_b200_ffn_backward, "roller_b200_ffn_backward", n,
+                   (("x", x, n, d), ("wg", wg, f, d), ("wu", wu, f, d), ("wd", wd, d, f)) + _NONE[:1] +
+                   (("g", g, n, f), ("u", u, n, f), ("dy", dy, n, d), ("dx", dx, n, d), ("dwg", dwg, f, d),
+                    ("dwu", dwu, f, d), ("dwd", dwd, d, f)), stream)
 
     def check_status(self) -> None:
         """Raises RollerError(TIMEOUT) if a launch since the last check gave up on a device-side

@@ -37,6 +37,7 @@ class OrthogonalPlan:
         if dtype not in types:
             raise TypeError(f"inputs are fp32, bf16 or fp16, not {dtype}")
         self.batch, self.rows, self.cols, self.dtype = batch, rows, cols, dtype
+        self._out_dtype = torch.bfloat16
         a, b, c = coefficients
         _lib.check(self._lib.roller_b200_ortho_create(batch, rows, cols, types[dtype], steps, a, b, c, eps,
                                                       C.byref(self._h)), "roller_b200_ortho_create")
@@ -58,17 +59,12 @@ class OrthogonalPlan:
 
     def run(self, g, out, stream=None) -> None:
         """Writes the orthogonalised g into out (bf16, same shape). g is not changed."""
-        import torch
         if not self._h:
             raise RuntimeError("the plan has been destroyed")
         ld_g, zs_g = self._strides(g, "g", self.dtype)
-        ld_o, zs_o = self._strides(out, "out", torch.bfloat16)
-        with torch.cuda.device(self.device):
-            if stream is None:
-                stream = torch.cuda.current_stream()
-            _lib.check(self._lib.roller_b200_ortho_run(self._h, g.data_ptr(), ld_g, zs_g, out.data_ptr(), ld_o,
-                                                       zs_o, C.c_void_p(getattr(stream, "cuda_stream", stream))),
-                       "roller_b200_ortho_run")
+        ld_o, zs_o = self._strides(out, "out", self._out_dtype)
+        _lib.check(_lib.on_device(self.device, stream, self._lib.roller_b200_ortho_run, self._h, g.data_ptr(), ld_g,
+                                  zs_g, out.data_ptr(), ld_o, zs_o), "roller_b200_ortho_run")
 
     def check_status(self) -> None:
         """Raises RollerError(TIMEOUT) if a launch since the last check gave up on a device-side

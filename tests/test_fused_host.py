@@ -44,6 +44,17 @@ def test_ortho_create_refuses_bad_arguments():
     assert not h
 
 
+def test_packed_operands_match_the_structure():
+    from mlir_roller_b200 import ffn
+    io = _lib.FfnIo()
+    assert ffn._IO.size == C.sizeof(io)
+    ffn._IO.pack_into(io, 0, 7, *range(100, 124))
+    assert io.tokens == 7
+    names = [n for n, _ in _lib.FfnIo._fields_[1:]]
+    for i, n in enumerate(names):
+        assert (getattr(io, n).ptr, getattr(io, n).ld) == (100 + 2 * i, 101 + 2 * i), n
+
+
 def test_tensor_checks():
     cpu, bf16 = torch.device("cpu"), torch.bfloat16
     t = torch.zeros(6, 10, dtype=bf16)
