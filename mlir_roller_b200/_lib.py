@@ -224,8 +224,10 @@ def on_device(device, stream, fn, *args) -> int:
     """fn(*args, stream) with `device` current; `stream` None is its current stream."""
     import torch
     if stream is None:
-        stream = torch.cuda.current_stream(device)
-    ptr = C.c_void_p(getattr(stream, "cuda_stream", stream))
+        # (the raw handle: building a Stream object costs as much as the rest of a call)
+        ptr = torch._C._cuda_getCurrentRawStream(device.index)
+    else:
+        ptr = getattr(stream, "cuda_stream", stream)
     if torch.cuda.current_device() == device.index:
         return fn(*args, ptr)
     with torch.cuda.device(device):

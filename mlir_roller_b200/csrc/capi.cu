@@ -168,11 +168,6 @@ int encode_batch16(CUtensorMap* tm, const void* base, long long cols, long long 
   return ROLLER_OK;
 }
 
-void pad_rows16(const void* src, long long ld_src, void* dst, long long ld_dst, int rows, int cols,
-                int blocks, cudaStream_t st) {
-  pad_rows(src, ld_src, dst, ld_dst, rows, cols, 2, blocks, st);
-}
-
 }  // namespace rb200
 
 struct roller_plan;

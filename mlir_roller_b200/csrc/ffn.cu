@@ -4,8 +4,10 @@
 //   forward    kOpGate:  h = act(x Wg^T) * (x Wu^T)        kOpDown:  y = h Wd^T
 //   backward   kOpDact:  dh = dy Wd, from which dg, du and h leave together (dh itself stays in the
 //                        accumulator, and h is made again from g and u rather than kept)
-//              kOpDw:    dWg = dg^T x and dWu = du^T x in one launch; dWd = dy^T h
 //              kOpDx:    dx = dg Wg + du Wu, one reduction over both
+//              kOpDw:    dWg = dg^T x and dWu = du^T x in one launch; dWd = dy^T h
+//              The last three launches need only what kOpDact wrote, so they overlap
+//              (FusedParams::late_wait); kOpDx goes first, because its few long tiles leave SMs free.
 #include <cstring>
 #include <new>
 
@@ -46,9 +48,9 @@ size_t pad_bytes(const roller_ffn_plan* p, int which) {
   return static_cast<size_t>(rows_of(p, which)) * up64(cols_of(p, which)) * 2;
 }
 
-// The operand as the tensor maps may take it: itself, or its copy with aligned rows.
-int usable(roller_ffn_plan* p, int which, const roller_mat& m, int rows, cudaStream_t st, const void** ptr,
-           long long* ld) {
+// The operand as the tensor maps may take it: itself, or a copy with aligned rows that `jobs` will make.
+int usable(roller_ffn_plan* p, int which, const roller_mat& m, int rows, cudaStream_t st, AlignJobs* jobs,
+           const void** ptr, long long* ld) {
   if (aligned16(m.ptr, m.ld)) {
     *ptr = m.ptr;
     *ld = m.ld;
@@ -65,8 +67,8 @@ int usable(roller_ffn_plan* p, int which, const roller_mat& m, int rows, cudaStr
       return ROLLER_ERR_NOMEM;
     }
   }
-  pad_rows16(m.ptr, m.ld, p->pad[which], ldp, rows, cols_of(p, which), p->ctx.dev.sm_count * 8, st);
-  FUSED_CUDA(cudaGetLastError());
+  jobs->job[jobs->n++] = AlignJob{static_cast<const uint16_t*>(m.ptr), static_cast<uint16_t*>(p->pad[which]), m.ld,
+                                  ldp, rows, cols_of(p, which), 0};
   *ptr = p->pad[which];
   *ld = ldp;
   return ROLLER_OK;
@@ -143,10 +145,13 @@ int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* s
   const bool bf16 = p->dt == 1;
   const void *x, *wg, *wu, *wd;
   long long ldx, ldg, ldu, ldd;
-  FUSED_OK(usable(p, kX, io->x, T, st, &x, &ldx));
-  FUSED_OK(usable(p, kWg, io->wg, F, st, &wg, &ldg));
-  FUSED_OK(usable(p, kWu, io->wu, F, st, &wu, &ldu));
-  FUSED_OK(usable(p, kWd, io->wd, D, st, &wd, &ldd));
+  AlignJobs jobs;
+  jobs.n = 0;
+  FUSED_OK(usable(p, kX, io->x, T, st, &jobs, &x, &ldx));
+  FUSED_OK(usable(p, kWg, io->wg, F, st, &jobs, &wg, &ldg));
+  FUSED_OK(usable(p, kWu, io->wu, F, st, &jobs, &wu, &ldu));
+  FUSED_OK(usable(p, kWd, io->wd, D, st, &jobs, &wd, &ldd));
+  FUSED_CUDA(align_rows(jobs, p->ctx.dev.sm_count, st));
   {
     Product g(p->ctx, kOpGate, p->dt, T, F, D, 1);
     g.p.act = p->act;
@@ -192,13 +197,16 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
   const bool bf16 = p->dt == 1;
   const void *x, *wg, *wu, *wd, *dy, *g, *u;
   long long ldx, ldg, ldu, ldd, ldy, ldsg, ldsu;
-  FUSED_OK(usable(p, kX, io->x, T, st, &x, &ldx));
-  FUSED_OK(usable(p, kWg, io->wg, F, st, &wg, &ldg));
-  FUSED_OK(usable(p, kWu, io->wu, F, st, &wu, &ldu));
-  FUSED_OK(usable(p, kWd, io->wd, D, st, &wd, &ldd));
-  FUSED_OK(usable(p, kDy, io->dy, T, st, &dy, &ldy));
-  FUSED_OK(usable(p, kG, io->g, T, st, &g, &ldsg));
-  FUSED_OK(usable(p, kU, io->u, T, st, &u, &ldsu));
+  AlignJobs jobs;
+  jobs.n = 0;
+  FUSED_OK(usable(p, kX, io->x, T, st, &jobs, &x, &ldx));
+  FUSED_OK(usable(p, kWg, io->wg, F, st, &jobs, &wg, &ldg));
+  FUSED_OK(usable(p, kWu, io->wu, F, st, &jobs, &wu, &ldu));
+  FUSED_OK(usable(p, kWd, io->wd, D, st, &jobs, &wd, &ldd));
+  FUSED_OK(usable(p, kDy, io->dy, T, st, &jobs, &dy, &ldy));
+  FUSED_OK(usable(p, kG, io->g, T, st, &jobs, &g, &ldsg));
+  FUSED_OK(usable(p, kU, io->u, T, st, &jobs, &u, &ldsu));
+  FUSED_CUDA(align_rows(jobs, p->ctx.dev.sm_count, st));
   const long long zs = static_cast<long long>(p->max_tokens) * p->ldf;   // dg to du
   {
     Product a(p->ctx, kOpDact, p->dt, T, F, D, 1);
@@ -213,27 +221,29 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     FUSED_OK(a.launch(st));
   }
   {
+    Product r(p->ctx, kOpDx, p->dt, T, D, F, 1);
+    r.p.b_early = 1;   // Wg and Wu do not come from the kernel above
+    FUSED_OK(r.a_k(p->dgu, F, T, 2, p->ldf, zs));
+    FUSED_OK(r.b_mn(0, wg, D, F, 1, ldg, 0));
+    FUSED_OK(r.b_mn(1, wu, D, F, 1, ldu, 0));
+    FUSED_OK(r.output(0, io->dx.ptr, 1, io->dx.ld, 0, bf16));
+    FUSED_OK(r.launch(st));
+  }
+  {
     Product w(p->ctx, kOpDw, p->dt, F, D, T, 2);
+    w.p.late_wait = 1;   // dg, du and h were complete before the kernel above started
     FUSED_OK(w.a_mn(p->dgu, F, T, 2, p->ldf, zs));
     FUSED_OK(w.b_mn(0, x, D, T, 1, ldx, 0));
     FUSED_OK(w.output(0, io->dwg.ptr, 1, io->dwg.ld, 0, bf16));
     FUSED_OK(w.output(1, io->dwu.ptr, 1, io->dwu.ld, 0, bf16));
     FUSED_OK(w.launch(st));
   }
-  {
-    Product w(p->ctx, kOpDw, p->dt, D, F, T, 1);
-    FUSED_OK(w.a_mn(dy, D, T, 1, ldy, 0));
-    FUSED_OK(w.b_mn(0, p->h, F, T, 1, p->ldf, 0));
-    FUSED_OK(w.output(0, io->dwd.ptr, 1, io->dwd.ld, 0, bf16));
-    FUSED_OK(w.launch(st));
-  }
-  Product r(p->ctx, kOpDx, p->dt, T, D, F, 1);
-  r.p.b_early = 1;   // Wg and Wu do not come from the kernel before
-  FUSED_OK(r.a_k(p->dgu, F, T, 2, p->ldf, zs));
-  FUSED_OK(r.b_mn(0, wg, D, F, 1, ldg, 0));
-  FUSED_OK(r.b_mn(1, wu, D, F, 1, ldu, 0));
-  FUSED_OK(r.output(0, io->dx.ptr, 1, io->dx.ld, 0, bf16));
-  return r.launch(st);
+  Product w(p->ctx, kOpDw, p->dt, D, F, T, 1);
+  w.p.late_wait = 1;
+  FUSED_OK(w.a_mn(dy, D, T, 1, ldy, 0));
+  FUSED_OK(w.b_mn(0, p->h, F, T, 1, p->ldf, 0));
+  FUSED_OK(w.output(0, io->dwd.ptr, 1, io->dwd.ld, 0, bf16));
+  return w.launch(st);
 }
 
 int roller_b200_ffn_status(roller_ffn_plan* p, uint32_t* device_status) {

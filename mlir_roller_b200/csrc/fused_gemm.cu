@@ -1,5 +1,6 @@
 // Which fused product kernel a problem runs on, and how its reduction is cut.
 #include "fused_product.h"
+#include "ptx_sm100.cuh"
 
 namespace rb200 {
 
@@ -18,9 +19,66 @@ struct TileCost {
   double kb_us;    // one k-block of one tile while every SM works
   double tile_us;  // fill and the last tile's epilogue
 };
-constexpr TileCost kTiles[] = {{2, 256, 0.36, 7.0}, {1, 256, 0.40, 6.0}, {1, 128, 0.28, 4.5}};
+constexpr TileCost kTiles[] = {{2, 256, 0.36, 7.0}, {1, 256, 0.40, 6.0}, {1, 128, 0.28, 4.5}, {1, 64, 0.22, 4.0}};
+
+// Copies the jobs' 16-bit rows into rows that start on 16 bytes. A warp takes 256 words (of two
+// elements) of a row at a time, a thread eight of them, all on their way together: a source row
+// that starts between two words gives each word from two neighbouring ones. (A word that holds an
+// element of the row may be read whole.)
+__global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__ AlignJobs jobs) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  int b = static_cast<int>(blockIdx.x), i = 0;
+  while (i + 1 < jobs.n && b >= jobs.job[i].blocks) b -= jobs.job[i++].blocks;
+  const AlignJob& j = jobs.job[i];
+  const int lane = threadIdx.x & 31;
+  const int words = (j.cols + 1) / 2, runs = (words + 255) / 256;
+  const long long units = static_cast<long long>(j.rows) * runs;
+  for (long long u = b * 8 + static_cast<int>(threadIdx.x >> 5); u < units; u += j.blocks * 8) {
+    const int row = static_cast<int>(u / runs), w0 = static_cast<int>(u - static_cast<long long>(row) * runs) * 256 + lane;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(j.src + row * j.ld_src);
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(at & ~static_cast<uintptr_t>(3));
+    uint32_t* dst = reinterpret_cast<uint32_t*>(j.dst + row * j.ld_dst);
+    const bool between = (at & 2) != 0;
+    uint32_t x[8], y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int w = w0 + 32 * k;
+      x[k] = w < words ? __ldg(src + w) : 0u;
+      y[k] = between && 2 * w + 1 < j.cols ? __ldg(src + w + 1) : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (w0 + 32 * k < words) dst[w0 + 32 * k] = between ? __byte_perm(x[k], y[k], 0x5432) : x[k];
+  }
+}
 
 }  // namespace
+
+cudaError_t align_rows(AlignJobs& jobs, int sm_count, cudaStream_t stream) {
+  if (jobs.n == 0) return cudaSuccess;
+  // blocks in proportion to the jobs' sizes, eight per SM in all
+  double total = 0.0;
+  for (int i = 0; i < jobs.n; ++i) total += static_cast<double>(jobs.job[i].rows) * jobs.job[i].cols;
+  int blocks = 0;
+  for (int i = 0; i < jobs.n; ++i) {
+    AlignJob& j = jobs.job[i];
+    const double most = (static_cast<double>(j.rows) * ((j.cols + 511) / 512) + 7) / 8;
+    const double b = 8.0 * sm_count * j.rows * j.cols / total + 1;
+    j.blocks = static_cast<int>(b < most ? b : most);
+    blocks += j.blocks;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, align_rows_kernel, jobs);
+}
 
 const FusedVariant* fused_find(int op, int cta_group, int block_n, int dt) {
   for (int i = 0; i < 3; ++i) {

@@ -42,7 +42,8 @@ struct FusedParams {
   int a_bytes;          // bytes one TMA load of A brings (fewer rows than 128 on single CTAs)
   int tiles_m, tiles_n, tiles_per_z, zcount;
   int split;            // parts of a cluster that share a tile's k (1 = none)
-  int b_early;          // the second operand may be read before the previous kernel is done
+  int b_early;          // the second operand may be read before the previous kernel is done ...
+  int late_wait;        // ... or everything: that kernel is only waited for at the end
   int act;
   int flags;
   float coef_a, coef_b, coef_c, inv_scale;

@@ -34,10 +34,15 @@
 // every access of a warp touches 32 lines.
 //
 // A launch may be scheduled while the previous one of its stream still runs (programmatic
-// dependent launch). It touches memory only behind griddepcontrol.wait, with one exception
-// (p.b_early): weights may be fetched before, when the previous kernel is one of this library
-// that does not write them. That is safe because a kernel here lets its successor start only
-// after its own wait has returned, so everything before the previous kernel is complete.
+// dependent launch). It touches memory only behind griddepcontrol.wait, with two exceptions, both
+// resting on this: a kernel here lets its successor start only after its own wait has returned,
+// so when the successor starts, everything before its predecessor is complete.
+//   * p.b_early: weights may be fetched before the wait, when the previous kernel is one of these
+//     and does not write them;
+//   * p.late_wait: a kernel that needs nothing from its predecessor (and writes nothing that one
+//     touches) waits for it only before it ends, so that its CTAs fill the SMs that the
+//     predecessor's last wave leaves idle. It ends after its predecessor, so what follows
+//     in the stream still finds both complete.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -71,15 +76,16 @@ struct FusedCfg {
   static constexpr int RING = OP == kOpDact ? 3 : 2;
   static constexpr int WARP_BOXES = INPUTS + RING;
   static constexpr int STAGING_BYTES = EPI_WARPS * WARP_BOXES * BOX_BYTES;
-  static constexpr int CTRL_BYTES = 256;
+  static constexpr int CTRL_BYTES = 384;
   static constexpr int SMEM_LIMIT = 232448;      // 227 KiB opt-in maximum per CTA
   static constexpr int STAGES_FIT = (SMEM_LIMIT - 1024 - CTRL_BYTES - STAGING_BYTES) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + STAGING_BYTES + CTRL_BYTES + 1024;
+  static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int SMEM_BYTES = RING_BYTES + STAGING_BYTES + CTRL_BYTES + 1024;
   static constexpr int TMEM_COLS = 2 * BN;
   static constexpr int FIRST_EPI_WARP = 4;
   static constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
-  static_assert(BN == 256 || BN == 128, "tile widths");
+  static_assert(BN == 256 || BN == 128 || (BN == 64 && OP != kOpGate), "tile widths");
   static constexpr int SYM_RATIO = BN / TILE_M;      // tile rows per tile column of a triangle
   static_assert(!SYM || SYM_RATIO == 1 || SYM_RATIO == 2, "triangle of tiles");
   // The exchange of partial sums in a splitting cluster goes through the ring's memory: each CTA
@@ -195,15 +201,15 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   constexpr int BN = Cfg::BN, CG = Cfg::CG, STAGES = Cfg::STAGES, DT = Cfg::DT, OP = Cfg::OP;
   extern __shared__ uint8_t smem_dyn[];
   const uint32_t smem_base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
-  const uint32_t staging = smem_base + STAGES * Cfg::STAGE_BYTES;
+  const uint32_t staging = smem_base + Cfg::RING_BYTES;
   const uint32_t ctrl = staging + Cfg::STAGING_BYTES;
   auto full_bar = [&](int s) { return ctrl + 8u * s; };
-  auto empty_bar = [&](int s) { return ctrl + 64u + 8u * s; };
-  auto tmem_full_bar = [&](int a) { return ctrl + 128u + 8u * a; };
-  auto tmem_empty_bar = [&](int a) { return ctrl + 144u + 8u * a; };
-  const uint32_t mma_done_bar = ctrl + 160u;
-  const uint32_t tmem_slot = ctrl + 176u;
-  auto in_bar = [&](int w) { return ctrl + 184u + 8u * w; };   // a warp's inputs have landed
+  auto empty_bar = [&](int s) { return ctrl + 128u + 8u * s; };
+  auto tmem_full_bar = [&](int a) { return ctrl + 256u + 8u * a; };
+  auto tmem_empty_bar = [&](int a) { return ctrl + 272u + 8u * a; };
+  const uint32_t mma_done_bar = ctrl + 288u;
+  const uint32_t tmem_slot = ctrl + 296u;
+  auto in_bar = [&](int w) { return ctrl + 304u + 8u * w; };   // a warp's inputs have landed
   const WaitCtx wc{p.status, p.spin_limit};
 
   const int warp = threadIdx.x >> 5;
@@ -302,7 +308,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
       if (t == worker) {
         const int early = p.b_early ? min(STAGES, kb1 - kb0) : 0;
         for (int i = 0; i < early; ++i) load_b(i, arm(i), c, kb + i);
-        grid_dependency_wait();
+        if (!p.late_wait) grid_dependency_wait();
         grid_launch_dependents();
         for (int i = 0; i < early; ++i)
           load_a(i, CG == 2 ? map_to_cta(full_bar(i), leader_rank) : full_bar(i), c, kb + i);
@@ -330,7 +336,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
                                               DT == 1 ? 1u : 0u);
     // one MMA covers 16 k: 32 bytes along a k-contiguous row, or 16 rows of 128 bytes
     constexpr uint64_t a_step = Cfg::A_MN ? 128 : 2, b_step = Cfg::B_MN ? 128 : 2;
-    grid_dependency_wait();
+    if (!p.late_wait) grid_dependency_wait();
     int s = 0, acc = 0;
     uint32_t ph = 0, acc_ph = 0;
     bool ok = true;
@@ -438,17 +444,32 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     } else {
       // rows that start anywhere: a warp writes 32 consecutive elements per instruction
       __syncwarp();
-      uint16_t* dst = static_cast<uint16_t*>(p.out[o]) + oz * p.out_zstride + col + lane;
-      const bool in = col + lane < p.out_cols;
-      for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
-        uint16_t x;
-        asm volatile("ld.shared.u16 %0, [%1];"
-                     : "=h"(x)
-                     : "r"(box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16) + (lane & 7) * 2)
-                     : "memory");
-        if (in) dst[static_cast<long long>(row0 + r) * p.out_ld[o]] = x;
+      uint16_t* dst = static_cast<uint16_t*>(p.out[o]) + oz * p.out_zstride + static_cast<long long>(row0) * p.out_ld[o] + col + lane;
+      const int rows = col + lane < p.out_cols ? p.M - row0 : 0;
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += 8) {
+        uint16_t x[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          asm volatile("ld.shared.u16 %0, [%1];"
+                       : "=h"(x[r])
+                       : "r"(box + (r0 + r) * 64 + (((lane >> 3) ^ (((r0 + r) >> 1) & 3)) * 16) + (lane & 7) * 2)
+                       : "memory");
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r0 + r < rows) dst[(r0 + r) * p.out_ld[o]] = x[r];
       }
       if (lane == 0) bulk_commit_group();   // (an empty group keeps the ring's count)
+    }
+  };
+  // The first n boxes to outputs 0 .. n - 1, which are the library's own, aligned memory.
+  auto hand_over = [&](int n, const FusedTile& c, int row0, int col) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (row0 < p.M)
+        for (int o = 0; o < n; ++o) tma_store_3d(&p.o[o], boxes + o * Cfg::BOX_BYTES, col, row0, c.z);
+      bulk_commit_group();
     }
   };
   // The mirror image of 32 x 32 elements of a symmetric fp16 matrix (its own box has no swizzle).
@@ -526,21 +547,12 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
             du[j] = dh * y;
             h[j] = y * uu;
           }
-          // three matrices, one hand-over (all three are the library's own, aligned memory)
           if (lane == 0) bulk_wait_read_all();
           __syncwarp();
           put(boxes, v, false);
           put(boxes + Cfg::BOX_BYTES, du, false);
           put(boxes + 2 * Cfg::BOX_BYTES, h, false);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (row0 < p.M) {
-#pragma unroll
-              for (int o = 0; o < 3; ++o) tma_store_3d(&p.o[o], boxes + o * Cfg::BOX_BYTES, col, row0, 0);
-            }
-            bulk_commit_group();
-          }
+          hand_over(3, c, row0, col);
         } else if constexpr (OP == kOpDown || OP == kOpDx || OP == kOpDw) {
           sums(tc, v);
           emit(OP == kOpDw ? c.z : 0, c, row0, col, v, false);
@@ -567,22 +579,34 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
           if (col < row0) emit_mirror(c, row0, col, v);
         } else {
           sums(tc, v);
-          const float dr = (OP == kOpUpdateWide && row < p.M) ? p.vec[c.z * p.vec_ld + row] : 0.0f;
+          if constexpr (OP == kOpUpdateWide) {
+            const float d = row < p.M ? p.vec[c.z * p.vec_ld + row] : 0.0f;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float dv = dr;
-            if constexpr (OP == kOpUpdateTall) dv = (col + j < p.out_cols) ? __ldg(p.vec + c.z * p.vec_ld + col + j) : 0.0f;
-            v[j] = dv * (input(0, j) + input(1, j)) + v[j] * p.inv_scale;
+            for (int j = 0; j < 32; ++j) v[j] = d * (input(0, j) + input(1, j)) + v[j] * p.inv_scale;
+          } else {
+            // (rows of vec are padded to 64; what lies in the padding meets columns that are not stored)
+            const float4* d4 = reinterpret_cast<const float4*>(p.vec + c.z * p.vec_ld + col);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 d = __ldg(d4 + j);
+              v[4 * j] = d.x * (input(0, 4 * j) + input(1, 4 * j)) + v[4 * j] * p.inv_scale;
+              v[4 * j + 1] = d.y * (input(0, 4 * j + 1) + input(1, 4 * j + 1)) + v[4 * j + 1] * p.inv_scale;
+              v[4 * j + 2] = d.z * (input(0, 4 * j + 2) + input(1, 4 * j + 2)) + v[4 * j + 2] * p.inv_scale;
+              v[4 * j + 3] = d.w * (input(0, 4 * j + 3) + input(1, 4 * j + 3)) + v[4 * j + 3] * p.inv_scale;
+            }
           }
           if (p.flags & kFusedLast) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
             emit(0, c, row0, col, v, true);
           } else {
-            emit(0, c, row0, col, v, false);
+            if (lane == 0) bulk_wait_read_all();
+            __syncwarp();
+            put(boxes, v, false);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
-            emit(1, c, row0, col, v, false);
+            put(boxes + Cfg::BOX_BYTES, v, false);
+            hand_over(2, c, row0, col);
           }
         }
       }
@@ -599,7 +623,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   constexpr int kSlabs = Cfg::OUT_COLS / 32;     // slabs of one warp of a whole tile
 
   if (epi && split == 1) {
-    grid_dependency_wait();
+    if (!p.late_wait) grid_dependency_wait();
     int acc = 0;
     uint32_t acc_ph = 0;
     for (int t = worker; epi_ok && t < tiles; t += workers) {
@@ -636,7 +660,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     const int my_slab = static_cast<int>(part) / apart * share;
     const bool receives = static_cast<int>(part) % apart == 0 && half < share;
     if (epi) {
-      grid_dependency_wait();
+      if (!p.late_wait) grid_dependency_wait();
       if constexpr (Cfg::INPUTS > 0) {
         const int col = c.nb * BN + (my_slab + half) * 32;
         if (receives && wanted(row0, col)) fetch(c, row0, col);
@@ -709,6 +733,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   // ------------------------------------------------------------------ teardown
   // stores handed to the TMA unit have to be performed before the CTA may go
   if (epi && lane == 0) bulk_wait_all();
+  if (p.late_wait) grid_dependency_wait();
   __syncwarp();
   // after a failed wait some role left its loop early: let bulk copies on their way land
   if (*reinterpret_cast<volatile uint32_t*>(p.status) != kDevOk) abort_grace_period();

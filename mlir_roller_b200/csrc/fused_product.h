@@ -37,6 +37,20 @@ int fused_context_create(FusedContext* c);    // on the current device; a roller
 void fused_context_destroy(FusedContext* c);
 int fused_context_status(FusedContext* c, uint32_t* device_status);   // reads and clears
 
+// Operands whose rows do not start on 16 bytes are copied, all of a call's in one launch.
+struct AlignJob {
+  const uint16_t* src;
+  uint16_t* dst;
+  long long ld_src, ld_dst;
+  int rows, cols;
+  int blocks;       // set by align_rows
+};
+struct AlignJobs {
+  AlignJob job[8];
+  int n;
+};
+cudaError_t align_rows(AlignJobs& jobs, int sm_count, cudaStream_t stream);
+
 // D is M x N, reduced over K, for z matrices; operand matrices are [z][rows][cols] in memory.
 struct Product {
   FusedParams p;

@@ -15,8 +15,4 @@ int encode_batch16(CUtensorMap* tm, const void* base, long long cols, long long 
                    long long ld, long long z_stride, int box_cols, int box_rows,
                    CUtensorMapSwizzle swz, bool bf16);
 
-// Copies 16-bit rows into rows whose stride is a multiple of 16 bytes.
-void pad_rows16(const void* src, long long ld_src, void* dst, long long ld_dst, int rows, int cols,
-                int blocks, cudaStream_t st);
-
 }  // namespace rb200

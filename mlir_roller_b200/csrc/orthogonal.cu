@@ -21,6 +21,7 @@
 #include <cuda_fp16.h>
 
 #include "fused_product.h"
+#include "ptx_sm100.cuh"
 
 using namespace rb200;
 
@@ -59,37 +60,87 @@ struct Source {
   const void* g;
   long long ld, zs;
   int rows, cols;
-  int vec;     // rows and matrices start on 16 bytes
-  int tx;      // threads along a row (power of two), the other 256 / tx take further rows
+  int vec;             // rows and matrices start on 16 bytes
+  uint32_t per_row;    // groups of eight elements in a row
 };
 
-// Sum of squares of each matrix, in fp64 (bound by the read: 8 bytes of fp64 work per element are
-// a few per cent of it), one partial sum per block.
-template <typename T>
-__global__ void __launch_bounds__(256) ortho_sumsq(Source s, double* __restrict__ part) {
-  const T* g = static_cast<const T*>(s.g) + blockIdx.y * s.zs;
-  const int x = threadIdx.x % s.tx, y = threadIdx.x / s.tx, ty = 256 / s.tx;
-  double sum = 0.0;
-  for (long long r = static_cast<long long>(blockIdx.x) * ty + y; r < s.rows; r += static_cast<long long>(gridDim.x) * ty) {
-    const T* row = g + r * s.ld;
-#pragma unroll 4
-    for (int c = x * 8; c < s.cols; c += s.tx * 8) {
-      float v[8];
-      load8(row, c, s.cols, s.vec, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum += static_cast<double>(v[j]) * static_cast<double>(v[j]);
+// A thread of the next two kernels takes every (grid's threads)-th group of eight elements of a
+// matrix, four groups at a time, so that 64 to 128 bytes per thread are on their way.
+constexpr int kGroupsAtOnce = 4;
+struct Walk {
+  uint32_t r, c, dr, dc, per_row;     // row and group in it; the step, likewise
+  __device__ explicit Walk(uint32_t per_row_) : per_row(per_row_) {
+    const uint32_t u = blockIdx.x * 256u + threadIdx.x, stride = gridDim.x * 256u;
+    r = u / per_row;
+    c = u - r * per_row;
+    dr = stride / per_row;
+    dc = stride - dr * per_row;
+  }
+  __device__ void step() {
+    r += dr;
+    c += dc;
+    if (c >= per_row) {
+      c -= per_row;
+      ++r;
     }
   }
+};
+
+__device__ __forceinline__ double block_sum(double sum) {
   __shared__ double warp_sum[8];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    double t = 0.0;
-    for (int i = 0; i < 8; ++i) t += warp_sum[i];
-    part[blockIdx.y * kSumBlocks + blockIdx.x] = t;
+  sum = 0.0;
+  for (int i = 0; i < 8; ++i) sum += warp_sum[i];
+  return sum;
+}
+
+// Sum of squares of each matrix, one partial sum per block. Eight elements at a time are scaled by a
+// power of two to below 4, squared and added in fp32, and their sum goes on in fp64: neither
+// tiny nor huge matrices leave the range, and the one conversion to fp64 per eight elements
+// does not bound the read (one per element would: 4 a cycle and SM).
+template <typename T>
+__global__ void __launch_bounds__(256) ortho_sumsq(Source s, double* __restrict__ part) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const T* g = static_cast<const T*>(s.g) + blockIdx.y * s.zs;
+  const uint32_t rows = static_cast<uint32_t>(s.rows);
+  double sum = 0.0;
+  Walk w(s.per_row);
+  while (w.r < rows) {
+    float v[kGroupsAtOnce][8];
+#pragma unroll
+    for (int i = 0; i < kGroupsAtOnce; ++i, w.step()) {
+      if (w.r < rows) {
+        load8(g + w.r * s.ld, static_cast<int>(w.c) * 8, s.cols, s.vec, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kGroupsAtOnce; ++i) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
+      // exponent of the largest; 255 (not finite) passes through unscaled
+      const uint32_t e = top >> 23;
+      const uint32_t k = e < 253u ? e : 253u;
+      const float scale = e == 255u ? 1.0f : __uint_as_float((254u - k) << 23);   // 2^(127 - k)
+      float q = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float f = v[i][j] * scale;
+        q = fmaf(f, f, q);
+      }
+      // times 2^(2 (k - 127))
+      sum += static_cast<double>(q) * __hiloint2double(static_cast<int>((769u + 2u * k) << 20), 0);
+    }
   }
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) part[blockIdx.y * kSumBlocks + blockIdx.x] = sum;
 }
 
 // x = S g / (|g| + eps) as hi + lo. Every block adds the partial sums in the same order.
@@ -97,48 +148,60 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 ortho_scale(Source s, const double* __restrict__ part, int parts, double eps, __half* __restrict__ hi,
             __half* __restrict__ lo, long long ldx, long long zsx) {
-  __shared__ double warp_sum[8];
+  grid_dependency_wait();
+  grid_launch_dependents();
   double sum = 0.0;
   for (int i = threadIdx.x; i < parts; i += 256) sum += part[blockIdx.y * kSumBlocks + i];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  sum = 0.0;
-  for (int i = 0; i < 8; ++i) sum += warp_sum[i];
+  sum = block_sum(sum);
   const float scale = static_cast<float>(static_cast<double>(kScale) / (sqrt(sum) + eps));
 
   const T* g = static_cast<const T*>(s.g) + blockIdx.y * s.zs;
-  const int x = threadIdx.x % s.tx, y = threadIdx.x / s.tx, ty = 256 / s.tx;
-  for (long long r = static_cast<long long>(blockIdx.x) * ty + y; r < s.rows; r += static_cast<long long>(gridDim.x) * ty) {
-    const T* row = g + r * s.ld;
-    const long long at = blockIdx.y * zsx + r * ldx;
-#pragma unroll 2
-    for (int c = x * 8; c < s.cols; c += s.tx * 8) {
-      float v[8];
-      load8(row, c, s.cols, s.vec, v);
+  const uint32_t rows = static_cast<uint32_t>(s.rows);
+  Walk w(s.per_row);
+  while (w.r < rows) {
+    float v[kGroupsAtOnce][8];
+    Walk back = w;
+#pragma unroll
+    for (int i = 0; i < kGroupsAtOnce; ++i, w.step())
+      if (w.r < rows) load8(g + w.r * s.ld, static_cast<int>(w.c) * 8, s.cols, s.vec, v[i]);
+#pragma unroll
+    for (int i = 0; i < kGroupsAtOnce; ++i, back.step()) {
+      if (back.r >= rows) break;
       alignas(16) __half h[8], l[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float f = v[j] * scale;
+        const float f = v[i][j] * scale;
         h[j] = __float2half_rn(f);
         l[j] = __float2half_rn(f - __half2float(h[j]));
       }
-      *reinterpret_cast<uint4*>(hi + at + c) = *reinterpret_cast<const uint4*>(h);
-      *reinterpret_cast<uint4*>(lo + at + c) = *reinterpret_cast<const uint4*>(l);
+      const long long at = blockIdx.y * zsx + back.r * ldx + back.c * 8;
+      *reinterpret_cast<uint4*>(hi + at) = *reinterpret_cast<const uint4*>(h);
+      *reinterpret_cast<uint4*>(lo + at) = *reinterpret_cast<const uint4*>(l);
     }
   }
 }
 
 template <typename T>
-int convert(const Source& s, int batch, int blocks, double* part, double eps, __half* hi, __half* lo,
+int convert(const Source& s, int batch, int sm_count, double* part, double eps, __half* hi, __half* lo,
             long long ldx, long long zsx, cudaStream_t st) {
-  const dim3 sums(static_cast<unsigned>(blocks < kSumBlocks ? blocks : kSumBlocks), static_cast<unsigned>(batch));
-  ortho_sumsq<T><<<sums, 256, 0, st>>>(s, part);
-  FUSED_CUDA(cudaGetLastError());
-  const dim3 grid(static_cast<unsigned>(blocks < kSumBlocks ? blocks : kSumBlocks), static_cast<unsigned>(batch));
-  ortho_scale<T><<<grid, 256, 0, st>>>(s, part, static_cast<int>(sums.x), eps, hi, lo, ldx, zsx);
-  FUSED_CUDA(cudaGetLastError());
+  // about eight blocks per SM over the whole batch
+  const long long groups = static_cast<long long>(s.per_row) * s.rows;
+  long long blocks = (groups + 256 * kGroupsAtOnce - 1) / (256 * kGroupsAtOnce);
+  const int most = (8 * sm_count + batch - 1) / batch;
+  if (blocks > most) blocks = most;
+  if (blocks > kSumBlocks) blocks = kSumBlocks;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(batch), 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  FUSED_CUDA(cudaLaunchKernelEx(&cfg, ortho_sumsq<T>, s, part));
+  FUSED_CUDA(cudaLaunchKernelEx(&cfg, ortho_scale<T>, s, static_cast<const double*>(part), static_cast<int>(blocks), eps, hi,
+                                lo, ldx, zsx));
   return ROLLER_OK;
 }
 
@@ -325,16 +388,14 @@ int roller_b200_ortho_run(roller_ortho_plan* p, const void* g, long long ld_g, l
   s.cols = p->cols;
   const int per16 = p->in_type == ROLLER_ORTHO_IN_F32 ? 4 : 8;
   s.vec = (reinterpret_cast<uintptr_t>(g) & 15) == 0 && ld_g % per16 == 0 && (p->batch == 1 || zs_g % per16 == 0);
-  s.tx = 1;
-  while (s.tx < 256 && s.tx * 8 < p->cols) s.tx *= 2;
-  const int ty = 256 / s.tx;
-  const int blocks = (p->rows + ty - 1) / ty;
+  s.per_row = static_cast<uint32_t>((p->cols + 7) / 8);
+  const int sms = p->ctx.dev.sm_count;
   if (p->in_type == ROLLER_ORTHO_IN_F32)
-    FUSED_OK(convert<float>(s, p->batch, blocks, p->part, p->eps, p->x[0][0], p->x[0][1], p->ldx, p->zsx, st));
+    FUSED_OK(convert<float>(s, p->batch, sms, p->part, p->eps, p->x[0][0], p->x[0][1], p->ldx, p->zsx, st));
   else if (p->in_type == ROLLER_ORTHO_IN_BF16)
-    FUSED_OK(convert<__nv_bfloat16>(s, p->batch, blocks, p->part, p->eps, p->x[0][0], p->x[0][1], p->ldx, p->zsx, st));
+    FUSED_OK(convert<__nv_bfloat16>(s, p->batch, sms, p->part, p->eps, p->x[0][0], p->x[0][1], p->ldx, p->zsx, st));
   else
-    FUSED_OK(convert<__half>(s, p->batch, blocks, p->part, p->eps, p->x[0][0], p->x[0][1], p->ldx, p->zsx, st));
+    FUSED_OK(convert<__half>(s, p->batch, sms, p->part, p->eps, p->x[0][0], p->x[0][1], p->ldx, p->zsx, st));
 
   for (int i = 0; i < p->steps; ++i) {
     const int w = i & 1;
