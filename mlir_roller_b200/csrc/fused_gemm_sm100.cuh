@@ -212,7 +212,8 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   auto in_bar = [&](int w) { return ctrl + 304u + 8u * w; };   // a warp's inputs have landed
   const WaitCtx wc{p.status, p.spin_limit};
 
-  const int warp = threadIdx.x >> 5;
+  // (the broadcast tells the compiler that the warp index is the same in all lanes)
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   // a cluster holds the `split` parts of one tile's k, each a CTA or a pair (ranks 2i and 2i + 1)
   const int split = p.split;
@@ -261,8 +262,10 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
 
   bool epi_ok = true;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
+    // (the whole warp walks the loop and one elected lane issues, as the MMA warp does)
+    const bool issues = elect_one();
     auto load_a = [&](int s, uint32_t bar, const FusedTile& c, int kb) {
       const int phase = (OP == kOpDx && kb >= p.num_kb) ? 1 : 0;
       const int m0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM;
@@ -288,15 +291,14 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
         fused_load<Cfg::BNL, Cfg::B_MN, CG == 2>(b_dst, &p.b[phase], bar, n0, k0, bz);
       }
     };
-    // The barrier counts the bytes of both operands (for a pair: of both CTAs, on the leader's,
+    // The barrier that counts the bytes of both operands (for a pair: of both CTAs, on the leader's,
     // which alone arms it).
+    auto counts = [&](int s) { return CG == 2 ? map_to_cta(full_bar(s), leader_rank) : full_bar(s); };
     auto arm = [&](int s) {
       if constexpr (CG == 2) {
         if (is_leader) mbar_expect_tx(full_bar(s), 2 * (Cfg::A_BYTES + Cfg::B_BYTES));
-        return map_to_cta(full_bar(s), leader_rank);
       } else {
         mbar_expect_tx(full_bar(s), p.a_bytes + Cfg::B_BYTES);
-        return full_bar(s);
       }
     };
     int s = 0;
@@ -307,62 +309,82 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
       int kb = kb0;
       if (t == worker) {
         const int early = p.b_early ? min(STAGES, kb1 - kb0) : 0;
-        for (int i = 0; i < early; ++i) load_b(i, arm(i), c, kb + i);
+        if (issues) {
+          for (int i = 0; i < early; ++i) {
+            arm(i);
+            load_b(i, counts(i), c, kb + i);
+          }
+        }
         if (!p.late_wait) grid_dependency_wait();
         grid_launch_dependents();
-        for (int i = 0; i < early; ++i)
-          load_a(i, CG == 2 ? map_to_cta(full_bar(i), leader_rank) : full_bar(i), c, kb + i);
+        if (issues)
+          for (int i = 0; i < early; ++i) load_a(i, counts(i), c, kb + i);
+        __syncwarp();
         kb += early;
         s = early;
         if (s == STAGES) { s = 0; ph ^= 1u; }
       }
       for (; kb < kb1; ++kb) {
-        if (!mbar_wait(empty_bar(s), ph ^ 1u, wc, kDevTimeoutEmpty)) { ok = false; break; }
-        const uint32_t bar = arm(s);
-        load_a(s, bar, c, kb);
-        load_b(s, bar, c, kb);
+        if (!mbar_wait_warp(empty_bar(s), ph ^ 1u, wc, kDevTimeoutEmpty)) { ok = false; break; }
+        if (issues) {
+          const uint32_t bar = counts(s);
+          arm(s);
+          load_a(s, bar, c, kb);
+          load_b(s, bar, c, kb);
+        }
+        __syncwarp();
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
     }
     // the MMA issuer's last releases must land in this CTA before it may exit
     for (int i = 0; i < STAGES && ok; ++i) {
-      ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kDevTimeoutTail);
+      ok = mbar_wait_warp(empty_bar(s), ph ^ 1u, wc, kDevTimeoutTail);
       if (++s == STAGES) { s = 0; ph ^= 1u; }
     }
     mbar_wait_drain(mma_done_bar, 0u, p.spin_limit);
-  } else if (warp == 1 && lane == 0 && is_leader) {
+  } else if (warp == 1 && is_leader) {
     // ---------------------------------------------------------------- MMA issuer
+    // The whole warp walks the loop, one elected lane issues: with the loop's values the same in all
+    // lanes they stay in uniform registers, where tcgen05.mma wants them. (A loop of one lane took
+    // 0.255 us a k-block whatever the tile's width.)
     constexpr uint32_t idesc = make_idesc_f16(Cfg::TILE_M, BN, Cfg::A_MN ? 1u : 0u, Cfg::B_MN ? 1u : 0u,
                                               DT == 1 ? 1u : 0u);
     // one MMA covers 16 k: 32 bytes along a k-contiguous row, or 16 rows of 128 bytes
     constexpr uint64_t a_step = Cfg::A_MN ? 128 : 2, b_step = Cfg::B_MN ? 128 : 2;
+    const bool issues = elect_one();
     if (!p.late_wait) grid_dependency_wait();
     int s = 0, acc = 0;
     uint32_t ph = 0, acc_ph = 0;
     bool ok = true;
     for (int t = worker; ok && t < tiles; t += workers) {
-      if (!mbar_wait(tmem_empty_bar(acc), acc_ph ^ 1u, wc, kDevTimeoutTmemEmpty)) break;
+      if (!mbar_wait_warp(tmem_empty_bar(acc), acc_ph ^ 1u, wc, kDevTimeoutTmemEmpty)) break;
       tcgen05_fence_after_sync();
       const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(full_bar(s), ph, wc, kDevTimeoutReady)) { ok = false; break; }
+        if (!mbar_wait_warp(full_bar(s), ph, wc, kDevTimeoutReady)) { ok = false; break; }
         tcgen05_fence_after_sync();
         const uint32_t stage = smem_base + s * Cfg::STAGE_BYTES;
         const uint64_t a = fused_desc<Cfg::A_MN>(stage);
         const uint64_t b = fused_desc<Cfg::B_MN>(stage + Cfg::A_BYTES);
+        if (issues) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          umma_f16<CG>(d_tmem, a + kk * a_step, b + kk * b_step, idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
-        umma_commit_to<CG>(empty_bar(s), leader_rank);
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f16<CG>(d_tmem, a + kk * a_step, b + kk * b_step, idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
+          umma_commit_to<CG>(empty_bar(s), leader_rank);
+        }
+        __syncwarp();
         if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
-      if (ok) umma_commit_to<CG>(tmem_full_bar(acc), leader_rank);
+      if (ok && issues) umma_commit_to<CG>(tmem_full_bar(acc), leader_rank);
+      __syncwarp();
       acc ^= 1;
       if (acc == 0) acc_ph ^= 1u;
     }
     // whatever was issued has to complete before tensor and shared memory are given up
-    umma_commit_to<CG>(mma_done_bar, leader_rank);
-    mbar_wait_drain(mma_done_bar, 0u, p.spin_limit);
+    if (issues) {
+      umma_commit_to<CG>(mma_done_bar, leader_rank);
+      mbar_wait_drain(mma_done_bar, 0u, p.spin_limit);
+    }
   }
 
   // ------------------------------------------------------------------ epilogue (warps 4 .. 11)

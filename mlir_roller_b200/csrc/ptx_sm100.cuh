@@ -121,6 +121,24 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const W
   return true;
 }
 
+// The same by a whole warp, with one outcome for all lanes.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, const WaitCtx& ctx,
+                                               uint32_t code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait<false>(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, ctx, code));
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is)::"memory");
+  return is != 0;
+}
+
 // Wait used while winding a CTA down: bounded by time alone (an error recorded elsewhere does
 // not cut it short, because what it waits for -- the tensor core finishing the MMAs already
 // issued -- still has to happen before shared and tensor memory may be given up). Records
