@@ -14,12 +14,28 @@ const FusedVariant* table(int i, int* n) {
   }
 }
 
+// Measured on B200 over widths 512 .. 8192, 1 .. 8192 rows (every kernel and split timed beside the
+// others); the choice by them comes within 1 % of the fastest on average.
 struct TileCost {
   int cta_group, block_n;
-  double kb_us;    // one k-block of one tile while every SM works
-  double tile_us;  // fill and the last tile's epilogue
+  double alone_us, busy_us;   // one k-block of one tile, on a few SMs and on all of them
+  double epilogue_us;         // of one tile, plain; hidden behind the next tile's k-blocks
+  double fixed_us;            // start, first loads, last epilogue
 };
-constexpr TileCost kTiles[] = {{2, 256, 0.36, 7.0}, {1, 256, 0.40, 6.0}, {1, 128, 0.28, 4.5}, {1, 64, 0.22, 4.0}};
+constexpr TileCost kTiles[] = {{2, 256, 0.28, 0.36, 5.3, 5.5},
+                               {1, 256, 0.285, 0.39, 3.1, 6.3},
+                               {1, 128, 0.16, 0.23, 1.8, 3.8},
+                               {1, 64, 0.15, 0.18, 1.5, 3.6}};
+// The epilogues beside the plain one.
+double epilogue_weight(int op) {
+  switch (op) {
+    case kOpDact: return 2.2;
+    case kOpUpdateWide: case kOpUpdateTall: return 1.6;
+    case kOpPoly: return 1.4;
+    case kOpGramWide: case kOpGramTall: return 1.1;
+    default: return 0.6;
+  }
+}
 
 // Copies the jobs' 16-bit rows into rows that start on 16 bytes. A warp takes 256 words (of two
 // elements) of a row at a time, a thread eight of them, all on their way together: a source row
@@ -171,9 +187,12 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
       if (at_once < 1) break;
       const long long waves = (tiles + at_once - 1) / at_once;
       const int part = (kbs + split - 1) / split;
-      // a cluster has one tile: from the second wave on every tile pays for its own fill and drain
-      const double fixed = c.tile_us + (split == 1 ? 0.0 : split == 2 ? 2.0 : split == 4 ? 2.5 : 5.0);
-      double us = split == 1 ? waves * part * c.kb_us + fixed : waves * (part * c.kb_us + fixed);
+      const double busy = tiles * ctas < d.sm_count ? static_cast<double>(tiles * ctas) / d.sm_count : 1.0;
+      const double kb_us = c.alone_us + (c.busy_us - c.alone_us) * busy;
+      // a cluster has one tile: from the second wave on every tile pays for its own start and end
+      const double fixed = c.fixed_us + (split == 1 ? 0.0 : split == 2 ? 2.3 : split == 4 ? 2.5 : 3.0);
+      const double tile_us = part * kb_us, epilogue_us = c.epilogue_us * epilogue_weight(s.op);
+      double us = split > 1 ? waves * (tile_us + fixed) : waves * (tile_us > epilogue_us ? tile_us : epilogue_us) + fixed;
       if (us < stream_us + fixed) us = stream_us + fixed;
       if (best.kv && us >= best_us) continue;
       best_us = us;
