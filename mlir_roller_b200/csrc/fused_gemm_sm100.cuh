@@ -195,576 +195,627 @@ __device__ __forceinline__ uint64_t fused_desc(uint32_t addr) {
   return MN ? make_smem_desc(addr, 8192, 1024, kLayoutSw128) : make_smem_desc(addr, 16, 1024, kLayoutSw128);
 }
 
+// Where a thread stands: addresses of the CTA's barriers and buffers, its role.
+struct FusedCta {
+  uint32_t smem_base, staging, ctrl, tmem_base;
+  int warp, lane;
+  int split;                  // parts of the cluster
+  uint32_t cluster_rank, cta_rank, part, leader_rank;
+  bool is_leader, epi;
+  int quarter, half;          // epilogue: TMEM lanes 32 quarter .., which half of the tile's columns
+  WaitCtx wc;
+  __device__ uint32_t full_bar(int s) const { return ctrl + 8u * s; }
+  __device__ uint32_t empty_bar(int s) const { return ctrl + 128u + 8u * s; }
+  __device__ uint32_t tmem_full_bar(int a) const { return ctrl + 256u + 8u * a; }
+  __device__ uint32_t tmem_empty_bar(int a) const { return ctrl + 272u + 8u * a; }
+  __device__ uint32_t mma_done_bar() const { return ctrl + 288u; }
+  __device__ uint32_t tmem_slot() const { return ctrl + 296u; }
+  __device__ uint32_t in_bar(int w) const { return ctrl + 304u + 8u * w; }   // a warp's inputs have landed
+};
+
+// How far a role has come in the rings it works on (stage, accumulator, inputs, result boxes).
+struct FusedRing {
+  int s = 0, acc = 0, box_at = 0;
+  uint32_t ph = 0, acc_ph = 0, in_ph = 0;
+  bool ok = true;
+};
+
+// Sets the CTA up: barriers and tensor memory. (Touches no global memory.)
 template <class Cfg>
-__global__ void __launch_bounds__(Cfg::THREADS, 1)
-fused_gemm_kernel(const __grid_constant__ FusedParams p) {
-  constexpr int BN = Cfg::BN, CG = Cfg::CG, STAGES = Cfg::STAGES, DT = Cfg::DT, OP = Cfg::OP;
-  extern __shared__ uint8_t smem_dyn[];
-  const uint32_t smem_base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
-  const uint32_t staging = smem_base + Cfg::RING_BYTES;
-  const uint32_t ctrl = staging + Cfg::STAGING_BYTES;
-  auto full_bar = [&](int s) { return ctrl + 8u * s; };
-  auto empty_bar = [&](int s) { return ctrl + 128u + 8u * s; };
-  auto tmem_full_bar = [&](int a) { return ctrl + 256u + 8u * a; };
-  auto tmem_empty_bar = [&](int a) { return ctrl + 272u + 8u * a; };
-  const uint32_t mma_done_bar = ctrl + 288u;
-  const uint32_t tmem_slot = ctrl + 296u;
-  auto in_bar = [&](int w) { return ctrl + 304u + 8u * w; };   // a warp's inputs have landed
-  const WaitCtx wc{p.status, p.spin_limit};
-
+__device__ __forceinline__ FusedCta fused_begin(uint8_t* smem_dyn, int split, uint32_t* status, long long spin_limit) {
+  FusedCta x;
+  x.smem_base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
+  x.staging = x.smem_base + Cfg::RING_BYTES;
+  x.ctrl = x.staging + Cfg::STAGING_BYTES;
+  x.wc = WaitCtx{status, spin_limit};
   // (the broadcast tells the compiler that the warp index is the same in all lanes)
-  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
-  const int lane = threadIdx.x & 31;
+  x.warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  x.lane = threadIdx.x & 31;
   // a cluster holds the `split` parts of one tile's k, each a CTA or a pair (ranks 2i and 2i + 1)
-  const int split = p.split;
-  const uint32_t cluster_rank = (CG == 2 || split > 1) ? cluster_ctarank() : 0u;
-  const uint32_t cta_rank = CG == 2 ? (cluster_rank & 1u) : 0u;
-  const uint32_t part = cluster_rank / CG;
-  const uint32_t leader_rank = cluster_rank - cta_rank;
-  const bool is_leader = (cta_rank == 0);
-
+  x.split = split;
+  x.cluster_rank = (Cfg::CG == 2 || split > 1) ? cluster_ctarank() : 0u;
+  x.cta_rank = Cfg::CG == 2 ? (x.cluster_rank & 1u) : 0u;
+  x.part = x.cluster_rank / Cfg::CG;
+  x.leader_rank = x.cluster_rank - x.cta_rank;
+  x.is_leader = x.cta_rank == 0;
+  x.epi = x.warp >= Cfg::FIRST_EPI_WARP;
+  x.quarter = x.warp & 3;
+  x.half = (x.warp - Cfg::FIRST_EPI_WARP) >> 2;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      mbar_init(x.full_bar(s), 1);
+      mbar_init(x.empty_bar(s), 1);
     }
     for (int a = 0; a < 2; ++a) {
-      mbar_init(tmem_full_bar(a), 1);
-      mbar_init(tmem_empty_bar(a), CG * Cfg::EPI_WARPS);
+      mbar_init(x.tmem_full_bar(a), 1);
+      mbar_init(x.tmem_empty_bar(a), Cfg::CG * Cfg::EPI_WARPS);
     }
-    mbar_init(mma_done_bar, 1);
-    for (int w = 0; w < Cfg::EPI_WARPS; ++w) mbar_init(in_bar(w), 1);
+    mbar_init(x.mma_done_bar(), 1);
+    for (int w = 0; w < Cfg::EPI_WARPS; ++w) mbar_init(x.in_bar(w), 1);
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc<CG>(tmem_slot, Cfg::TMEM_COLS);
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&p.a);
-    tma_prefetch_desc(&p.b[0]);
-    if (OP == kOpGate || OP == kOpDx) tma_prefetch_desc(&p.b[1]);
-    tma_prefetch_desc(&p.o[0]);
-  }
+  if (x.warp == 1) tmem_alloc<Cfg::CG>(x.tmem_slot(), Cfg::TMEM_COLS);
   tcgen05_fence_before_sync();
-  if constexpr (CG == 2) cluster_sync(); else __syncthreads();
+  if constexpr (Cfg::CG == 2) cluster_sync(); else __syncthreads();
   tcgen05_fence_after_sync();
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x.tmem_base) : "r"(x.tmem_slot()));
+  return x;
+}
 
-  uint32_t tmem_base;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
+// Ends the producer's work: the MMA issuer's last releases must land in this CTA before it may exit.
+template <class Cfg>
+__device__ __forceinline__ void fused_end_producer(const FusedCta& x, FusedRing& r) {
+  for (int i = 0; i < Cfg::STAGES && r.ok; ++i) {
+    r.ok = mbar_wait_warp(x.empty_bar(r.s), r.ph ^ 1u, x.wc, kDevTimeoutTail);
+    if (++r.s == Cfg::STAGES) { r.s = 0; r.ph ^= 1u; }
+  }
+  mbar_wait_drain(x.mma_done_bar(), 0u, x.wc.limit);
+}
+// Ends the MMA issuer's: what was issued has to complete before tensor and shared memory are given up.
+template <class Cfg>
+__device__ __forceinline__ void fused_end_mma(const FusedCta& x, bool issues) {
+  if (issues) {
+    umma_commit_to<Cfg::CG>(x.mma_done_bar(), x.leader_rank);
+    mbar_wait_drain(x.mma_done_bar(), 0u, x.wc.limit);
+  }
+}
+template <class Cfg>
+__device__ __forceinline__ void fused_end(const FusedCta& x) {
+  // stores handed to the TMA unit have to be performed before the CTA may go
+  if (x.epi && x.lane == 0) bulk_wait_all();
+  __syncwarp();
+  // after a failed wait some role left its loop early: let bulk copies on their way land
+  if (*reinterpret_cast<volatile uint32_t*>(x.wc.status) != kDevOk) abort_grace_period();
+  tcgen05_fence_before_sync();
+  if constexpr (Cfg::CG == 2) cluster_sync(); else __syncthreads();
+  if (x.warp == 1) {
+    tcgen05_fence_after_sync();
+    tmem_dealloc<Cfg::CG>(x.tmem_base, Cfg::TMEM_COLS);
+  }
+}
 
-  const int per_z = p.tiles_per_z;
-  const int tiles = per_z * p.zcount;
-  const int total_kb = p.num_kb * (OP == kOpDx ? 2 : 1);
+// One product, as the roles of a CTA see it.
+template <class Cfg>
+struct FusedWork {
+  static constexpr int BN = Cfg::BN, CG = Cfg::CG, STAGES = Cfg::STAGES, DT = Cfg::DT, OP = Cfg::OP;
+  const FusedParams& p;
+  const FusedCta& me;
+  int per_z, tiles, total_kb;
   // Tiles go round-robin to the CTAs, pairs or clusters; a CTA of a splitting cluster takes its part
   // of k, and its cluster has exactly one tile.
-  const int workers = static_cast<int>(gridDim.x) / (CG * split);
-  const int worker = static_cast<int>(blockIdx.x) / (CG * split);
-  const int kb0 = static_cast<int>(static_cast<long long>(total_kb) * part / split);
-  const int kb1 = static_cast<int>(static_cast<long long>(total_kb) * (part + 1) / split);
+  int workers, worker, kb0, kb1;
+  uint32_t in_boxes, boxes, tmem_lane;
 
-  bool epi_ok = true;
+  __device__ FusedWork(const FusedParams& p_, const FusedCta& me_) : p(p_), me(me_) {
+    per_z = p.tiles_per_z;
+    tiles = per_z * p.zcount;
+    total_kb = p.num_kb * (OP == kOpDx ? 2 : 1);
+    workers = static_cast<int>(gridDim.x) / (CG * me.split);
+    worker = static_cast<int>(blockIdx.x) / (CG * me.split);
+    kb0 = static_cast<int>(static_cast<long long>(total_kb) * me.part / me.split);
+    kb1 = static_cast<int>(static_cast<long long>(total_kb) * (me.part + 1) / me.split);
+    in_boxes = me.staging + static_cast<uint32_t>(me.warp - Cfg::FIRST_EPI_WARP) * (Cfg::WARP_BOXES * Cfg::BOX_BYTES);
+    boxes = in_boxes + Cfg::INPUTS * Cfg::BOX_BYTES;
+    tmem_lane = static_cast<uint32_t>(me.quarter * 32) << 16;
+  }
 
-  if (warp == 0) {
-    // ---------------------------------------------------------------- TMA producer
-    // (the whole warp walks the loop and one elected lane issues, as the MMA warp does)
-    const bool issues = elect_one();
+  // ---------------------------------------------------------------- TMA producer (warp 0)
+  // The whole warp walks the loop and one elected lane issues: with the loop's values the same in
+  // all lanes they stay in uniform registers, where tcgen05.mma and the TMA instructions want
+  // them. (Loops of one lane took 0.255 us a k-block whatever the tile's width.)
+  // before_loads: what has to be waited for in front of the first load (but p.b_early's).
+  template <class F>
+  __device__ __forceinline__ void produce(FusedRing& r, bool issues, F before_loads) {
     auto load_a = [&](int s, uint32_t bar, const FusedTile& c, int kb) {
       const int phase = (OP == kOpDx && kb >= p.num_kb) ? 1 : 0;
-      const int m0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM;
-      fused_load<Cfg::BM, Cfg::A_MN, CG == 2>(smem_base + s * Cfg::STAGE_BYTES, &p.a, bar, m0,
+      const int m0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM;
+      fused_load<Cfg::BM, Cfg::A_MN, CG == 2>(me.smem_base + s * Cfg::STAGE_BYTES, &p.a, bar, m0,
                                               (kb - phase * p.num_kb) * Cfg::BK, OP == kOpDx ? phase : c.z);
     };
     auto load_b = [&](int s, uint32_t bar, const FusedTile& c, int kb) {
-      const uint32_t b_dst = smem_base + s * Cfg::STAGE_BYTES + Cfg::A_BYTES;
+      const uint32_t b_dst = me.smem_base + s * Cfg::STAGE_BYTES + Cfg::A_BYTES;
       const int phase = (OP == kOpDx && kb >= p.num_kb) ? 1 : 0;
       const int k0 = (kb - phase * p.num_kb) * Cfg::BK;
       if constexpr (OP == kOpGate) {
         // tile columns: BN/2 rows of Wg, then the same BN/2 rows of Wu
         const int f0 = c.nb * (BN / 2);
         if constexpr (CG == 2) {
-          fused_load<Cfg::BNL, false, true>(b_dst, &p.b[cta_rank], bar, f0, k0, 0);
+          fused_load<Cfg::BNL, false, true>(b_dst, &p.b[me.cta_rank], bar, f0, k0, 0);
         } else {
           fused_load<BN / 2, false, false>(b_dst, &p.b[0], bar, f0, k0, 0);
           fused_load<BN / 2, false, false>(b_dst + Cfg::B_BYTES / 2, &p.b[1], bar, f0, k0, 0);
         }
       } else {
         const int bz = (OP == kOpDw || OP == kOpDx) ? 0 : c.z;
-        const int n0 = c.nb * BN + static_cast<int>(cta_rank) * Cfg::BNL;
+        const int n0 = c.nb * BN + static_cast<int>(me.cta_rank) * Cfg::BNL;
         fused_load<Cfg::BNL, Cfg::B_MN, CG == 2>(b_dst, &p.b[phase], bar, n0, k0, bz);
       }
     };
     // The barrier that counts the bytes of both operands (for a pair: of both CTAs, on the leader's,
     // which alone arms it).
-    auto counts = [&](int s) { return CG == 2 ? map_to_cta(full_bar(s), leader_rank) : full_bar(s); };
+    auto counts = [&](int s) { return CG == 2 ? map_to_cta(me.full_bar(s), me.leader_rank) : me.full_bar(s); };
     auto arm = [&](int s) {
       if constexpr (CG == 2) {
-        if (is_leader) mbar_expect_tx(full_bar(s), 2 * (Cfg::A_BYTES + Cfg::B_BYTES));
+        if (me.is_leader) mbar_expect_tx(me.full_bar(s), 2 * (Cfg::A_BYTES + Cfg::B_BYTES));
       } else {
-        mbar_expect_tx(full_bar(s), p.a_bytes + Cfg::B_BYTES);
+        mbar_expect_tx(me.full_bar(s), p.a_bytes + Cfg::B_BYTES);
       }
     };
-    int s = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    for (int t = worker; ok && t < tiles; t += workers) {
+    for (int t = worker; r.ok && t < tiles; t += workers) {
       const FusedTile c = fused_tile<Cfg::SYM ? Cfg::SYM_RATIO : 0>(t, p.tiles_m, p.tiles_n, per_z);
       int kb = kb0;
       if (t == worker) {
-        const int early = p.b_early ? min(STAGES, kb1 - kb0) : 0;
+        const int early = p.b_early ? min(STAGES, kb1 - kb0) : 0;    // (of a launch's first tiles)
         if (issues) {
           for (int i = 0; i < early; ++i) {
             arm(i);
             load_b(i, counts(i), c, kb + i);
           }
         }
-        if (!p.late_wait) grid_dependency_wait();
-        grid_launch_dependents();
+        if (!before_loads()) { r.ok = false; break; }
         if (issues)
           for (int i = 0; i < early; ++i) load_a(i, counts(i), c, kb + i);
         __syncwarp();
         kb += early;
-        s = early;
-        if (s == STAGES) { s = 0; ph ^= 1u; }
+        r.s += early;
+        if (r.s == STAGES) { r.s = 0; r.ph ^= 1u; }
       }
       for (; kb < kb1; ++kb) {
-        if (!mbar_wait_warp(empty_bar(s), ph ^ 1u, wc, kDevTimeoutEmpty)) { ok = false; break; }
+        if (!mbar_wait_warp(me.empty_bar(r.s), r.ph ^ 1u, me.wc, kDevTimeoutEmpty)) { r.ok = false; break; }
         if (issues) {
-          const uint32_t bar = counts(s);
-          arm(s);
-          load_a(s, bar, c, kb);
-          load_b(s, bar, c, kb);
+          const uint32_t bar = counts(r.s);
+          arm(r.s);
+          load_a(r.s, bar, c, kb);
+          load_b(r.s, bar, c, kb);
         }
         __syncwarp();
-        if (++s == STAGES) { s = 0; ph ^= 1u; }
+        if (++r.s == STAGES) { r.s = 0; r.ph ^= 1u; }
       }
     }
-    // the MMA issuer's last releases must land in this CTA before it may exit
-    for (int i = 0; i < STAGES && ok; ++i) {
-      ok = mbar_wait_warp(empty_bar(s), ph ^ 1u, wc, kDevTimeoutTail);
-      if (++s == STAGES) { s = 0; ph ^= 1u; }
-    }
-    mbar_wait_drain(mma_done_bar, 0u, p.spin_limit);
-  } else if (warp == 1 && is_leader) {
-    // ---------------------------------------------------------------- MMA issuer
-    // The whole warp walks the loop, one elected lane issues: with the loop's values the same in all
-    // lanes they stay in uniform registers, where tcgen05.mma wants them. (A loop of one lane took
-    // 0.255 us a k-block whatever the tile's width.)
+  }
+
+  // ---------------------------------------------------------------- MMA issuer (warp 1 of the leader)
+  __device__ __forceinline__ void multiply(FusedRing& r, bool issues) {
     constexpr uint32_t idesc = make_idesc_f16(Cfg::TILE_M, BN, Cfg::A_MN ? 1u : 0u, Cfg::B_MN ? 1u : 0u,
                                               DT == 1 ? 1u : 0u);
     // one MMA covers 16 k: 32 bytes along a k-contiguous row, or 16 rows of 128 bytes
     constexpr uint64_t a_step = Cfg::A_MN ? 128 : 2, b_step = Cfg::B_MN ? 128 : 2;
-    const bool issues = elect_one();
-    if (!p.late_wait) grid_dependency_wait();
-    int s = 0, acc = 0;
-    uint32_t ph = 0, acc_ph = 0;
-    bool ok = true;
-    for (int t = worker; ok && t < tiles; t += workers) {
-      if (!mbar_wait_warp(tmem_empty_bar(acc), acc_ph ^ 1u, wc, kDevTimeoutTmemEmpty)) break;
+    for (int t = worker; r.ok && t < tiles; t += workers) {
+      if (!mbar_wait_warp(me.tmem_empty_bar(r.acc), r.acc_ph ^ 1u, me.wc, kDevTimeoutTmemEmpty)) { r.ok = false; break; }
       tcgen05_fence_after_sync();
-      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+      const uint32_t d_tmem = me.tmem_base + static_cast<uint32_t>(r.acc * BN);
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_warp(full_bar(s), ph, wc, kDevTimeoutReady)) { ok = false; break; }
+        if (!mbar_wait_warp(me.full_bar(r.s), r.ph, me.wc, kDevTimeoutReady)) { r.ok = false; break; }
         tcgen05_fence_after_sync();
-        const uint32_t stage = smem_base + s * Cfg::STAGE_BYTES;
+        const uint32_t stage = me.smem_base + r.s * Cfg::STAGE_BYTES;
         const uint64_t a = fused_desc<Cfg::A_MN>(stage);
         const uint64_t b = fused_desc<Cfg::B_MN>(stage + Cfg::A_BYTES);
         if (issues) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             umma_f16<CG>(d_tmem, a + kk * a_step, b + kk * b_step, idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
-          umma_commit_to<CG>(empty_bar(s), leader_rank);
+          umma_commit_to<CG>(me.empty_bar(r.s), me.leader_rank);
         }
         __syncwarp();
-        if (++s == STAGES) { s = 0; ph ^= 1u; }
+        if (++r.s == STAGES) { r.s = 0; r.ph ^= 1u; }
       }
-      if (ok && issues) umma_commit_to<CG>(tmem_full_bar(acc), leader_rank);
+      if (r.ok && issues) umma_commit_to<CG>(me.tmem_full_bar(r.acc), me.leader_rank);
       __syncwarp();
-      acc ^= 1;
-      if (acc == 0) acc_ph ^= 1u;
-    }
-    // whatever was issued has to complete before tensor and shared memory are given up
-    if (issues) {
-      umma_commit_to<CG>(mma_done_bar, leader_rank);
-      mbar_wait_drain(mma_done_bar, 0u, p.spin_limit);
+      r.acc ^= 1;
+      if (r.acc == 0) r.acc_ph ^= 1u;
     }
   }
 
-  // ------------------------------------------------------------------ epilogue (warps 4 .. 11)
-  const bool epi = warp >= Cfg::FIRST_EPI_WARP;
-  const int quarter = warp & 3;                     // TMEM lanes 32 * (warp id mod 4)
-  const int half = (warp - Cfg::FIRST_EPI_WARP) >> 2;
-  const uint32_t in_boxes = staging + static_cast<uint32_t>(warp - Cfg::FIRST_EPI_WARP) * (Cfg::WARP_BOXES * Cfg::BOX_BYTES);
-  const uint32_t boxes = in_boxes + Cfg::INPUTS * Cfg::BOX_BYTES;
-  const uint32_t tmem_lane = static_cast<uint32_t>(quarter * 32) << 16;
-  int box_at = 0;      // ring of result boxes
-  uint32_t in_ph = 0;
-
-  auto load_d = [&](uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    tmem_ld_32x32(taddr, r);
-    tmem_ld_wait();
+  // ---------------------------------------------------------------- epilogue (warps 4 .. 11)
+  // split: the whole CTA calls this (it meets the cluster's others at barriers).
+  template <class F>
+  __device__ __forceinline__ void finish(FusedRing& r, F before_loads) {
+    auto load_d = [&](uint32_t taddr, float (&v)[32]) {
+      uint32_t r[32];
+      tmem_ld_32x32(taddr, r);
+      tmem_ld_wait();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-  };
-  // The inputs of one slab are sent for, and later taken into registers (16-bit pairs).
-  auto fetch = [&](const FusedTile& c, int row0, int col) {
-    __syncwarp();      // (every lane has taken the previous slab's)
-    if (lane == 0) {
-      const uint32_t bar = in_bar(warp - Cfg::FIRST_EPI_WARP);
-      mbar_expect_tx(bar, Cfg::INPUTS * Cfg::BOX_BYTES);
+      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+    };
+    // The inputs of one slab are sent for, and later taken into registers (16-bit pairs).
+    auto fetch = [&](const FusedTile& c, int row0, int col) {
+      __syncwarp();      // (every lane has taken the previous slab's)
+      if (me.lane == 0) {
+        const uint32_t bar = me.in_bar(me.warp - Cfg::FIRST_EPI_WARP);
+        mbar_expect_tx(bar, Cfg::INPUTS * Cfg::BOX_BYTES);
 #pragma unroll
-      for (int q = 0; q < Cfg::INPUTS; ++q) tma_load_3d(in_boxes + q * Cfg::BOX_BYTES, &p.i[q], bar, col, row0, c.z);
-    }
-  };
-  auto take = [&](uint32_t (&raw)[Cfg::INPUTS ? Cfg::INPUTS : 1][16]) {
-    const bool ok = __all_sync(0xffffffffu, mbar_wait(in_bar(warp - Cfg::FIRST_EPI_WARP), in_ph, wc, kDevTimeoutFull));
-    in_ph ^= 1u;
-#pragma unroll
-    for (int q = 0; q < Cfg::INPUTS; ++q)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(raw[q][4 * j]), "=r"(raw[q][4 * j + 1]), "=r"(raw[q][4 * j + 2]), "=r"(raw[q][4 * j + 3])
-                     : "r"(in_boxes + q * Cfg::BOX_BYTES + lane * 64 + (j ^ ((lane >> 1) & 3)) * 16)
-                     : "memory");
-    return ok;
-  };
-  // A staging box that the TMA unit has read (the one handed out RING boxes ago).
-  auto free_box = [&]() {
-    if (lane == 0) bulk_wait_read<Cfg::RING - 1>();
-    __syncwarp();
-    const uint32_t b = boxes + static_cast<uint32_t>(box_at) * Cfg::BOX_BYTES;
-    box_at = box_at + 1 == Cfg::RING ? 0 : box_at + 1;
-    return b;
-  };
-  // 32 columns of this warp's 32 rows, as 16-bit values, into a box ...
-  auto put = [&](uint32_t box, const float (&v)[32], bool as_bf16) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = (as_bf16 && DT != 1) ? fused_pack<1>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1])
-                                    : fused_pack<DT>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
-      // 64-byte swizzle: 16-byte chunks of a 64-byte row, exchanged by bits 1..2 of the row
-      const int chunk = j ^ ((lane >> 1) & 3);
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 64 + chunk * 16),
-                   "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                   : "memory");
-    }
-  };
-  // ... and from there to columns col.. of output `o`.
-  auto emit = [&](int o, const FusedTile& c, int row0, int col, const float (&v)[32], bool as_bf16) {
-    const uint32_t box = free_box();
-    put(box, v, as_bf16);
-    const int oz = OP == kOpDw ? 0 : c.z;
-    if (p.out_tma & (1 << o)) {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        if (row0 < p.M) tma_store_3d(&p.o[o], box, col, row0, oz);
-        bulk_commit_group();
-      }
-    } else {
-      // rows that start anywhere: a warp writes 32 consecutive elements per instruction
-      __syncwarp();
-      uint16_t* dst = static_cast<uint16_t*>(p.out[o]) + oz * p.out_zstride + static_cast<long long>(row0) * p.out_ld[o] + col + lane;
-      const int rows = col + lane < p.out_cols ? p.M - row0 : 0;
-#pragma unroll 1
-      for (int r0 = 0; r0 < 32; r0 += 8) {
-        uint16_t x[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          asm volatile("ld.shared.u16 %0, [%1];"
-                       : "=h"(x[r])
-                       : "r"(box + (r0 + r) * 64 + (((lane >> 3) ^ (((r0 + r) >> 1) & 3)) * 16) + (lane & 7) * 2)
-                       : "memory");
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (r0 + r < rows) dst[(r0 + r) * p.out_ld[o]] = x[r];
-      }
-      if (lane == 0) bulk_commit_group();   // (an empty group keeps the ring's count)
-    }
-  };
-  // The first n boxes to outputs 0 .. n - 1, which are the library's own, aligned memory.
-  auto hand_over = [&](int n, const FusedTile& c, int row0, int col) {
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      if (row0 < p.M)
-        for (int o = 0; o < n; ++o) tma_store_3d(&p.o[o], boxes + o * Cfg::BOX_BYTES, col, row0, c.z);
-      bulk_commit_group();
-    }
-  };
-  // The mirror image of 32 x 32 elements of a symmetric fp16 matrix (its own box has no swizzle).
-  // Neighbouring lanes exchange halves, so that each word holds two neighbouring columns.
-  auto emit_mirror = [&](const FusedTile& c, int row0, int col, const float (&v)[32]) {
-    const uint32_t box = free_box();
-    const bool odd = lane & 1;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t ab = fused_pack<DT>(v[2 * j], v[2 * j + 1]);
-      const uint32_t got = __shfl_xor_sync(0xffffffffu, ab, 1);
-      const uint32_t word = odd ? __byte_perm(got, ab, 0x7632) : __byte_perm(ab, got, 0x5410);
-      asm volatile("st.shared.b32 [%0], %1;" ::"r"(box + (2 * j + odd) * 64 + (lane >> 1) * 4), "r"(word) : "memory");
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      if (row0 < p.M) tma_store_3d(&p.o[1], box, row0, col, c.z);
-      bulk_commit_group();
-    }
-  };
-
-  // Whether a slab has anything to do (it decides whether inputs are sent for).
-  auto wanted = [&](int row0, int col) { return col < p.out_cols && (!Cfg::SYM || col <= row0); };
-
-  // The epilogue of this warp's slabs slab0, slab0 + step, .. < slab_end of tile `c`. Slab i is the 32
-  // result columns from tile column 32 i on; `sums(tile_col, v)` gives 32 columns of D.
-  // The first slab's inputs have been sent for.
-  auto epilogue = [&](const FusedTile& c, int slab0, int step, int slab_end, auto sums) {
-    const int row0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32;
-    const int row = row0 + lane;
-    const int col_base = c.nb * (OP == kOpGate ? BN / 2 : BN);
-    auto run = [&](auto act_tag) {
-      constexpr int ACT = decltype(act_tag)::value;
-#pragma unroll 1
-      for (int i = slab0; i < slab_end; i += step) {
-        const int tc = i * 32, col = col_base + tc;
-        // (uniform over the warp; above the diagonal a slab is the mirror image of another one)
-        if (!wanted(row0, col)) break;
-        float v[32];
-        uint32_t raw[Cfg::INPUTS ? Cfg::INPUTS : 1][16];
-        if constexpr (Cfg::INPUTS > 0) {
-          epi_ok = take(raw) && epi_ok;
-          // the next slab's inputs are on their way while this one is worked on
-          if (i + step < slab_end && wanted(row0, col + step * 32)) fetch(c, row0, col + step * 32);
-        }
-        auto input = [&](int q, int k) {      // element k of input q
-          const float2 f = fused_unpack<DT>(raw[q][k / 2]);
-          return k & 1 ? f.y : f.x;
-        };
-        if constexpr (OP == kOpGate) {
-          float w[32];
-          sums(tc, v);
-          sums(tc + BN / 2, w);
-          if (p.flags & kFusedSave) {
-            emit(1, c, row0, col, v, false);
-            emit(2, c, row0, col, w, false);
-          }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float y, slope;
-            activation<ACT>(v[j], y, slope);
-            v[j] = y * w[j];
-          }
-          emit(0, c, row0, col, v, false);
-        } else if constexpr (OP == kOpDact) {
-          float du[32], h[32];
-          sums(tc, v);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float y, slope;
-            activation<ACT>(input(0, j), y, slope);
-            const float dh = v[j], uu = input(1, j);
-            v[j] = dh * uu * slope;    // dg
-            du[j] = dh * y;
-            h[j] = y * uu;
-          }
-          if (lane == 0) bulk_wait_read_all();
-          __syncwarp();
-          put(boxes, v, false);
-          put(boxes + Cfg::BOX_BYTES, du, false);
-          put(boxes + 2 * Cfg::BOX_BYTES, h, false);
-          hand_over(3, c, row0, col);
-        } else if constexpr (OP == kOpDown || OP == kOpDx || OP == kOpDw) {
-          sums(tc, v);
-          emit(OP == kOpDw ? c.z : 0, c, row0, col, v, false);
-        } else if constexpr (Cfg::SYM) {
-          if constexpr (OP == kOpPoly) {
-            sums(tc, v);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = p.coef_b * input(0, j) + p.coef_c * v[j];
-            // what rounding q's diagonal to 16 bits loses is as large as the rest of that
-            // rounding together: it goes into the vector that scales x instead
-            const int dj = row - col;
-            if (row < p.M && dj >= 0 && dj < 32) {
-              float x = 0.0f;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) x = (j == dj) ? v[j] : x;
-              p.vec[c.z * p.vec_ld + row] = p.coef_a + (x - __half2float(__float2half_rn(x))) * p.inv_scale;
-            }
-          } else {
-            sums(tc, v);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
-          }
-          emit(0, c, row0, col, v, false);
-          if (col < row0) emit_mirror(c, row0, col, v);
-        } else {
-          sums(tc, v);
-          if constexpr (OP == kOpUpdateWide) {
-            const float d = row < p.M ? p.vec[c.z * p.vec_ld + row] : 0.0f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = d * (input(0, j) + input(1, j)) + v[j] * p.inv_scale;
-          } else {
-            // (rows of vec are padded to 64; what lies in the padding meets columns that are not stored)
-            const float4* d4 = reinterpret_cast<const float4*>(p.vec + c.z * p.vec_ld + col);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float4 d = __ldg(d4 + j);
-              v[4 * j] = d.x * (input(0, 4 * j) + input(1, 4 * j)) + v[4 * j] * p.inv_scale;
-              v[4 * j + 1] = d.y * (input(0, 4 * j + 1) + input(1, 4 * j + 1)) + v[4 * j + 1] * p.inv_scale;
-              v[4 * j + 2] = d.z * (input(0, 4 * j + 2) + input(1, 4 * j + 2)) + v[4 * j + 2] * p.inv_scale;
-              v[4 * j + 3] = d.w * (input(0, 4 * j + 3) + input(1, 4 * j + 3)) + v[4 * j + 3] * p.inv_scale;
-            }
-          }
-          if (p.flags & kFusedLast) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
-            emit(0, c, row0, col, v, true);
-          } else {
-            if (lane == 0) bulk_wait_read_all();
-            __syncwarp();
-            put(boxes, v, false);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
-            put(boxes + Cfg::BOX_BYTES, v, false);
-            hand_over(2, c, row0, col);
-          }
-        }
+        for (int q = 0; q < Cfg::INPUTS; ++q) tma_load_3d(in_boxes + q * Cfg::BOX_BYTES, &p.i[q], bar, col, row0, c.z);
       }
     };
-    if constexpr (OP == kOpGate || OP == kOpDact) {
-      if (p.act == kActSilu) run(IntTag<kActSilu>{});
-      else if (p.act == kActGelu) run(IntTag<kActGelu>{});
-      else run(IntTag<kActGeluTanh>{});
-    } else {
-      run(IntTag<0>{});
-    }
-  };
-
-  constexpr int kSlabs = Cfg::OUT_COLS / 32;     // slabs of one warp of a whole tile
-
-  if (epi && split == 1) {
-    if (!p.late_wait) grid_dependency_wait();
-    int acc = 0;
-    uint32_t acc_ph = 0;
-    for (int t = worker; epi_ok && t < tiles; t += workers) {
-      const FusedTile c = fused_tile<Cfg::SYM ? Cfg::SYM_RATIO : 0>(t, p.tiles_m, p.tiles_n, per_z);
-      if constexpr (Cfg::INPUTS > 0) {     // they do not depend on the product
-        const int col = c.nb * BN + half * Cfg::OUT_COLS;
-        const int row0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32;
-        if (wanted(row0, col)) fetch(c, row0, col);
-      }
-      epi_ok = __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(acc), acc_ph, wc, kDevTimeoutTmemFull));
-      if (!epi_ok) break;
-      tcgen05_fence_after_sync();
-      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN) + tmem_lane;
-      epilogue(c, half * kSlabs, 1, (half + 1) * kSlabs,
-               [&](int tc, float (&v)[32]) { load_d(d_tmem + tc, v); });
-      tcgen05_fence_before_sync();
+    auto take = [&](uint32_t (&raw)[Cfg::INPUTS ? Cfg::INPUTS : 1][16]) {
+      const bool ok = __all_sync(0xffffffffu, mbar_wait(me.in_bar(me.warp - Cfg::FIRST_EPI_WARP), r.in_ph, me.wc, kDevTimeoutFull));
+      r.in_ph ^= 1u;
+#pragma unroll
+      for (int q = 0; q < Cfg::INPUTS; ++q)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(raw[q][4 * j]), "=r"(raw[q][4 * j + 1]), "=r"(raw[q][4 * j + 2]), "=r"(raw[q][4 * j + 3])
+                       : "r"(in_boxes + q * Cfg::BOX_BYTES + me.lane * 64 + (j ^ ((me.lane >> 1) & 3)) * 16)
+                       : "memory");
+      return ok;
+    };
+    // A staging box that the TMA unit has read (the one handed out RING boxes ago).
+    auto free_box = [&]() {
+      if (me.lane == 0) bulk_wait_read<Cfg::RING - 1>();
       __syncwarp();
-      if (lane == 0) {
-        if constexpr (CG == 2) mbar_arrive_cluster(tmem_empty_bar(acc), leader_rank);
-        else mbar_arrive(tmem_empty_bar(acc));
-      }
-      acc ^= 1;
-      if (acc == 0) acc_ph ^= 1u;
-    }
-  }
-
-  if (split > 1) {
-    // ---- the cluster holds the tile's parts: their sums are put together, each CTA taking a share
-    // of the slabs: slab i is received by part i / share, or by every `apart`-th part
-    const FusedTile c = fused_tile<Cfg::SYM ? Cfg::SYM_RATIO : 0>(worker, p.tiles_m, p.tiles_n, per_z);
-    const int row0 = (c.mb * CG + static_cast<int>(cta_rank)) * Cfg::BM + quarter * 32;
-    const bool row_ok = row0 + lane < p.M;
-    const int share = max(Cfg::SLABS / split, 1), apart = max(split / Cfg::SLABS, 1);
-    const int my_slab = static_cast<int>(part) / apart * share;
-    const bool receives = static_cast<int>(part) % apart == 0 && half < share;
-    if (epi) {
-      if (!p.late_wait) grid_dependency_wait();
-      if constexpr (Cfg::INPUTS > 0) {
-        const int col = c.nb * BN + (my_slab + half) * 32;
-        if (receives && wanted(row0, col)) fetch(c, row0, col);
-      }
-      epi_ok = __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(0), 0u, wc, kDevTimeoutTmemFull));
-    }
-    __syncwarp();
-    cluster_sync();      // all MMAs of the cluster are done: the rings' memory is free
-    // Exchange area of a CTA: [sender][32-column group][4 columns][row] float4. The gate has two
-    // groups per slab (g, then u).
-    constexpr int kGroups = OP == kOpGate ? 2 : 1;
-    const uint32_t sender_bytes = static_cast<uint32_t>(share * kGroups) * 16384u;
-    const uint32_t lane_at = static_cast<uint32_t>(quarter * 32 + lane) * 16u;
-    if (epi && epi_ok) {
-      tcgen05_fence_after_sync();
-      for (int i = half; i < Cfg::SLABS; i += 2) {
-        const uint32_t to = static_cast<uint32_t>(i / share * apart);
-        if (to == part) continue;
-        // senders in the order of k, the receiver itself left out
-        const uint32_t place = part - (part > to ? 1u : 0u);
+      const uint32_t b = boxes + static_cast<uint32_t>(r.box_at) * Cfg::BOX_BYTES;
+      r.box_at = r.box_at + 1 == Cfg::RING ? 0 : r.box_at + 1;
+      return b;
+    };
+    // 32 columns of this warp's 32 rows, as 16-bit values, into a box ...
+    auto put = [&](uint32_t box, const float (&v)[32], bool as_bf16) {
 #pragma unroll
-        for (int q = 0; q < kGroups; ++q) {
-          float v[32];
-          load_d(tmem_base + tmem_lane + i * 32 + q * (BN / 2), v);
-          if (row_ok) {
-            const uint32_t dst = map_to_cta(
-                smem_base + place * sender_bytes + static_cast<uint32_t>((i % share) * kGroups + q) * 16384u + lane_at,
-                to * CG + cta_rank);
+      for (int j = 0; j < 4; ++j) {
+        uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + j * 2048u),
-                           "f"(v[4 * j]), "f"(v[4 * j + 1]), "f"(v[4 * j + 2]), "f"(v[4 * j + 3])
-                           : "memory");
-          }
+        for (int i = 0; i < 4; ++i)
+          w[i] = (as_bf16 && DT != 1) ? fused_pack<1>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1])
+                                      : fused_pack<DT>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
+        // 64-byte swizzle: 16-byte chunks of a 64-byte row, exchanged by bits 1..2 of the row
+        const int chunk = j ^ ((me.lane >> 1) & 3);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + me.lane * 64 + chunk * 16),
+                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                     : "memory");
+      }
+    };
+    // ... and from there to columns col.. of output `o`.
+    auto emit = [&](int o, const FusedTile& c, int row0, int col, const float (&v)[32], bool as_bf16) {
+      const uint32_t box = free_box();
+      put(box, v, as_bf16);
+      const int oz = OP == kOpDw ? 0 : c.z;
+      if (p.out_tma & (1 << o)) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (me.lane == 0) {
+          if (row0 < p.M) tma_store_3d(&p.o[o], box, col, row0, oz);
+          bulk_commit_group();
         }
+      } else {
+        // rows that start anywhere: a warp writes 32 consecutive elements per instruction
+        __syncwarp();
+        uint16_t* dst = static_cast<uint16_t*>(p.out[o]) + oz * p.out_zstride + static_cast<long long>(row0) * p.out_ld[o] + col + me.lane;
+        const int rows = col + me.lane < p.out_cols ? p.M - row0 : 0;
+#pragma unroll 1
+        for (int r0 = 0; r0 < 32; r0 += 8) {
+          uint16_t x[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            asm volatile("ld.shared.u16 %0, [%1];"
+                         : "=h"(x[r])
+                         : "r"(box + (r0 + r) * 64 + (((me.lane >> 3) ^ (((r0 + r) >> 1) & 3)) * 16) + (me.lane & 7) * 2)
+                         : "memory");
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (r0 + r < rows) dst[(r0 + r) * p.out_ld[o]] = x[r];
+        }
+        if (me.lane == 0) bulk_commit_group();   // (an empty group keeps the ring's count)
       }
-    }
-    __syncwarp();
-    cluster_sync();
-    if (epi && epi_ok && receives) {
-      epilogue(c, my_slab + half, 2, my_slab + share, [&](int tc, float (&v)[32]) {
-        const int q = (OP == kOpGate && tc >= BN / 2) ? 1 : 0;
-        const int i = (tc - q * (BN / 2)) / 32 - my_slab;
-        float own[32];
-        load_d(tmem_base + tmem_lane + tc, own);
+    };
+    // The first n boxes to outputs 0 .. n - 1, which are the library's own, aligned memory.
+    auto hand_over = [&](int n, const FusedTile& c, int row0, int col) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (me.lane == 0) {
+        if (row0 < p.M)
+          for (int o = 0; o < n; ++o) tma_store_3d(&p.o[o], boxes + o * Cfg::BOX_BYTES, col, row0, c.z);
+        bulk_commit_group();
+      }
+    };
+    // The mirror image of 32 x 32 elements of a symmetric fp16 matrix (its own box has no swizzle).
+    // Neighbouring lanes exchange halves, so that each word holds two neighbouring columns.
+    auto emit_mirror = [&](const FusedTile& c, int row0, int col, const float (&v)[32]) {
+      const uint32_t box = free_box();
+      const bool odd = me.lane & 1;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-        for (int r = 0; r < split; ++r) {
-          if (r == static_cast<int>(part)) {
+      for (int j = 0; j < 16; ++j) {
+        const uint32_t ab = fused_pack<DT>(v[2 * j], v[2 * j + 1]);
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, ab, 1);
+        const uint32_t word = odd ? __byte_perm(got, ab, 0x7632) : __byte_perm(ab, got, 0x5410);
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(box + (2 * j + odd) * 64 + (me.lane >> 1) * 4), "r"(word) : "memory");
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (me.lane == 0) {
+        if (row0 < p.M) tma_store_3d(&p.o[1], box, row0, col, c.z);
+        bulk_commit_group();
+      }
+    };
+
+    // Whether a slab has anything to do (it decides whether inputs are sent for).
+    auto wanted = [&](int row0, int col) { return col < p.out_cols && (!Cfg::SYM || col <= row0); };
+
+    // The epilogue of this warp's slabs slab0, slab0 + step, .. < slab_end of tile `c`. Slab i is the 32
+    // result columns from tile column 32 i on; `sums(tile_col, v)` gives 32 columns of D.
+    // The first slab's inputs have been sent for.
+    auto epilogue = [&](const FusedTile& c, int slab0, int step, int slab_end, auto sums) {
+      const int row0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM + me.quarter * 32;
+      const int row = row0 + me.lane;
+      const int col_base = c.nb * (OP == kOpGate ? BN / 2 : BN);
+      auto run = [&](auto act_tag) {
+        constexpr int ACT = decltype(act_tag)::value;
+#pragma unroll 1
+        for (int i = slab0; i < slab_end; i += step) {
+          const int tc = i * 32, col = col_base + tc;
+          // (uniform over the warp; above the diagonal a slab is the mirror image of another one)
+          if (!wanted(row0, col)) break;
+          float v[32];
+          uint32_t raw[Cfg::INPUTS ? Cfg::INPUTS : 1][16];
+          if constexpr (Cfg::INPUTS > 0) {
+            r.ok = take(raw) && r.ok;
+            // the next slab's inputs are on their way while this one is worked on
+            if (i + step < slab_end && wanted(row0, col + step * 32)) fetch(c, row0, col + step * 32);
+          }
+          auto input = [&](int q, int k) {      // element k of input q
+            const float2 f = fused_unpack<DT>(raw[q][k / 2]);
+            return k & 1 ? f.y : f.x;
+          };
+          if constexpr (OP == kOpGate) {
+            float w[32];
+            sums(tc, v);
+            sums(tc + BN / 2, w);
+            if (p.flags & kFusedSave) {
+              emit(1, c, row0, col, v, false);
+              emit(2, c, row0, col, w, false);
+            }
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] += own[j];
-          } else if (row_ok) {
-            const uint32_t src = smem_base + static_cast<uint32_t>(r - (r > static_cast<int>(part) ? 1 : 0)) * sender_bytes +
-                                 static_cast<uint32_t>(i * kGroups + q) * 16384u + lane_at;
+            for (int j = 0; j < 32; ++j) {
+              float y, slope;
+              activation<ACT>(v[j], y, slope);
+              v[j] = y * w[j];
+            }
+            emit(0, c, row0, col, v, false);
+          } else if constexpr (OP == kOpDact) {
+            float du[32], h[32];
+            sums(tc, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              float4 x;
-              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                           : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
-                           : "r"(src + j * 2048u)
-                           : "memory");
-              v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
+            for (int j = 0; j < 32; ++j) {
+              float y, slope;
+              activation<ACT>(input(0, j), y, slope);
+              const float dh = v[j], uu = input(1, j);
+              v[j] = dh * uu * slope;    // dg
+              du[j] = dh * y;
+              h[j] = y * uu;
+            }
+            if (me.lane == 0) bulk_wait_read_all();
+            __syncwarp();
+            put(boxes, v, false);
+            put(boxes + Cfg::BOX_BYTES, du, false);
+            put(boxes + 2 * Cfg::BOX_BYTES, h, false);
+            hand_over(3, c, row0, col);
+          } else if constexpr (OP == kOpDown || OP == kOpDx || OP == kOpDw) {
+            sums(tc, v);
+            emit(OP == kOpDw ? c.z : 0, c, row0, col, v, false);
+          } else if constexpr (Cfg::SYM) {
+            if constexpr (OP == kOpPoly) {
+              sums(tc, v);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = p.coef_b * input(0, j) + p.coef_c * v[j];
+              // what rounding q's diagonal to 16 bits loses is as large as the rest of that
+              // rounding together: it goes into the vector that scales x instead
+              const int dj = row - col;
+              if (row < p.M && dj >= 0 && dj < 32) {
+                float x = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x = (j == dj) ? v[j] : x;
+                p.vec[c.z * p.vec_ld + row] = p.coef_a + (x - __half2float(__float2half_rn(x))) * p.inv_scale;
+              }
+            } else {
+              sums(tc, v);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
+            }
+            emit(0, c, row0, col, v, false);
+            if (col < row0) emit_mirror(c, row0, col, v);
+          } else {
+            sums(tc, v);
+            if constexpr (OP == kOpUpdateWide) {
+              const float d = row < p.M ? p.vec[c.z * p.vec_ld + row] : 0.0f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = d * (input(0, j) + input(1, j)) + v[j] * p.inv_scale;
+            } else {
+              // (rows of vec are padded to 64; what lies in the padding meets columns that are not stored)
+              const float4* d4 = reinterpret_cast<const float4*>(p.vec + c.z * p.vec_ld + col);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float4 d = __ldg(d4 + j);
+                v[4 * j] = d.x * (input(0, 4 * j) + input(1, 4 * j)) + v[4 * j] * p.inv_scale;
+                v[4 * j + 1] = d.y * (input(0, 4 * j + 1) + input(1, 4 * j + 1)) + v[4 * j + 1] * p.inv_scale;
+                v[4 * j + 2] = d.z * (input(0, 4 * j + 2) + input(1, 4 * j + 2)) + v[4 * j + 2] * p.inv_scale;
+                v[4 * j + 3] = d.w * (input(0, 4 * j + 3) + input(1, 4 * j + 3)) + v[4 * j + 3] * p.inv_scale;
+              }
+            }
+            if (p.flags & kFusedLast) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
+              emit(0, c, row0, col, v, true);
+            } else {
+              if (me.lane == 0) bulk_wait_read_all();
+              __syncwarp();
+              put(boxes, v, false);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
+              put(boxes + Cfg::BOX_BYTES, v, false);
+              hand_over(2, c, row0, col);
             }
           }
         }
-      });
+      };
+      if constexpr (OP == kOpGate || OP == kOpDact) {
+        if (p.act == kActSilu) run(IntTag<kActSilu>{});
+        else if (p.act == kActGelu) run(IntTag<kActGelu>{});
+        else run(IntTag<kActGeluTanh>{});
+      } else {
+        run(IntTag<0>{});
+      }
+    };
+
+    constexpr int kSlabs = Cfg::OUT_COLS / 32;     // slabs of one warp of a whole tile
+
+    if (me.split == 1) {
+      if (!before_loads()) r.ok = false;
+      for (int t = worker; r.ok && t < tiles; t += workers) {
+        const FusedTile c = fused_tile<Cfg::SYM ? Cfg::SYM_RATIO : 0>(t, p.tiles_m, p.tiles_n, per_z);
+        if constexpr (Cfg::INPUTS > 0) {     // they do not depend on the product
+          const int col = c.nb * BN + me.half * Cfg::OUT_COLS;
+          const int row0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM + me.quarter * 32;
+          if (wanted(row0, col)) fetch(c, row0, col);
+        }
+        r.ok = __all_sync(0xffffffffu, mbar_wait(me.tmem_full_bar(r.acc), r.acc_ph, me.wc, kDevTimeoutTmemFull));
+        if (!r.ok) break;
+        tcgen05_fence_after_sync();
+        const uint32_t d_tmem = me.tmem_base + static_cast<uint32_t>(r.acc * BN) + tmem_lane;
+        epilogue(c, me.half * kSlabs, 1, (me.half + 1) * kSlabs,
+                 [&](int tc, float (&v)[32]) { load_d(d_tmem + tc, v); });
+        tcgen05_fence_before_sync();
+        __syncwarp();
+        if (me.lane == 0) {
+          if constexpr (CG == 2) mbar_arrive_cluster(me.tmem_empty_bar(r.acc), me.leader_rank);
+          else mbar_arrive(me.tmem_empty_bar(r.acc));
+        }
+        r.acc ^= 1;
+        if (r.acc == 0) r.acc_ph ^= 1u;
+      }
+    } else {
+      // ---- the cluster holds the tile's parts: their sums are put together, each CTA taking a share
+      // of the slabs: slab i is received by part i / share, or by every `apart`-th part
+      const FusedTile c = fused_tile<Cfg::SYM ? Cfg::SYM_RATIO : 0>(worker, p.tiles_m, p.tiles_n, per_z);
+      const int row0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM + me.quarter * 32;
+      const bool row_ok = row0 + me.lane < p.M;
+      const int share = max(Cfg::SLABS / me.split, 1), apart = max(me.split / Cfg::SLABS, 1);
+      const int my_slab = static_cast<int>(me.part) / apart * share;
+      const bool receives = static_cast<int>(me.part) % apart == 0 && me.half < share;
+      if (me.epi) {
+        before_loads();
+        if constexpr (Cfg::INPUTS > 0) {
+          const int col = c.nb * BN + (my_slab + me.half) * 32;
+          if (receives && wanted(row0, col)) fetch(c, row0, col);
+        }
+        r.ok = __all_sync(0xffffffffu, mbar_wait(me.tmem_full_bar(0), 0u, me.wc, kDevTimeoutTmemFull));
+      }
+      __syncwarp();
+      cluster_sync();      // all MMAs of the cluster are done: the rings' memory is free
+      // Exchange area of a CTA: [sender][32-column group][4 columns][row] float4. The gate has two
+      // groups per slab (g, then u).
+      constexpr int kGroups = OP == kOpGate ? 2 : 1;
+      const uint32_t sender_bytes = static_cast<uint32_t>(share * kGroups) * 16384u;
+      const uint32_t lane_at = static_cast<uint32_t>(me.quarter * 32 + me.lane) * 16u;
+      if (me.epi && r.ok) {
+        tcgen05_fence_after_sync();
+        for (int i = me.half; i < Cfg::SLABS; i += 2) {
+          const uint32_t to = static_cast<uint32_t>(i / share * apart);
+          if (to == me.part) continue;
+          // senders in the order of k, the receiver itself left out
+          const uint32_t place = me.part - (me.part > to ? 1u : 0u);
+#pragma unroll
+          for (int q = 0; q < kGroups; ++q) {
+            float v[32];
+            load_d(me.tmem_base + tmem_lane + i * 32 + q * (BN / 2), v);
+            if (row_ok) {
+              const uint32_t dst = map_to_cta(
+                  me.smem_base + place * sender_bytes + static_cast<uint32_t>((i % share) * kGroups + q) * 16384u + lane_at,
+                  to * CG + me.cta_rank);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + j * 2048u),
+                             "f"(v[4 * j]), "f"(v[4 * j + 1]), "f"(v[4 * j + 2]), "f"(v[4 * j + 3])
+                             : "memory");
+            }
+          }
+        }
+      }
+      __syncwarp();
+      cluster_sync();
+      if (me.epi && r.ok && receives) {
+        epilogue(c, my_slab + me.half, 2, my_slab + share, [&](int tc, float (&v)[32]) {
+          const int q = (OP == kOpGate && tc >= BN / 2) ? 1 : 0;
+          const int i = (tc - q * (BN / 2)) / 32 - my_slab;
+          float own[32];
+          load_d(me.tmem_base + tmem_lane + tc, own);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+          for (int r = 0; r < me.split; ++r) {
+            if (r == static_cast<int>(me.part)) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] += own[j];
+            } else if (row_ok) {
+              const uint32_t src = me.smem_base + static_cast<uint32_t>(r - (r > static_cast<int>(me.part) ? 1 : 0)) * sender_bytes +
+                                   static_cast<uint32_t>(i * kGroups + q) * 16384u + lane_at;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                float4 x;
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                             : "r"(src + j * 2048u)
+                             : "memory");
+                v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
+              }
+            }
+          }
+        });
+      }
     }
   }
+};
 
-  // ------------------------------------------------------------------ teardown
-  // stores handed to the TMA unit have to be performed before the CTA may go
-  if (epi && lane == 0) bulk_wait_all();
-  if (p.late_wait) grid_dependency_wait();
-  __syncwarp();
-  // after a failed wait some role left its loop early: let bulk copies on their way land
-  if (*reinterpret_cast<volatile uint32_t*>(p.status) != kDevOk) abort_grace_period();
-  tcgen05_fence_before_sync();
-  if constexpr (CG == 2) cluster_sync(); else __syncthreads();
-  if (warp == 1) {
-    tcgen05_fence_after_sync();
-    tmem_dealloc<CG>(tmem_base, Cfg::TMEM_COLS);
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::THREADS, 1)
+fused_gemm_kernel(const __grid_constant__ FusedParams p) {
+  extern __shared__ uint8_t smem_dyn[];
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&p.a);
+    tma_prefetch_desc(&p.b[0]);
+    if (Cfg::OP == kOpGate || Cfg::OP == kOpDx) tma_prefetch_desc(&p.b[1]);
+    tma_prefetch_desc(&p.o[0]);
   }
+  const FusedCta x = fused_begin<Cfg>(smem_dyn, p.split, p.status, p.spin_limit);
+  FusedWork<Cfg> work(p, x);
+  FusedRing r;
+  auto previous = [&]() {
+    if (!p.late_wait) grid_dependency_wait();
+    return true;
+  };
+  if (x.warp == 0) {
+    work.produce(r, elect_one(), [&]() {
+      previous();
+      grid_launch_dependents();
+      return true;
+    });
+    fused_end_producer<Cfg>(x, r);
+  } else if (x.warp == 1 && x.is_leader) {
+    const bool issues = elect_one();
+    previous();
+    work.multiply(r, issues);
+    fused_end_mma<Cfg>(x, issues);
+  }
+  if (x.epi || x.split > 1) work.finish(r, previous);
+  if (p.late_wait) grid_dependency_wait();
+  fused_end<Cfg>(x);
 }
 
 }  // namespace rb200
