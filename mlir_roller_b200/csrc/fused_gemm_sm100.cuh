@@ -281,8 +281,9 @@ __device__ __forceinline__ void fused_end_mma(const FusedCta& x, bool issues) {
 }
 template <class Cfg>
 __device__ __forceinline__ void fused_end(const FusedCta& x) {
-  // stores handed to the TMA unit have to be performed before the CTA may go
-  if (x.epi && x.lane == 0) bulk_wait_all();
+  // the TMA unit has to have read what it stores before the CTA may go (its stores are complete when
+  // the grid is)
+  if (x.epi && x.lane == 0) bulk_wait_read_all();
   __syncwarp();
   // after a failed wait some role left its loop early: let bulk copies on their way land
   if (*reinterpret_cast<volatile uint32_t*>(x.wc.status) != kDevOk) abort_grace_period();
