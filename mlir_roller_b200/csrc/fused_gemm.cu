@@ -193,7 +193,8 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
       const double fixed = c.fixed_us + (split == 1 ? 0.0 : split == 2 ? 2.3 : split == 4 ? 2.5 : 3.0);
       const double tile_us = part * kb_us, epilogue_us = c.epilogue_us * epilogue_weight(s.op);
       double us = split > 1 ? waves * (tile_us + fixed) : waves * (tile_us > epilogue_us ? tile_us : epilogue_us) + fixed;
-      if (us < stream_us + fixed) us = stream_us + fixed;
+      // (among kernels that all wait for memory, the one with the most to spare)
+      if (us < stream_us + 4.8) us = stream_us + 4.8 + 0.02 * us;
       if (best.kv && us >= best_us) continue;
       best_us = us;
       best = f;
