@@ -328,7 +328,8 @@ int roller_b200_gemm_destroy(roller_plan* plan);
  * row-major 16-bit floats of the plan's type (the layout in which a linear layer keeps its weight,
  * outputs x inputs). Sums are kept in fp32. H and the gradients of G and U are rounded to the
  * operand type once, because they are operands of a tensor-core product; Y, G, U and the
- * gradients are rounded once when they are stored. Any d_model, d_ff and tokens are accepted, and any row
+ * gradients are rounded once when they are stored. (In fp16, H, dG and dU have fp16's range: over
+ * 65504 they become infinite, under 6e-8 zero; gradients want the usual loss scale.) Any d_model, d_ff and tokens are accepted, and any row
  * stride that is at least the row's length; a product's operand whose base or row stride is not a
  * multiple of 16 bytes is first copied into rows that are. */
 typedef struct roller_ffn_plan roller_ffn_plan;

@@ -7,7 +7,8 @@ weight: outputs x inputs), all bf16 or all fp16, row-major with any row stride. 
 plans (`_lib.GemmPlan`), a plan owns the workspaces, the caller owns operands and outputs, calls only
 enqueue on a stream, and calls of one plan have to be ordered on the device: use one plan per
 stream, and do not replay two graphs captured from one plan at the same time. Sums are kept in
-fp32. There is no CPU fallback.
+fp32; h and the gradients of g and u are operands of a product and hold the operand type (in fp16
+with its range: over 65504 they become infinite). There is no CPU fallback.
 
     plan = GatedFfnPlan(4096, d_model, d_ff, activation="silu", training=True)
     g, u = plan.new_saved(x.shape[0])
