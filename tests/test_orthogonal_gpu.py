@@ -20,6 +20,8 @@ S = 1024.0
 def exact(g, steps=5, coefficients=MUON_COEFFICIENTS, eps=1e-7):
     a, b, c = coefficients
     x = g.double()
+    if x.shape[0] > x.shape[1]:      # (the polynomial commutes with the transpose)
+        return exact(g.T, steps, coefficients, eps).T
     x = x / (x.square().sum().sqrt() + eps)
     for _ in range(steps):
         p = x @ x.T
