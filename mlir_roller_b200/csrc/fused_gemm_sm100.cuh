@@ -28,8 +28,8 @@
 // the columns through distributed shared memory (the ring's, which is free by then), adds them in the
 // order of k and runs the epilogue on its share. Results do not depend on timing.
 //
-// Epilogue inputs come and results go through the TMA unit in boxes of 32 rows x 32 columns, one
-// warp's slab. Loads and stores from registers, a thread per row, were measured beside it (whole
+// Epilogue inputs come and results go through the TMA unit in boxes of 32 rows x 32 (or 64) columns,
+// one warp's slab. Loads and stores from registers, a thread per row, were measured beside it (whole
 // 32-byte sectors): the pair kernels got a third slower with kOpDact and kOpUpdate*, because
 // every access of a warp touches 32 lines.
 //
@@ -66,15 +66,18 @@ struct FusedCfg {
   static constexpr bool UPDATE = (OP == kOpUpdateWide || OP == kOpUpdateTall);
   static constexpr int A_BYTES = BM * 128, B_BYTES = BNL * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  // columns of the result one epilogue warp owns; they leave in boxes of 32 rows x 32 columns
+  // Columns of the result one epilogue warp owns. They leave in boxes of 32 rows x 32 columns, or
+  // 64 where an epilogue reads two matrices and writes two or three: there the TMA unit's rows
+  // count (64-byte ones beside the main loop's 128-byte ones made kOpDact a third slower than
+  // kOpDown). These boxes serve twice: a matrix read is replaced, in place, by one written.
   static constexpr int OUT_COLS = (OP == kOpGate ? BN / 4 : BN / 2);
   static constexpr int INPUTS = (OP == kOpDact || UPDATE) ? 2 : OP == kOpPoly ? 1 : 0;
-  static constexpr int BOX_BYTES = 32 * 64;
+  static constexpr bool WIDE = INPUTS == 2;
+  static constexpr int BOX_BYTES = WIDE ? 32 * 128 : 32 * 64;
   static constexpr int EPI_WARPS = 8;
-  // boxes of one warp: its inputs, and the results it has under way (those of one slab where an
-  // epilogue writes several matrices)
-  static constexpr int RING = OP == kOpDact ? 3 : 2;
-  static constexpr int WARP_BOXES = INPUTS + RING;
+  // boxes of one warp: narrow: its inputs, and two results under way
+  static constexpr int RING = 2;
+  static constexpr int WARP_BOXES = OP == kOpDact ? 3 : UPDATE ? 2 : INPUTS + RING;
   static constexpr int STAGING_BYTES = EPI_WARPS * WARP_BOXES * BOX_BYTES;
   static constexpr int CTRL_BYTES = 384;
   static constexpr int SMEM_LIMIT = 232448;      // 227 KiB opt-in maximum per CTA
@@ -86,13 +89,14 @@ struct FusedCfg {
   static constexpr int FIRST_EPI_WARP = 4;
   static constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
   static_assert(BN == 256 || BN == 128 || (BN == 64 && OP != kOpGate), "tile widths");
+  static_assert(!WIDE || OUT_COLS % 64 == 0, "whole boxes");
   static constexpr int SYM_RATIO = BN / TILE_M;      // tile rows per tile column of a triangle
   static_assert(!SYM || SYM_RATIO == 1 || SYM_RATIO == 2, "triangle of tiles");
   // The exchange of partial sums in a splitting cluster goes through the ring's memory: each CTA
   // receives its share of the columns of 128 rows from every other part. (With more parts than
   // slabs of 32 columns, some only give.)
   static constexpr int SLABS = (OP == kOpGate ? BN / 2 : BN) / 32;
-  static constexpr int MAX_SPLIT = CG == 2 ? (OP == kOpGate ? 2 : 4) : OP == kOpGate ? 4 : 8;
+  static constexpr int MAX_SPLIT = WIDE ? 1 : CG == 2 ? (OP == kOpGate ? 2 : 4) : OP == kOpGate ? 4 : 8;
   static constexpr int exchange_bytes(int split) {
     return (split - 1) * (SLABS > split ? SLABS / split : 1) * (OP == kOpGate ? 2 : 1) * 16384;
   }
@@ -316,7 +320,7 @@ struct FusedWork {
     kb0 = static_cast<int>(static_cast<long long>(total_kb) * me.part / me.split);
     kb1 = static_cast<int>(static_cast<long long>(total_kb) * (me.part + 1) / me.split);
     in_boxes = me.staging + static_cast<uint32_t>(me.warp - Cfg::FIRST_EPI_WARP) * (Cfg::WARP_BOXES * Cfg::BOX_BYTES);
-    boxes = in_boxes + Cfg::INPUTS * Cfg::BOX_BYTES;
+    boxes = in_boxes + (Cfg::WIDE ? 0 : Cfg::INPUTS) * Cfg::BOX_BYTES;
     tmem_lane = static_cast<uint32_t>(me.quarter * 32) << 16;
   }
 
@@ -427,6 +431,176 @@ struct FusedWork {
     }
   }
 
+  // ---------------------------------------------------------------- epilogue (warps 4 .. 11), wide
+  // 64 columns at a time, in two halves: a thread takes 32 elements of its row of both inputs out of
+  // the boxes and puts 32 elements of the results in their place.
+  template <class F>
+  __device__ __forceinline__ void finish_wide(FusedRing& r, F before_loads) {
+    const uint32_t bar = me.in_bar(me.warp - Cfg::FIRST_EPI_WARP);
+    auto at = [&](int b, int half, int j) {      // 16 bytes: chunk j of a half, 128-byte swizzle
+      return in_boxes + b * Cfg::BOX_BYTES + me.lane * 128 + (((half * 4 + j) ^ (me.lane & 7)) << 4);
+    };
+    auto fetch = [&](const FusedTile& c, int row0, int col) {
+      if (me.lane == 0) {
+        bulk_wait_read_all();        // the boxes' last results are on their way
+        mbar_expect_tx(bar, 2 * Cfg::BOX_BYTES);
+        tma_load_3d(in_boxes, &p.i[0], bar, col, row0, c.z);
+        tma_load_3d(in_boxes + Cfg::BOX_BYTES, &p.i[1], bar, col, row0, c.z);
+      }
+    };
+    auto take = [&](int q, int half, uint32_t (&raw)[16]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(raw[4 * j]), "=r"(raw[4 * j + 1]), "=r"(raw[4 * j + 2]), "=r"(raw[4 * j + 3])
+                     : "r"(at(q, half, j))
+                     : "memory");
+    };
+    auto put = [&](int b, int half, const float (&v)[32], auto dt) {
+      constexpr int T = decltype(dt)::value;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at(b, half, j)),
+                     "r"(fused_pack<T>(v[8 * j], v[8 * j + 1])), "r"(fused_pack<T>(v[8 * j + 2], v[8 * j + 3])),
+                     "r"(fused_pack<T>(v[8 * j + 4], v[8 * j + 5])), "r"(fused_pack<T>(v[8 * j + 6], v[8 * j + 7]))
+                     : "memory");
+    };
+    // the first n boxes to outputs 0 .. n - 1, through the TMA unit
+    auto hand_over = [&](int n, const FusedTile& c, int row0, int col) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (me.lane == 0) {
+        if (row0 < p.M)
+          for (int o = 0; o < n; ++o) tma_store_3d(&p.o[o], in_boxes + o * Cfg::BOX_BYTES, col, row0, c.z);
+        bulk_commit_group();
+      }
+    };
+    // box 0 to rows that start anywhere: a warp writes 32 consecutive elements per instruction
+    auto store_unaligned = [&](const FusedTile& c, int row0, int col) {
+      __syncwarp();
+      uint16_t* dst = static_cast<uint16_t*>(p.out[0]) + c.z * p.out_zstride + static_cast<long long>(row0) * p.out_ld[0] + col + me.lane;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        const int rows = col + h * 32 + me.lane < p.out_cols ? p.M - row0 : 0;
+#pragma unroll 1
+        for (int r0 = 0; r0 < 32; r0 += 8) {
+          uint16_t w[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            asm volatile("ld.shared.u16 %0, [%1];"
+                         : "=h"(w[k])
+                         : "r"(in_boxes + (r0 + k) * 128 + (((h * 4 + (me.lane >> 3)) ^ k) << 4) + (me.lane & 7) * 2)
+                         : "memory");
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (r0 + k < rows) dst[(r0 + k) * p.out_ld[0] + h * 32] = w[k];
+        }
+      }
+      __syncwarp();
+    };
+
+    if (!before_loads()) r.ok = false;
+    for (int t = worker; r.ok && t < tiles; t += workers) {
+      const FusedTile c = fused_tile<0>(t, p.tiles_m, p.tiles_n, per_z);
+      const int row0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM + me.quarter * 32;
+      const int row = row0 + me.lane;
+      const int col0 = c.nb * BN + me.half * Cfg::OUT_COLS;
+      __syncwarp();
+      if (col0 < p.out_cols) fetch(c, row0, col0);       // they do not depend on the product
+      r.ok = mbar_wait_warp(me.tmem_full_bar(r.acc), r.acc_ph, me.wc, kDevTimeoutTmemFull);
+      if (!r.ok) break;
+      tcgen05_fence_after_sync();
+      const uint32_t d_tmem = me.tmem_base + static_cast<uint32_t>(r.acc * BN + me.half * Cfg::OUT_COLS) + tmem_lane;
+      auto run = [&](auto act_tag) {
+        constexpr int ACT = decltype(act_tag)::value;
+#pragma unroll 1
+        for (int k = 0; k < Cfg::OUT_COLS; k += 64) {
+          const int col = col0 + k;
+          if (col >= p.out_cols) break;     // (uniform over the warp)
+          if (k > 0) {
+            __syncwarp();
+            fetch(c, row0, col);
+          }
+          r.ok = mbar_wait_warp(bar, r.in_ph, me.wc, kDevTimeoutFull) && r.ok;
+          r.in_ph ^= 1u;
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            uint32_t d[32], raw0[16], raw1[16];
+            float v[32];
+            tmem_ld_32x32(d_tmem + k + half * 32, d);
+            take(0, half, raw0);
+            take(1, half, raw1);
+            tmem_ld_wait();
+            auto element = [&](const uint32_t (&raw)[16], int j) {
+              const float2 f = fused_unpack<DT>(raw[j / 2]);
+              return j & 1 ? f.y : f.x;
+            };
+            if constexpr (OP == kOpDact) {
+              float du[32], h[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                float y, slope;
+                activation<ACT>(element(raw0, j), y, slope);
+                const float dh = __uint_as_float(d[j]), uu = element(raw1, j);
+                v[j] = dh * uu * slope;    // dg
+                du[j] = dh * y;
+                h[j] = y * uu;
+              }
+              put(0, half, v, IntTag<DT>{});
+              put(1, half, du, IntTag<DT>{});
+              put(2, half, h, IntTag<DT>{});
+            } else {
+              // x = vec x + D / S; vec belongs to rows (q x) or columns (x q)
+              if constexpr (OP == kOpUpdateWide) {
+                const float s = row < p.M ? __ldcg(p.vec + c.z * p.vec_ld + row) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  v[j] = s * (element(raw0, j) + element(raw1, j)) + __uint_as_float(d[j]) * p.inv_scale;
+              } else {
+                // (rows of vec are padded to 64; what lies in the padding meets columns that are not stored)
+                const float4* s4 = reinterpret_cast<const float4*>(p.vec + c.z * p.vec_ld + col + half * 32);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const float4 s = __ldcg(s4 + j);
+                  const float sv[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    v[4 * j + i] = sv[i] * (element(raw0, 4 * j + i) + element(raw1, 4 * j + i)) +
+                                   __uint_as_float(d[4 * j + i]) * p.inv_scale;
+                }
+              }
+              if (p.flags & kFusedLast) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
+                put(0, half, v, IntTag<1>{});        // bf16
+              } else {
+                put(0, half, v, IntTag<DT>{});
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
+                put(1, half, v, IntTag<DT>{});
+              }
+            }
+          }
+          if (OP == kOpDact) hand_over(3, c, row0, col);
+          else if (!(p.flags & kFusedLast)) hand_over(2, c, row0, col);
+          else if (p.out_tma & 1) hand_over(1, c, row0, col);
+          else store_unaligned(c, row0, col);
+        }
+      };
+      if (OP != kOpDact || p.act == kActSilu) run(IntTag<kActSilu>{});
+      else if (p.act == kActGelu) run(IntTag<kActGelu>{});
+      else run(IntTag<kActGeluTanh>{});
+      tcgen05_fence_before_sync();
+      __syncwarp();
+      if (me.lane == 0) {
+        if constexpr (CG == 2) mbar_arrive_cluster(me.tmem_empty_bar(r.acc), me.leader_rank);
+        else mbar_arrive(me.tmem_empty_bar(r.acc));
+      }
+      r.acc ^= 1;
+      if (r.acc == 0) r.acc_ph ^= 1u;
+    }
+  }
+
   // ---------------------------------------------------------------- epilogue (warps 4 .. 11)
   // split: the whole CTA calls this (it meets the cluster's others at barriers).
   template <class F>
@@ -518,16 +692,6 @@ struct FusedWork {
         if (me.lane == 0) bulk_commit_group();   // (an empty group keeps the ring's count)
       }
     };
-    // The first n boxes to outputs 0 .. n - 1, which are the library's own, aligned memory.
-    auto hand_over = [&](int n, const FusedTile& c, int row0, int col) {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (me.lane == 0) {
-        if (row0 < p.M)
-          for (int o = 0; o < n; ++o) tma_store_3d(&p.o[o], boxes + o * Cfg::BOX_BYTES, col, row0, c.z);
-        bulk_commit_group();
-      }
-    };
     // The mirror image of 32 x 32 elements of a symmetric fp16 matrix (its own box has no swizzle).
     // Neighbouring lanes exchange halves, so that each word holds two neighbouring columns.
     auto emit_mirror = [&](const FusedTile& c, int row0, int col, const float (&v)[32]) {
@@ -591,25 +755,7 @@ struct FusedWork {
               v[j] = y * w[j];
             }
             emit(0, c, row0, col, v, false);
-          } else if constexpr (OP == kOpDact) {
-            float du[32], h[32];
-            sums(tc, v);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              float y, slope;
-              activation<ACT>(input(0, j), y, slope);
-              const float dh = v[j], uu = input(1, j);
-              v[j] = dh * uu * slope;    // dg
-              du[j] = dh * y;
-              h[j] = y * uu;
-            }
-            if (me.lane == 0) bulk_wait_read_all();
-            __syncwarp();
-            put(boxes, v, false);
-            put(boxes + Cfg::BOX_BYTES, du, false);
-            put(boxes + 2 * Cfg::BOX_BYTES, h, false);
-            hand_over(3, c, row0, col);
-          } else if constexpr (OP == kOpDown || OP == kOpDx || OP == kOpDw) {
+            } else if constexpr (OP == kOpDown || OP == kOpDx || OP == kOpDw) {
             sums(tc, v);
             emit(OP == kOpDw ? c.z : 0, c, row0, col, v, false);
           } else if constexpr (Cfg::SYM) {
@@ -633,41 +779,10 @@ struct FusedWork {
             }
             emit(0, c, row0, col, v, false);
             if (col < row0) emit_mirror(c, row0, col, v);
-          } else {
-            sums(tc, v);
-            if constexpr (OP == kOpUpdateWide) {
-              const float d = row < p.M ? p.vec[c.z * p.vec_ld + row] : 0.0f;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = d * (input(0, j) + input(1, j)) + v[j] * p.inv_scale;
-            } else {
-              // (rows of vec are padded to 64; what lies in the padding meets columns that are not stored)
-              const float4* d4 = reinterpret_cast<const float4*>(p.vec + c.z * p.vec_ld + col);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float4 d = __ldg(d4 + j);
-                v[4 * j] = d.x * (input(0, 4 * j) + input(1, 4 * j)) + v[4 * j] * p.inv_scale;
-                v[4 * j + 1] = d.y * (input(0, 4 * j + 1) + input(1, 4 * j + 1)) + v[4 * j + 1] * p.inv_scale;
-                v[4 * j + 2] = d.z * (input(0, 4 * j + 2) + input(1, 4 * j + 2)) + v[4 * j + 2] * p.inv_scale;
-                v[4 * j + 3] = d.w * (input(0, 4 * j + 3) + input(1, 4 * j + 3)) + v[4 * j + 3] * p.inv_scale;
-              }
-            }
-            if (p.flags & kFusedLast) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
-              emit(0, c, row0, col, v, true);
-            } else {
-              if (me.lane == 0) bulk_wait_read_all();
-              __syncwarp();
-              put(boxes, v, false);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
-              put(boxes + Cfg::BOX_BYTES, v, false);
-              hand_over(2, c, row0, col);
-            }
           }
         }
       };
-      if constexpr (OP == kOpGate || OP == kOpDact) {
+      if constexpr (OP == kOpGate) {
         if (p.act == kActSilu) run(IntTag<kActSilu>{});
         else if (p.act == kActGelu) run(IntTag<kActGelu>{});
         else run(IntTag<kActGeluTanh>{});
@@ -814,7 +929,11 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
     work.multiply(r, issues);
     fused_end_mma<Cfg>(x, issues);
   }
-  if (x.epi || x.split > 1) work.finish(r, previous);
+  if constexpr (Cfg::WIDE) {
+    if (x.epi) work.finish_wide(r, previous);
+  } else {
+    if (x.epi || x.split > 1) work.finish(r, previous);
+  }
   if (p.late_wait) grid_dependency_wait();
   fused_end<Cfg>(x);
 }

@@ -93,17 +93,23 @@ struct Product {
   int b_mn(int i, const void* base, long long cols, long long rows, long long z, long long ld, long long zs) {
     return encode_batch16(&p.b[i], base, cols, rows, z, ld, zs, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, bf16);
   }
+  // The boxes one epilogue warp reads and writes (FusedCfg::WIDE).
+  int box_map(CUtensorMap* map, const void* base, long long z, long long ld, long long zs, bool as_bf16) const {
+    const bool wide = op == kOpDact || op == kOpUpdateWide || op == kOpUpdateTall;
+    return encode_batch16(map, base, p.out_cols, p.M, z, ld, zs, wide ? 64 : 32, 32,
+                          wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, as_bf16);
+  }
   int output(int i, void* base, long long z, long long ld, long long zs, bool as_bf16) {
     p.out[i] = base;
     p.out_ld[i] = ld;
     p.out_zstride = zs;
     if (!aligned16(base, ld) || (z > 1 && (zs % 8 != 0 || zs < ld * p.M))) return ROLLER_OK;
     p.out_tma |= 1 << i;
-    return encode_batch16(&p.o[i], base, p.out_cols, p.M, z, ld, zs, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, as_bf16);
+    return box_map(&p.o[i], base, z, ld, zs, as_bf16);
   }
   // A matrix that the epilogue reads beside D.
   int input(int i, const void* base, long long z, long long ld, long long zs) {
-    return encode_batch16(&p.i[i], base, p.out_cols, p.M, z, ld, zs, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, bf16);
+    return box_map(&p.i[i], base, z, ld, zs, bf16);
   }
   // The mirror image of a symmetric output (always the library's own, aligned memory).
   int mirror(void* base, long long z, long long ld, long long zs) {
