@@ -145,12 +145,14 @@ int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* s
   const bool bf16 = p->dt == 1;
   const void *x, *wg, *wu, *wd;
   long long ldx, ldg, ldu, ldd;
-  AlignJobs jobs;
-  jobs.n = 0;
+  // Copies of unaligned operands: those of the first product before it, the others behind it, where
+  // they run on the SMs that its last wave leaves idle.
+  AlignJobs jobs, later;
+  later.late = 1;
   FUSED_OK(usable(p, kX, io->x, T, st, &jobs, &x, &ldx));
   FUSED_OK(usable(p, kWg, io->wg, F, st, &jobs, &wg, &ldg));
   FUSED_OK(usable(p, kWu, io->wu, F, st, &jobs, &wu, &ldu));
-  FUSED_OK(usable(p, kWd, io->wd, D, st, &jobs, &wd, &ldd));
+  FUSED_OK(usable(p, kWd, io->wd, D, st, &later, &wd, &ldd));
   FUSED_CUDA(align_rows(jobs, p->ctx.dev.sm_count, st));
   {
     Product g(p->ctx, kOpGate, p->dt, T, F, D, 1);
@@ -166,8 +168,9 @@ int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* s
     }
     FUSED_OK(g.launch(st));
   }
+  FUSED_CUDA(align_rows(later, p->ctx.dev.sm_count, st));
   Product d(p->ctx, kOpDown, p->dt, T, D, F, 1);
-  d.p.b_early = 1;   // Wd does not come from the gate kernel
+  d.p.b_early = later.n == 0;   // Wd does not come from the gate kernel
   FUSED_OK(d.a_k(p->h, F, T, 1, p->ldf, 0));
   FUSED_OK(d.b_k(0, wd, F, D, 1, ldd, 0));
   FUSED_OK(d.output(0, io->y.ptr, 1, io->y.ld, 0, bf16));
@@ -197,11 +200,13 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
   const bool bf16 = p->dt == 1;
   const void *x, *wg, *wu, *wd, *dy, *g, *u;
   long long ldx, ldg, ldu, ldd, ldy, ldsg, ldsu;
-  AlignJobs jobs;
-  jobs.n = 0;
-  FUSED_OK(usable(p, kX, io->x, T, st, &jobs, &x, &ldx));
-  FUSED_OK(usable(p, kWg, io->wg, F, st, &jobs, &wg, &ldg));
-  FUSED_OK(usable(p, kWu, io->wu, F, st, &jobs, &wu, &ldu));
+  // Copies of unaligned operands: those of the first product before it, the others behind it, where
+  // they run on the SMs that its last wave leaves idle.
+  AlignJobs jobs, later;
+  later.late = 1;
+  FUSED_OK(usable(p, kX, io->x, T, st, &later, &x, &ldx));
+  FUSED_OK(usable(p, kWg, io->wg, F, st, &later, &wg, &ldg));
+  FUSED_OK(usable(p, kWu, io->wu, F, st, &later, &wu, &ldu));
   FUSED_OK(usable(p, kWd, io->wd, D, st, &jobs, &wd, &ldd));
   FUSED_OK(usable(p, kDy, io->dy, T, st, &jobs, &dy, &ldy));
   FUSED_OK(usable(p, kG, io->g, T, st, &jobs, &g, &ldsg));
@@ -220,9 +225,10 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     FUSED_OK(a.input(1, u, 1, ldsu, 0));
     FUSED_OK(a.launch(st));
   }
+  FUSED_CUDA(align_rows(later, p->ctx.dev.sm_count, st));
   {
     Product r(p->ctx, kOpDx, p->dt, T, D, F, 1);
-    r.p.b_early = 1;   // Wg and Wu do not come from the kernel above
+    r.p.b_early = later.n == 0;   // Wg and Wu do not come from the kernel above
     FUSED_OK(r.a_k(p->dgu, F, T, 2, p->ldf, zs));
     FUSED_OK(r.b_mn(0, wg, D, F, 1, ldg, 0));
     FUSED_OK(r.b_mn(1, wu, D, F, 1, ldu, 0));

@@ -41,8 +41,9 @@ double epilogue_weight(int op) {
 // elements) of a row at a time, a thread eight of them, all on their way together: a source row
 // that starts between two words gives each word from two neighbouring ones. (A word that holds an
 // element of the row may be read whole.)
+// jobs.late: as FusedParams::late_wait, the copies need nothing from the previous kernel.
 __global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__ AlignJobs jobs) {
-  grid_dependency_wait();
+  if (!jobs.late) grid_dependency_wait();
   grid_launch_dependents();
   int b = static_cast<int>(blockIdx.x), i = 0;
   while (i + 1 < jobs.n && b >= jobs.job[i].blocks) b -= jobs.job[i++].blocks;
@@ -67,6 +68,7 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__
     for (int k = 0; k < 8; ++k)
       if (w0 + 32 * k < words) dst[w0 + 32 * k] = between ? __byte_perm(x[k], y[k], 0x5432) : x[k];
   }
+  if (jobs.late) grid_dependency_wait();
 }
 
 }  // namespace

@@ -47,7 +47,8 @@ struct AlignJob {
 };
 struct AlignJobs {
   AlignJob job[8];
-  int n;
+  int n = 0;
+  int late = 0;     // the previous kernel of the stream is one of these and has nothing to do with them
 };
 cudaError_t align_rows(AlignJobs& jobs, int sm_count, cudaStream_t stream);
 
