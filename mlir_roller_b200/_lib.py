@@ -220,17 +220,23 @@ def _stream_ptr(stream) -> C.c_void_p:
     return C.c_void_p(getattr(stream, "cuda_stream", stream))
 
 
+_torch = None
+
+
 def on_device(device, stream, fn, *args) -> int:
     """fn(*args, stream) with `device` current; `stream` None is its current stream."""
-    import torch
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
     if stream is None:
         # (the raw handle: building a Stream object costs as much as the rest of a call)
-        ptr = torch._C._cuda_getCurrentRawStream(device.index)
+        ptr = _torch._C._cuda_getCurrentRawStream(device.index)
     else:
         ptr = getattr(stream, "cuda_stream", stream)
-    if torch.cuda.current_device() == device.index:
+    if _torch.cuda.current_device() == device.index:
         return fn(*args, ptr)
-    with torch.cuda.device(device):
+    with _torch.cuda.device(device):
         return fn(*args, ptr)
 
 

@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kMaxExtent = 1 << 20;
 
+enum { kPGate = 0, kPDown, kPDact, kPDx, kPDwUp, kPDwDown, kProducts };
 enum Operand { kX = 0, kWg, kWu, kWd, kDy, kG, kU, kOperands };
 
 }  // namespace
@@ -33,6 +34,9 @@ struct roller_ffn_plan {
   void* h;                 // [max_tokens, ldf]
   void* dgu;               // [2][max_tokens, ldf]
   void* pad[kOperands];    // copies of unaligned operands, made when one is needed
+  // The kernels chosen for the last number of tokens (choosing costs as much host time as a launch).
+  int chosen_tokens;
+  FusedChoice choice[kProducts];
 };
 
 namespace {
@@ -72,6 +76,18 @@ int usable(roller_ffn_plan* p, int which, const roller_mat& m, int rows, cudaStr
   *ptr = p->pad[which];
   *ld = ldp;
   return ROLLER_OK;
+}
+
+// The choices for `T` tokens.
+const FusedChoice* choices(roller_ffn_plan* p, int T) {
+  if (p->chosen_tokens != T) {
+    const FusedShape shapes[kProducts] = {
+        {kOpGate, p->dt, T, p->f, p->d, 1}, {kOpDown, p->dt, T, p->d, p->f, 1}, {kOpDact, p->dt, T, p->f, p->d, 1},
+        {kOpDx, p->dt, T, p->d, p->f, 1},   {kOpDw, p->dt, p->f, p->d, T, 2},   {kOpDw, p->dt, p->d, p->f, T, 1}};
+    for (int i = 0; i < (p->training ? kProducts : kPDact); ++i) p->choice[i] = fused_choose(shapes[i], p->ctx.dev);
+    p->chosen_tokens = T;
+  }
+  return p->choice;
 }
 
 bool given(const roller_mat& m, long long cols) { return m.ptr && m.ld >= cols; }
@@ -143,6 +159,7 @@ int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* s
       if (outs[i] && outs[i] == all[j]) return ROLLER_ERR_INVALID;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf16 = p->dt == 1;
+  const FusedChoice* choice = choices(p, T);
   const void *x, *wg, *wu, *wd;
   long long ldx, ldg, ldu, ldd;
   // Copies of unaligned operands: those of the first product before it, the others behind it, where
@@ -155,7 +172,7 @@ int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* s
   FUSED_OK(usable(p, kWd, io->wd, D, st, &later, &wd, &ldd));
   FUSED_CUDA(align_rows(jobs, p->ctx.dev.sm_count, st));
   {
-    Product g(p->ctx, kOpGate, p->dt, T, F, D, 1);
+    Product g(p->ctx, kOpGate, p->dt, T, F, D, 1, &choice[kPGate]);
     g.p.act = p->act;
     FUSED_OK(g.a_k(x, D, T, 1, ldx, 0));
     FUSED_OK(g.b_k(0, wg, D, F, 1, ldg, 0));
@@ -169,7 +186,7 @@ int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* s
     FUSED_OK(g.launch(st));
   }
   FUSED_CUDA(align_rows(later, p->ctx.dev.sm_count, st));
-  Product d(p->ctx, kOpDown, p->dt, T, D, F, 1);
+  Product d(p->ctx, kOpDown, p->dt, T, D, F, 1, &choice[kPDown]);
   d.p.b_early = later.n == 0;   // Wd does not come from the gate kernel
   FUSED_OK(d.a_k(p->h, F, T, 1, p->ldf, 0));
   FUSED_OK(d.b_k(0, wd, F, D, 1, ldd, 0));
@@ -198,6 +215,7 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     for (int j = 0; j < i; ++j)
       if (all[i] == all[j]) return ROLLER_ERR_INVALID;
   const bool bf16 = p->dt == 1;
+  const FusedChoice* choice = choices(p, T);
   const void *x, *wg, *wu, *wd, *dy, *g, *u;
   long long ldx, ldg, ldu, ldd, ldy, ldsg, ldsu;
   // Copies of unaligned operands: those of the first product before it, the others behind it, where
@@ -214,7 +232,7 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
   FUSED_CUDA(align_rows(jobs, p->ctx.dev.sm_count, st));
   const long long zs = static_cast<long long>(p->max_tokens) * p->ldf;   // dg to du
   {
-    Product a(p->ctx, kOpDact, p->dt, T, F, D, 1);
+    Product a(p->ctx, kOpDact, p->dt, T, F, D, 1, &choice[kPDact]);
     a.p.act = p->act;
     FUSED_OK(a.a_k(dy, D, T, 1, ldy, 0));
     FUSED_OK(a.b_mn(0, wd, F, D, 1, ldd, 0));
@@ -227,7 +245,7 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
   }
   FUSED_CUDA(align_rows(later, p->ctx.dev.sm_count, st));
   {
-    Product r(p->ctx, kOpDx, p->dt, T, D, F, 1);
+    Product r(p->ctx, kOpDx, p->dt, T, D, F, 1, &choice[kPDx]);
     r.p.b_early = later.n == 0;   // Wg and Wu do not come from the kernel above
     FUSED_OK(r.a_k(p->dgu, F, T, 2, p->ldf, zs));
     FUSED_OK(r.b_mn(0, wg, D, F, 1, ldg, 0));
@@ -236,7 +254,7 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     FUSED_OK(r.launch(st));
   }
   {
-    Product w(p->ctx, kOpDw, p->dt, F, D, T, 2);
+    Product w(p->ctx, kOpDw, p->dt, F, D, T, 2, &choice[kPDwUp]);
     w.p.late_wait = 1;   // dg, du and h were complete before the kernel above started
     FUSED_OK(w.a_mn(p->dgu, F, T, 2, p->ldf, zs));
     FUSED_OK(w.b_mn(0, x, D, T, 1, ldx, 0));
@@ -244,7 +262,7 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     FUSED_OK(w.output(1, io->dwu.ptr, 1, io->dwu.ld, 0, bf16));
     FUSED_OK(w.launch(st));
   }
-  Product w(p->ctx, kOpDw, p->dt, D, F, T, 1);
+  Product w(p->ctx, kOpDw, p->dt, D, F, T, 1, &choice[kPDwDown]);
   w.p.late_wait = 1;
   FUSED_OK(w.a_mn(dy, D, T, 1, ldy, 0));
   FUSED_OK(w.b_mn(0, p->h, F, T, 1, p->ldf, 0));

@@ -59,10 +59,12 @@ struct Product {
   int op;
   bool bf16;
 
-  Product(const FusedContext& x, int op_, int dt, long long M, long long N, long long K, int z)
+  // `known`: the choice for an earlier product of these sizes.
+  Product(const FusedContext& x, int op_, int dt, long long M, long long N, long long K, int z,
+          const FusedChoice* known = nullptr)
       : op(op_), bf16(dt == 1) {
     memset(&p, 0, sizeof(p));
-    c = fused_choose(FusedShape{op, dt, M, N, K, z}, x.dev);
+    c = known ? *known : fused_choose(FusedShape{op, dt, M, N, K, z}, x.dev);
     p.M = static_cast<int>(M);
     p.out_cols = static_cast<int>(N);
     p.num_kb = c.num_kb;

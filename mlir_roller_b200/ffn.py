@@ -25,9 +25,10 @@ import struct
 
 from . import _lib
 
-# roller_ffn_io: the number of tokens (padded to eight bytes), then twelve bases and row strides
-_IO = struct.Struct("@i4x" + 12 * "Pq")
-_NONE = 12 * (("", None, 0, 0),)
+# roller_ffn_io: the number of tokens (padded to eight bytes), then bases and row strides; the forward
+# pass reads the first seven matrices of twelve
+_FORWARD = struct.Struct("@i4x" + 7 * "Pq")
+_BACKWARD = struct.Struct("@i4x" + 12 * "Pq")
 
 ACTIVATIONS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
 
@@ -72,6 +73,7 @@ class GatedFfnPlan:
                    "roller_b200_ffn_create")
         self.device = torch.device("cuda", torch.cuda.current_device())
         self._io = _lib.FfnIo()
+        self._io_ref = C.byref(self._io)
 
     def new_saved(self, tokens: int):
         """Two tensors for g and u, with rows that start on 32 bytes (the fast layout for any d_ff)."""
@@ -80,19 +82,21 @@ class GatedFfnPlan:
         return tuple(torch.empty(tokens, ld, dtype=self.dtype, device=self.device)[:, :self.d_ff]
                      for _ in range(2))
 
-    def _call(self, fn, name: str, tokens: int, mats, stream) -> None:
-        """`mats`: (name, tensor or None, rows, cols) in the order of roller_ffn_io."""
+    def _mat(self, t, name: str, rows: int, cols: int):
+        """Base and row stride of one operand, checked."""
+        if t.dtype is not self.dtype or t.device != self.device or t.shape != (rows, cols):
+            check_matrix(t, name, self.dtype, self.device, rows, cols)      # says what is wrong
+        ld, step = t.stride()
+        if step != 1 or ld < cols or rows < 2:
+            ld = check_matrix(t, name, self.dtype, self.device, rows, cols)
+        return t.data_ptr(), ld
+
+    def _call(self, fn, name: str, stream) -> None:
         if not self._h:
             raise RuntimeError("the plan has been destroyed")
-        words = [tokens]
-        for what, t, rows, cols in mats:
-            if t is None:
-                words += (0, 0)
-                continue
-            ld = check_matrix(t, what, self.dtype, self.device, rows, cols)
-            words += (t.data_ptr(), ld)
-        _IO.pack_into(self._io, 0, *words)
-        _lib.check(_lib.on_device(self.device, stream, fn, self._h, C.byref(self._io)), name)
+        status = _lib.on_device(self.device, stream, fn, self._h, self._io_ref)
+        if status:
+            _lib.check(status, name)
 
     def _tokens(self, x) -> int:
         tokens = x.shape[0]
@@ -104,19 +108,20 @@ class GatedFfnPlan:
         """Writes y, and g and u when they are given (both or neither)."""
         if (g is None) != (u is None):
             raise ValueError("g and u are written together: give both or neither")
-        n, d, f = self._tokens(x), self.d_model, self.d_ff
-        self._call(self._lib.roller_b200_ffn_forward, "roller_b200_ffn_forward", n,
-                   (("x", x, n, d), ("wg", wg, f, d), ("wu", wu, f, d), ("wd", wd, d, f), ("y", y, n, d),
-                    ("g", g, n, f), ("u", u, n, f)) + _NONE[:5], stream)
+        n, d, f, mat = self._tokens(x), self.d_model, self.d_ff, self._mat
+        saved = (0, 0, 0, 0) if g is None else (*mat(g, "g", n, f), *mat(u, "u", n, f))
+        _FORWARD.pack_into(self._io, 0, n, *mat(x, "x", n, d), *mat(wg, "wg", f, d), *mat(wu, "wu", f, d),
+                           *mat(wd, "wd", d, f), *mat(y, "y", n, d), *saved)
+        self._call(self._lib.roller_b200_ffn_forward, "roller_b200_ffn_forward", stream)
 
     def backward(self, x, wg, wu, wd, g, u, dy, dx, dwg, dwu, dwd, stream=None) -> None:
         """Writes dx, dwg, dwu and dwd (not added to) for the gradient dy of y. g and u are what
         `forward` wrote for the same x and weights. The plan has to be made with training=True."""
-        n, d, f = self._tokens(x), self.d_model, self.d_ff
-        self._call(self._lib.roller_b200_ffn_backward, "roller_b200_ffn_backward", n,
-                   (("x", x, n, d), ("wg", wg, f, d), ("wu", wu, f, d), ("wd", wd, d, f)) + _NONE[:1] +
-                   (("g", g, n, f), ("u", u, n, f), ("dy", dy, n, d), ("dx", dx, n, d), ("dwg", dwg, f, d),
-                    ("dwu", dwu, f, d), ("dwd", dwd, d, f)), stream)
+        n, d, f, mat = self._tokens(x), self.d_model, self.d_ff, self._mat
+        _BACKWARD.pack_into(self._io, 0, n, *mat(x, "x", n, d), *mat(wg, "wg", f, d), *mat(wu, "wu", f, d),
+                            *mat(wd, "wd", d, f), 0, 0, *mat(g, "g", n, f), *mat(u, "u", n, f), *mat(dy, "dy", n, d),
+                            *mat(dx, "dx", n, d), *mat(dwg, "dwg", f, d), *mat(dwu, "dwu", f, d), *mat(dwd, "dwd", d, f))
+        self._call(self._lib.roller_b200_ffn_backward, "roller_b200_ffn_backward", stream)
 
     def check_status(self) -> None:
         """Raises RollerError(TIMEOUT) if a launch since the last check gave up on a device-side

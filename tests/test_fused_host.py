@@ -47,12 +47,14 @@ def test_ortho_create_refuses_bad_arguments():
 def test_packed_operands_match_the_structure():
     from mlir_roller_b200 import ffn
     io = _lib.FfnIo()
-    assert ffn._IO.size == C.sizeof(io)
-    ffn._IO.pack_into(io, 0, 7, *range(100, 124))
+    assert ffn._BACKWARD.size == C.sizeof(io)
+    ffn._BACKWARD.pack_into(io, 0, 7, *range(100, 124))
     assert io.tokens == 7
     names = [n for n, _ in _lib.FfnIo._fields_[1:]]
     for i, n in enumerate(names):
         assert (getattr(io, n).ptr, getattr(io, n).ld) == (100 + 2 * i, 101 + 2 * i), n
+    ffn._FORWARD.pack_into(io, 0, 3, *range(200, 214))
+    assert io.tokens == 3 and names[6] == "u" and io.u.ld == 213 and io.dy.ptr == 114
 
 
 def test_tensor_checks():
