@@ -22,18 +22,20 @@ struct TileCost {
   double epilogue_us;         // of one tile, plain; hidden behind the next tile's k-blocks
   double fixed_us;            // start, first loads, last epilogue
 };
-constexpr TileCost kTiles[] = {{2, 256, 0.28, 0.36, 5.3, 5.5},
-                               {1, 256, 0.285, 0.39, 3.1, 6.3},
-                               {1, 128, 0.16, 0.23, 1.8, 3.8},
-                               {1, 64, 0.15, 0.18, 1.5, 3.6}};
+constexpr TileCost kTiles[] = {{2, 256, 0.26, 0.33, 4.1, 7.0},
+                               {2, 128, 0.145, 0.20, 2.4, 4.8},
+                               {1, 256, 0.285, 0.39, 3.2, 6.4},
+                               {1, 128, 0.18, 0.23, 3.2, 3.7},
+                               {1, 64, 0.155, 0.172, 1.5, 2.9}};
 // The epilogues beside the plain one.
 double epilogue_weight(int op) {
   switch (op) {
-    case kOpDact: return 2.2;
-    case kOpUpdateWide: case kOpUpdateTall: return 1.6;
-    case kOpPoly: return 1.4;
-    case kOpGramWide: case kOpGramTall: return 1.1;
-    default: return 0.6;
+    case kOpDact: return 3.5;
+    case kOpUpdateTall: return 2.0;
+    case kOpUpdateWide: return 1.0;
+    case kOpGate: return 0.9;
+    case kOpDw: return 0.3;
+    default: return 0.55;
   }
 }
 
@@ -176,9 +178,9 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
     f.tiles_m = static_cast<int>((s.M + bm - 1) / bm);
     f.tiles_n = static_cast<int>((s.N + bn - 1) / bn);
     f.tiles_per_z = f.tiles_m * f.tiles_n;
-    if (sym) {   // `ratio` tile rows each have 1, 2, 3 .. tiles (fused_tile)
-      const int ratio = bn / bm, q = f.tiles_m / ratio;
-      f.tiles_per_z = ratio * q * (q + 1) / 2 + f.tiles_m % ratio * (q + 1);
+    if (sym) {   // fused_tile: 1, 2, 3 .. tiles in each `ratio` tile rows, or 2, 4, 6 .. in a row
+      const int ratio = bn / bm, q = ratio ? f.tiles_m / ratio : 0;
+      f.tiles_per_z = ratio ? ratio * q * (q + 1) / 2 + f.tiles_m % ratio * (q + 1) : f.tiles_m * (f.tiles_m + 1);
     }
     f.num_kb = static_cast<int>((s.K + 63) / 64);
     const int kbs = f.num_kb * (s.op == kOpDx ? 2 : 1);
@@ -192,7 +194,7 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
       const double busy = tiles * ctas < d.sm_count ? static_cast<double>(tiles * ctas) / d.sm_count : 1.0;
       const double kb_us = c.alone_us + (c.busy_us - c.alone_us) * busy;
       // a cluster has one tile: from the second wave on every tile pays for its own start and end
-      const double fixed = c.fixed_us + (split == 1 ? 0.0 : split == 2 ? 2.3 : split == 4 ? 2.5 : 3.0);
+      const double fixed = c.fixed_us + (split == 1 ? 0.0 : split == 2 ? 2.1 : 3.0);
       const double tile_us = part * kb_us, epilogue_us = c.epilogue_us * epilogue_weight(s.op);
       double us = split > 1 ? waves * (tile_us + fixed) : waves * (tile_us > epilogue_us ? tile_us : epilogue_us) + fixed;
       // (among kernels that all wait for memory, the one with the most to spare)

@@ -90,8 +90,9 @@ struct FusedCfg {
   static constexpr int THREADS = (FIRST_EPI_WARP + EPI_WARPS) * 32;
   static_assert(BN == 256 || BN == 128 || (BN == 64 && OP != kOpGate), "tile widths");
   static_assert(!WIDE || OUT_COLS % 64 == 0, "whole boxes");
-  static constexpr int SYM_RATIO = BN / TILE_M;      // tile rows per tile column of a triangle
-  static_assert(!SYM || SYM_RATIO == 1 || SYM_RATIO == 2, "triangle of tiles");
+  // triangle of tiles: tile rows per tile column, or minus tile columns per tile row; 0 = all tiles
+  static constexpr int SYM_RATIO = !SYM ? 0 : BN >= TILE_M ? BN / TILE_M : -(TILE_M / BN);
+  static_assert(SYM_RATIO >= -2 && SYM_RATIO <= 2, "triangle of tiles");
   // The exchange of partial sums in a splitting cluster goes through the ring's memory: each CTA
   // receives its share of the columns of 128 rows from every other part. (With more parts than
   // slabs of 32 columns, some only give.)
@@ -150,13 +151,20 @@ struct FusedTile {
 
 // Tile order. Rectangular problems: panels of 8 tile rows, so that the tiles in flight share
 // operand rows and columns in L2. Symmetric ones: the tiles that touch the lower triangle, row by
-// row (RATIO tile rows to a tile column; 0 = not symmetric).
+// row (RATIO: FusedCfg::SYM_RATIO).
 template <int RATIO>
 __device__ __forceinline__ FusedTile fused_tile(int t, int tiles_m, int tiles_n, int per_z) {
   FusedTile c;
   c.z = t / per_z;
   int r = t - c.z * per_z;
-  if constexpr (RATIO > 0) {
+  if constexpr (RATIO < 0) {
+    // row mb has 2 (mb + 1) tiles, mb (mb + 1) come before it
+    int q = static_cast<int>((sqrtf(4.0f * static_cast<float>(r) + 1.0f) - 1.0f) * 0.5f);
+    while (q * (q + 1) > r) --q;
+    while ((q + 1) * (q + 2) <= r) ++q;
+    c.mb = q;
+    c.nb = r - q * (q + 1);
+  } else if constexpr (RATIO > 0) {
     // RATIO rows have q + 1 tiles each, RATIO q (q + 1) / 2 tiles come before them
     int q = static_cast<int>((sqrtf(8.0f / RATIO * static_cast<float>(r) + 1.0f) - 1.0f) * 0.5f);
     while (RATIO * q * (q + 1) / 2 > r) --q;
@@ -367,7 +375,7 @@ struct FusedWork {
       }
     };
     for (int t = worker; r.ok && t < tiles; t += workers) {
-      const FusedTile c = fused_tile<Cfg::SYM ? Cfg::SYM_RATIO : 0>(t, p.tiles_m, p.tiles_n, per_z);
+      const FusedTile c = fused_tile<Cfg::SYM_RATIO>(t, p.tiles_m, p.tiles_n, per_z);
       int kb = kb0;
       if (t == worker) {
         const int early = p.b_early ? min(STAGES, kb1 - kb0) : 0;    // (of a launch's first tiles)
@@ -796,7 +804,7 @@ struct FusedWork {
     if (me.split == 1) {
       if (!before_loads()) r.ok = false;
       for (int t = worker; r.ok && t < tiles; t += workers) {
-        const FusedTile c = fused_tile<Cfg::SYM ? Cfg::SYM_RATIO : 0>(t, p.tiles_m, p.tiles_n, per_z);
+        const FusedTile c = fused_tile<Cfg::SYM_RATIO>(t, p.tiles_m, p.tiles_n, per_z);
         if constexpr (Cfg::INPUTS > 0) {     // they do not depend on the product
           const int col = c.nb * BN + me.half * Cfg::OUT_COLS;
           const int row0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM + me.quarter * 32;
@@ -820,7 +828,7 @@ struct FusedWork {
     } else {
       // ---- the cluster holds the tile's parts: their sums are put together, each CTA taking a share
       // of the slabs: slab i is received by part i / share, or by every `apart`-th part
-      const FusedTile c = fused_tile<Cfg::SYM ? Cfg::SYM_RATIO : 0>(worker, p.tiles_m, p.tiles_n, per_z);
+      const FusedTile c = fused_tile<Cfg::SYM_RATIO>(worker, p.tiles_m, p.tiles_n, per_z);
       const int row0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM + me.quarter * 32;
       const bool row_ok = row0 + me.lane < p.M;
       const int share = max(Cfg::SLABS / me.split, 1), apart = max(me.split / Cfg::SLABS, 1);

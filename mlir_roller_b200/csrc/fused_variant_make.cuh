@@ -42,17 +42,17 @@ static FusedVariant fused_make() {
   return v;
 }
 
-// The feed-forward products of one operand type: the pair tile 256 x 256 and, for few rows or
+// The feed-forward products of one operand type: the pair tiles 256 x 256 and 256 x 128 and, for few rows or
 // columns, single CTAs of 128 x 256, 128 x 128 and 128 x 64.
 template <int DT>
 static const FusedVariant* fused_ffn_table(int* n) {
   static const FusedVariant t[] = {
-      fused_make<kOpGate, 2, 256, DT>(), fused_make<kOpGate, 1, 256, DT>(), fused_make<kOpGate, 1, 128, DT>(),
-      fused_make<kOpDown, 2, 256, DT>(), fused_make<kOpDown, 1, 256, DT>(), fused_make<kOpDown, 1, 128, DT>(),
+      fused_make<kOpGate, 2, 256, DT>(), fused_make<kOpGate, 2, 128, DT>(), fused_make<kOpGate, 1, 256, DT>(), fused_make<kOpGate, 1, 128, DT>(),
+      fused_make<kOpDown, 2, 256, DT>(), fused_make<kOpDown, 2, 128, DT>(), fused_make<kOpDown, 1, 256, DT>(), fused_make<kOpDown, 1, 128, DT>(),
       fused_make<kOpDown, 1, 64, DT>(),  fused_make<kOpDx, 1, 64, DT>(),
-      fused_make<kOpDact, 2, 256, DT>(), fused_make<kOpDact, 1, 128, DT>(),
-      fused_make<kOpDx, 2, 256, DT>(),   fused_make<kOpDx, 1, 256, DT>(), fused_make<kOpDx, 1, 128, DT>(),
-      fused_make<kOpDw, 2, 256, DT>(),   fused_make<kOpDw, 1, 128, DT>(),
+      fused_make<kOpDact, 2, 256, DT>(), fused_make<kOpDact, 2, 128, DT>(), fused_make<kOpDact, 1, 128, DT>(),
+      fused_make<kOpDx, 2, 256, DT>(), fused_make<kOpDx, 2, 128, DT>(),   fused_make<kOpDx, 1, 256, DT>(), fused_make<kOpDx, 1, 128, DT>(),
+      fused_make<kOpDw, 2, 256, DT>(), fused_make<kOpDw, 2, 128, DT>(),   fused_make<kOpDw, 1, 128, DT>(),
   };
   *n = static_cast<int>(sizeof(t) / sizeof(t[0]));
   return t;
