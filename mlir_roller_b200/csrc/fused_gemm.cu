@@ -23,16 +23,16 @@ struct TileCost {
   double fixed_us;            // start, first loads, last epilogue
 };
 constexpr TileCost kTiles[] = {{2, 256, 0.26, 0.33, 4.1, 7.0},
-                               {2, 128, 0.145, 0.20, 2.4, 4.8},
+                               {2, 128, 0.145, 0.20, 2.6, 4.8},
                                {1, 256, 0.285, 0.39, 3.2, 6.4},
                                {1, 128, 0.18, 0.23, 3.2, 3.7},
                                {1, 64, 0.155, 0.172, 1.5, 2.9}};
 // The epilogues beside the plain one.
 double epilogue_weight(int op) {
   switch (op) {
-    case kOpDact: return 3.5;
+    case kOpDact: return 4.7;
     case kOpUpdateTall: return 2.0;
-    case kOpUpdateWide: return 1.0;
+    case kOpUpdateWide: return 1.5;
     case kOpGate: return 0.9;
     case kOpDw: return 0.3;
     default: return 0.55;
@@ -198,7 +198,7 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
       const double tile_us = part * kb_us, epilogue_us = c.epilogue_us * epilogue_weight(s.op);
       double us = split > 1 ? waves * (tile_us + fixed) : waves * (tile_us > epilogue_us ? tile_us : epilogue_us) + fixed;
       // (among kernels that all wait for memory, the one with the most to spare)
-      if (us < stream_us + 4.8) us = stream_us + 4.8 + 0.02 * us;
+      us = (us < stream_us + 4.8 ? stream_us + 4.8 : us) + 0.05 * us;
       if (best.kv && us >= best_us) continue;
       best_us = us;
       best = f;
