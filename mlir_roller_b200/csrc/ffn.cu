@@ -31,9 +31,11 @@ struct roller_ffn_plan {
   int act;
   bool training;
   long long ldf;           // row stride of h, dg, du
+  Arena arena;
   void* h;                 // [max_tokens, ldf]
   void* dgu;               // [2][max_tokens, ldf]
-  void* pad[kOperands];    // copies of unaligned operands, made when one is needed
+  void* pad[kOperands];    // copies of unaligned operands, in the arena ...
+  void* own_pad[kOperands];  // ... or made when one turned out to be needed
   // The kernels chosen for the last number of tokens (choosing costs as much host time as a launch).
   int chosen_tokens;
   FusedChoice choice[kProducts];
@@ -65,11 +67,12 @@ int usable(roller_ffn_plan* p, int which, const roller_mat& m, int rows, cudaStr
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     FUSED_CUDA(cudaStreamIsCapturing(st, &cap));
     if (cap != cudaStreamCaptureStatusNone) return ROLLER_ERR_UNSUPPORTED;
-    if (cudaMalloc(&p->pad[which], pad_bytes(p, which)) != cudaSuccess) {
+    if (cudaMalloc(&p->own_pad[which], pad_bytes(p, which)) != cudaSuccess) {
       cudaGetLastError();
-      p->pad[which] = nullptr;
+      p->own_pad[which] = nullptr;
       return ROLLER_ERR_NOMEM;
     }
+    p->pad[which] = p->own_pad[which];
   }
   jobs->job[jobs->n++] = AlignJob{static_cast<const uint16_t*>(m.ptr), static_cast<uint16_t*>(p->pad[which]), m.ld,
                                   ldp, rows, cols_of(p, which), 0};
@@ -116,7 +119,7 @@ int roller_b200_ffn_create(int max_tokens, int d_model, int d_ff, int mode, int 
   if (flags & ~ROLLER_FFN_TRAINING) return ROLLER_ERR_INVALID;
   roller_ffn_plan* p = new (std::nothrow) roller_ffn_plan();
   if (!p) return ROLLER_ERR_NOMEM;
-  memset(p, 0, sizeof(*p));
+  memset(static_cast<void*>(p), 0, sizeof(*p));
   const int rc = fused_context_create(&p->ctx);
   if (rc != ROLLER_OK) {
     delete p;
@@ -130,16 +133,26 @@ int roller_b200_ffn_create(int max_tokens, int d_model, int d_ff, int mode, int 
   p->training = (flags & ROLLER_FFN_TRAINING) != 0;
   p->ldf = up64(d_ff);
   const size_t h_bytes = static_cast<size_t>(max_tokens) * p->ldf * 2;
-  cudaError_t e = cudaMalloc(&p->h, h_bytes);
-  if (e == cudaSuccess && p->training) e = cudaMalloc(&p->dgu, 2 * h_bytes);
-  for (int i = 0; i < kOperands && e == cudaSuccess; ++i)
-    if (cols_of(p, i) % 8 != 0 && (i < kDy || p->training)) e = cudaMalloc(&p->pad[i], pad_bytes(p, i));
+  const size_t h = p->arena.take(h_bytes);
+  const size_t dgu = p->training ? p->arena.take(2 * h_bytes) : 0;
+  size_t pad[kOperands];
+  bool padded[kOperands];      // operands that are unaligned when they are contiguous
+  for (int i = 0; i < kOperands; ++i) {
+    padded[i] = cols_of(p, i) % 8 != 0 && (i < kDy || p->training);
+    pad[i] = padded[i] ? p->arena.take(pad_bytes(p, i)) : 0;
+  }
+  const cudaError_t e = p->arena.allocate();
   if (e != cudaSuccess) {
     const int failed = e == cudaErrorMemoryAllocation ? ROLLER_ERR_NOMEM : report_cuda_error(e, "ffn plan setup");
     cudaGetLastError();
+    p->arena.base = nullptr;
     roller_b200_ffn_destroy(p);
     return failed;
   }
+  p->h = p->arena.at<void>(h);
+  if (p->training) p->dgu = p->arena.at<void>(dgu);
+  for (int i = 0; i < kOperands; ++i)
+    if (padded[i]) p->pad[i] = p->arena.at<void>(pad[i]);
   *out = p;
   return ROLLER_OK;
 }
@@ -277,9 +290,8 @@ int roller_b200_ffn_status(roller_ffn_plan* p, uint32_t* device_status) {
 
 int roller_b200_ffn_destroy(roller_ffn_plan* p) {
   if (!p) return ROLLER_OK;
-  cudaFree(p->h);
-  cudaFree(p->dgu);
-  for (void* b : p->pad) cudaFree(b);
+  cudaFree(p->arena.base);
+  for (void* b : p->own_pad) cudaFree(b);
   fused_context_destroy(&p->ctx);
   cudaGetLastError();
   delete p;

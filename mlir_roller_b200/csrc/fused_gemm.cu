@@ -1,4 +1,6 @@
 // Which fused product kernel a problem runs on, and how its reduction is cut.
+#include <atomic>
+
 #include "fused_product.h"
 #include "ptx_sm100.cuh"
 
@@ -209,14 +211,33 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
   return best;
 }
 
+// What bind_device found on each device: asking again costs every new plan the better part of a
+// millisecond. (A thread that comes while another one is asking uses its own answer.)
+static cudaError_t device_facts(int dev, FusedDevice* d) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> state[kDevices];      // 0 = not asked, 1 = being written, 2 = known
+  static FusedDevice known[kDevices];
+  if (dev < kDevices && state[dev].load(std::memory_order_acquire) == 2) {
+    *d = known[dev];
+    return cudaSuccess;
+  }
+  cudaError_t e = cudaDeviceGetAttribute(&d->sm_count, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = bind_device(d);
+  int expected = 0;
+  if (e == cudaSuccess && dev < kDevices && state[dev].compare_exchange_strong(expected, 1)) {
+    known[dev] = *d;
+    state[dev].store(2, std::memory_order_release);
+  }
+  return e;
+}
+
 int fused_context_create(FusedContext* c) {
   memset(c, 0, sizeof(*c));
   FUSED_CUDA(cudaGetDevice(&c->device));
-  cudaDeviceProp prop;
-  FUSED_CUDA(cudaGetDeviceProperties(&prop, c->device));
-  if (prop.major != 10) return ROLLER_ERR_DEVICE;
-  c->dev.sm_count = prop.multiProcessorCount;
-  cudaError_t e = bind_device(&c->dev);
+  int major = 0;
+  FUSED_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, c->device));
+  if (major != 10) return ROLLER_ERR_DEVICE;
+  cudaError_t e = device_facts(c->device, &c->dev);
   if (e == cudaSuccess) e = cudaMalloc(&c->status, sizeof(uint32_t));
   if (e == cudaSuccess) e = cudaMemset(c->status, 0, sizeof(uint32_t));
   if (e == cudaSuccess) return ROLLER_OK;

@@ -520,7 +520,7 @@ struct FusedWork {
       tcgen05_fence_after_sync();
       const uint32_t d_tmem = me.tmem_base + static_cast<uint32_t>(r.acc * BN + me.half * Cfg::OUT_COLS) + tmem_lane;
       auto run = [&](auto act_tag) {
-        constexpr int ACT = decltype(act_tag)::value;
+        [[maybe_unused]] constexpr int ACT = decltype(act_tag)::value;
 #pragma unroll 1
         for (int k = 0; k < Cfg::OUT_COLS; k += 64) {
           const int col = col0 + k;
@@ -728,17 +728,17 @@ struct FusedWork {
     // The first slab's inputs have been sent for.
     auto epilogue = [&](const FusedTile& c, int slab0, int step, int slab_end, auto sums) {
       const int row0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM + me.quarter * 32;
-      const int row = row0 + me.lane;
+      [[maybe_unused]] const int row = row0 + me.lane;
       const int col_base = c.nb * (OP == kOpGate ? BN / 2 : BN);
       auto run = [&](auto act_tag) {
-        constexpr int ACT = decltype(act_tag)::value;
+        [[maybe_unused]] constexpr int ACT = decltype(act_tag)::value;
 #pragma unroll 1
         for (int i = slab0; i < slab_end; i += step) {
           const int tc = i * 32, col = col_base + tc;
           // (uniform over the warp; above the diagonal a slab is the mirror image of another one)
           if (!wanted(row0, col)) break;
           float v[32];
-          uint32_t raw[Cfg::INPUTS ? Cfg::INPUTS : 1][16];
+          uint32_t raw[Cfg::INPUTS ? Cfg::INPUTS : 1][16] = {};
           if constexpr (Cfg::INPUTS > 0) {
             r.ok = take(raw) && r.ok;
             // the next slab's inputs are on their way while this one is worked on

@@ -37,6 +37,21 @@ int fused_context_create(FusedContext* c);    // on the current device; a roller
 void fused_context_destroy(FusedContext* c);
 int fused_context_status(FusedContext* c, uint32_t* device_status);   // reads and clears
 
+// One allocation for all workspaces of a plan: sizes are asked for first, pointers given afterwards
+// (each on a 1024-byte boundary).
+struct Arena {
+  char* base = nullptr;
+  size_t bytes = 0;
+  size_t take(size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 1023) / 1024 * 1024;
+    return at;
+  }
+  cudaError_t allocate() { return cudaMalloc(&base, bytes); }
+  template <class T>
+  T* at(size_t offset) const { return reinterpret_cast<T*>(base + offset); }
+};
+
 // Operands whose rows do not start on 16 bytes are copied, all of a call's in one launch.
 struct AlignJob {
   const uint16_t* src;

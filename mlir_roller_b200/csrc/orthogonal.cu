@@ -224,6 +224,7 @@ struct roller_ortho_plan {
   bool tall;
   float a, b, c, eps;
   long long ldx, zsx, ldm, zsm;
+  Arena arena;
   double* part;            // partial sums of squares
   __half* x[2][2];         // [which][hi, lo], [batch][rows][ldx]
   __half *pm, *qm;         // p and q, [batch][m][ldm]
@@ -341,18 +342,24 @@ int roller_b200_ortho_create(int batch, int rows, int cols, int in_type, int ste
   p->zsx = p->ldx * rows;
   p->ldm = up64(p->m);
   p->zsm = p->ldm * p->m;
-  cudaError_t e = cudaMalloc(&p->part, sizeof(double) * kSumBlocks * batch);
-  for (int i = 0; i < 4 && e == cudaSuccess; ++i)
-    e = cudaMalloc(&p->x[i / 2][i % 2], sizeof(__half) * p->zsx * batch);
-  if (e == cudaSuccess) e = cudaMalloc(&p->pm, sizeof(__half) * p->zsm * batch);
-  if (e == cudaSuccess) e = cudaMalloc(&p->qm, sizeof(__half) * p->zsm * batch);
-  if (e == cudaSuccess) e = cudaMalloc(&p->vec, sizeof(float) * p->ldm * batch);
+  size_t x[4];
+  for (size_t& at : x) at = p->arena.take(sizeof(__half) * p->zsx * batch);
+  const size_t pm = p->arena.take(sizeof(__half) * p->zsm * batch), qm = p->arena.take(sizeof(__half) * p->zsm * batch);
+  const size_t vec = p->arena.take(sizeof(float) * p->ldm * batch);
+  const size_t part = p->arena.take(sizeof(double) * kSumBlocks * batch);
+  const cudaError_t e = p->arena.allocate();
   if (e != cudaSuccess) {
     const int failed = e == cudaErrorMemoryAllocation ? ROLLER_ERR_NOMEM : report_cuda_error(e, "ortho plan setup");
     cudaGetLastError();
+    p->arena.base = nullptr;
     roller_b200_ortho_destroy(p);
     return failed;
   }
+  for (int i = 0; i < 4; ++i) p->x[i / 2][i % 2] = p->arena.at<__half>(x[i]);
+  p->pm = p->arena.at<__half>(pm);
+  p->qm = p->arena.at<__half>(qm);
+  p->vec = p->arena.at<float>(vec);
+  p->part = p->arena.at<double>(part);
   const int built = build_products(p);
   if (built != ROLLER_OK) {
     roller_b200_ortho_destroy(p);
@@ -420,12 +427,7 @@ int roller_b200_ortho_status(roller_ortho_plan* p, uint32_t* device_status) {
 int roller_b200_ortho_destroy(roller_ortho_plan* p) {
   if (!p) return ROLLER_OK;
   for (Product* q : {p->gram[0], p->gram[1], p->poly, p->update[0], p->update[1], p->last[0], p->last[1]}) delete q;
-  cudaFree(p->part);
-  for (auto& pair : p->x)
-    for (__half* b : pair) cudaFree(b);
-  cudaFree(p->pm);
-  cudaFree(p->qm);
-  cudaFree(p->vec);
+  cudaFree(p->arena.base);
   fused_context_destroy(&p->ctx);
   cudaGetLastError();
   delete p;
