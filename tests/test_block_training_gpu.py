@@ -119,3 +119,59 @@ def test_orthogonal_offsets_beyond_32_bits():
     plan.destroy()
     ortho.check(out[-1], g[-1])
     assert torch.equal(out[0], out[batch // 2])
+
+
+@pytest.mark.parametrize("tokens,d,f", [(1, 512, 2048), (40, 512, 1536), (300, 264, 520), (90, 129, 257), (700, 768, 2000)])
+def test_calls_in_a_row_see_what_the_calls_before_them_wrote(tokens, d, f):
+    """Launches overlap (weights fetched early, independent gradient products side by side, copies of
+    unaligned operands behind the first product). A chain of two blocks whose weights are rewritten
+    right before every step gives the same bits with and without waiting in between."""
+    dtype = torch.bfloat16
+    fresh = [[block.make(tokens, d, f, dtype, seed=60 + 2 * i + j) for j in range(2)] for i in range(6)]
+
+    def chain(wait):
+        plans = [GatedFfnPlan(tokens, d, f, training=True) for _ in range(2)]
+        muon = OrthogonalPlan(f, d)
+        live = [{k: torch.zeros_like(v) for k, v in s.items()} for s in fresh[0]]
+        seen = []
+
+        def step():
+            if wait:
+                torch.cuda.synchronize()
+
+        for data in fresh:
+            for now, s in zip(live, data):
+                for k in s:
+                    now[k].copy_(s[k])
+            step()
+            x = live[0]["x"]
+            saved = []
+            for plan, w in zip(plans, live):
+                y = torch.empty_like(x)
+                g, u = plan.new_saved(tokens)
+                plan.forward(x, w["wg"], w["wu"], w["wd"], y, g, u)
+                step()
+                saved.append((x, g, u))
+                seen += [y, g, u]
+                x = y
+            dy = live[1]["dy"]
+            for plan, w, (x, g, u) in reversed(list(zip(plans, live, saved))):
+                dx, dwg, dwu, dwd = (torch.empty_like(t) for t in (x, w["wg"], w["wu"], w["wd"]))
+                plan.backward(x, w["wg"], w["wu"], w["wd"], g, u, dy, dx, dwg, dwu, dwd)
+                step()
+                update = torch.empty_like(dwg)
+                muon.run(dwg, update)
+                step()
+                w["wg"].add_(update, alpha=-0.1)       # the very next kernel writes a weight
+                w["wd"].add_(dwd)
+                step()
+                seen += [dx, dwg, dwu, dwd, update]
+                dy = dx
+        torch.cuda.synchronize()
+        for p in plans + [muon]:
+            p.check_status()
+            p.destroy()
+        return seen
+
+    for a, b in zip(chain(False), chain(True)):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
