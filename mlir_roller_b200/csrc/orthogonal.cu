@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(256) ortho_sumsq(Source s, double* __restrict_
   if (threadIdx.x == 0) part[blockIdx.y * kSumBlocks + blockIdx.x] = sum;
 }
 
-// x = S g / (|g| + eps) as hi + lo. Every block adds the partial sums in the same order.
+// x = S g / (|g| + eps) as hi + lo. Every block adds the partial sums in the same order. The factor
+// itself can leave fp32's range (norms under 1e-35 or over 1e40), so a power of two goes first.
 template <typename T>
 __global__ void __launch_bounds__(256)
 ortho_scale(Source s, const double* __restrict__ part, int parts, double eps, __half* __restrict__ hi,
@@ -153,7 +154,10 @@ ortho_scale(Source s, const double* __restrict__ part, int parts, double eps, __
   double sum = 0.0;
   for (int i = threadIdx.x; i < parts; i += 256) sum += part[blockIdx.y * kSumBlocks + i];
   sum = block_sum(sum);
-  const float scale = static_cast<float>(static_cast<double>(kScale) / (sqrt(sum) + eps));
+  const double norm = sqrt(sum) + eps;
+  const int e = ((__double2hiint(norm) >> 20) & 0x7FF) - 1023;
+  const float near_one = __uint_as_float(static_cast<uint32_t>(127 - max(-100, min(100, e))) << 23);
+  const float scale = static_cast<float>(static_cast<double>(kScale) / (norm * near_one));
 
   const T* g = static_cast<const T*>(s.g) + blockIdx.y * s.zs;
   const uint32_t rows = static_cast<uint32_t>(s.rows);
@@ -170,7 +174,7 @@ ortho_scale(Source s, const double* __restrict__ part, int parts, double eps, __
       alignas(16) __half h[8], l[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float f = v[i][j] * scale;
+        const float f = v[i][j] * near_one * scale;
         h[j] = __float2half_rn(f);
         l[j] = __float2half_rn(f - __half2float(h[j]));
       }

@@ -160,6 +160,16 @@ def test_zero_small_and_large():
     assert run(g * 1e-25).abs().max() < 1e-10
 
 
+def test_norms_whose_inverse_leaves_fp32():
+    # every element a normal number (subnormal ones count as zero)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    for shape, size in (((5, 7), 3e-37), ((5, 7), 1.6e38), ((300, 400), 1.6e38), ((400, 300), 1.6e38)):
+        signs = torch.randint(0, 2, shape, generator=gen, device="cuda") * 2 - 1
+        g = signs * (1 + torch.rand(shape, generator=gen, device="cuda")) * size
+        for dtype in (torch.float32, torch.bfloat16):
+            check(run(g.to(dtype), eps=0.0), g.to(dtype), eps=0.0)
+
+
 def test_not_finite_stays_in_its_matrix():
     g = make(64, 100, "decay", seed=6, batch=3)
     want = run(g)
