@@ -220,6 +220,13 @@ def _stream_ptr(stream) -> C.c_void_p:
     return C.c_void_p(getattr(stream, "cuda_stream", stream))
 
 
+def check_ints(**values) -> None:
+    """Refuses sizes that a C int would not hold (ctypes takes them modulo 2^32)."""
+    for name, v in values.items():
+        if not -(1 << 31) <= v < 1 << 31:
+            raise RollerError(ERR_INVALID, f"{name} = {v}")
+
+
 _torch = None
 
 

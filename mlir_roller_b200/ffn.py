@@ -65,6 +65,7 @@ class GatedFfnPlan:
             raise TypeError(f"the block exists for bf16 and fp16 operands, not {dtype}")
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation {activation!r} is not one of {sorted(ACTIVATIONS)}")
+        _lib.check_ints(max_tokens=max_tokens, d_model=d_model, d_ff=d_ff)
         self.max_tokens, self.d_model, self.d_ff = max_tokens, d_model, d_ff
         self.dtype, self.activation, self.training = dtype, activation, training
         _lib.check(self._lib.roller_b200_ffn_create(max_tokens, d_model, d_ff, modes[dtype],

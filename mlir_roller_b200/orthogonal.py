@@ -6,7 +6,8 @@ drives the singular values of each matrix g of a batch towards one and leaves it
 vectors. |g| is the Frobenius norm. Inputs are fp32, bf16 or fp16, [rows, cols] or [batch, rows, cols] with
 contiguous rows and any other strides; results are bf16. The products are fp16 with fp32 sums and
 x is carried with 22 bits in between, so that a matrix of low rank comes out as clean as a full
-one (about 2e-3 of |x| against 64 bits, most of it the last rounding to bf16).
+one (about 2e-3 of |x| against 64 bits, most of it the last rounding to bf16). Where |g| is under
+about 1e-5 eps the result, itself close to zero, keeps only an absolute accuracy.
 
 A plan owns the workspaces; calls only enqueue on a stream, and calls of one plan have to be ordered
 on the device. There is no CPU fallback. The reference has no counterpart: it multiplies two matrices
@@ -36,6 +37,7 @@ class OrthogonalPlan:
                  torch.float16: _lib.ORTHO_IN_F16}
         if dtype not in types:
             raise TypeError(f"inputs are fp32, bf16 or fp16, not {dtype}")
+        _lib.check_ints(batch=batch, rows=rows, cols=cols, steps=steps)
         self.batch, self.rows, self.cols, self.dtype = batch, rows, cols, dtype
         self._out_dtype = torch.bfloat16
         a, b, c = coefficients

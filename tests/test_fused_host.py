@@ -93,3 +93,14 @@ def test_plans_name_what_they_do_not_take():
     with pytest.raises(_lib.RollerError) as e:
         OrthogonalPlan(4, 4, steps=0)
     assert e.value.status == _lib.ERR_INVALID
+
+
+def test_sizes_beyond_a_c_int_are_refused():
+    from mlir_roller_b200 import GatedFfnPlan, OrthogonalPlan
+    wrap = (1 << 32) + 8          # modulo 2^32 an ordinary size
+    for make in (lambda: GatedFfnPlan(wrap, 8, 8), lambda: GatedFfnPlan(8, wrap, 8), lambda: GatedFfnPlan(8, 8, wrap),
+                 lambda: OrthogonalPlan(wrap, 8), lambda: OrthogonalPlan(8, wrap), lambda: OrthogonalPlan(8, 8, batch=wrap),
+                 lambda: OrthogonalPlan(8, 8, steps=wrap)):
+        with pytest.raises(_lib.RollerError) as e:
+            make()
+        assert e.value.status == _lib.ERR_INVALID
