@@ -359,8 +359,8 @@ typedef struct roller_ffn_io {
 } roller_ffn_io;
 
 /* Binds the block to the current device. `mode` is ROLLER_MODE_BF16 or ROLLER_MODE_F16,
- * `activation` a ROLLER_ACT_*. Allocates the workspaces (H, partial sums, padded copies of operands
- * whose rows are not a multiple of 16 bytes when they are contiguous). max_tokens and the widths
+ * `activation` a ROLLER_ACT_*. Allocates the workspaces (H, the gradients of G and U, aligned copies of
+ * operands whose rows are not a multiple of 16 bytes when they are contiguous). max_tokens and the widths
  * are 1 .. 2^20. There is no counterpart in the reference, whose generated kernels have no
  * epilogue (src/roller.py:47-68). */
 int roller_b200_ffn_create(int max_tokens, int d_model, int d_ff, int mode, int activation, int flags,
@@ -395,7 +395,9 @@ int roller_b200_ffn_destroy(roller_ffn_plan* plan);
  * one, as the Muon optimiser does with the update of a weight matrix. |G| is the Frobenius norm
  * of one matrix. The products run on the shorter side of the matrix, in fp16 with fp32 sums; X
  * itself is carried as a pair of fp16 numbers (22 bits), because whatever is rounded off it in a
- * weak direction grows with that direction, about a-fold per step. */
+ * weak direction grows with that direction, about a-fold per step. Its elements are held to 2^-35 at
+ * best, which matters only where |G| is under about 1e-5 eps: there the result, itself close to
+ * zero, is off by up to 2^-35 a^steps per element. Subnormal inputs in fp32 and bf16 count as zero. */
 typedef struct roller_ortho_plan roller_ortho_plan;
 
 #define ROLLER_ORTHO_IN_F32 0

@@ -412,3 +412,32 @@ def test_refusals():
     plan.destroy()
     with pytest.raises(RuntimeError):
         plan.forward(s["x"], *w, y)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_far_out_activations_stay_finite(act):
+    # beyond 1.8e19 the square of g leaves fp32; the activation is g or zero there, its slope one or zero
+    s = make(9, 40, 24, torch.bfloat16, 21)
+    sign = torch.ones(9, 24, device="cuda")
+    sign[::2] = -1
+    s["g"] = (sign * 1e25).bfloat16()
+    s["u"] = torch.full_like(s["g"], 1e-20)
+    plan = GatedFfnPlan(9, 40, 24, activation=act, training=True)
+    out = [torch.empty_like(s[k]) for k in ("x", "wg", "wu", "wd")]
+    plan.backward(*(s[k] for k in ("x", "wg", "wu", "wd", "g", "u", "dy")), *out)
+    plan.check_status()
+    plan.destroy()
+    a, slope = torch.where(sign > 0, s["g"].double(), 0.0), (sign > 0).double()
+    # dg, du, h: one rounding each; the products: another, and their sums
+    dh = s["dy"].double() @ s["wd"].double()
+    dg, du, h = dh * s["u"].double() * slope, dh * a, a * s["u"].double()
+    off = acc(40) * (s["dy"].double().abs() @ s["wd"].double().abs())
+    u_ = half_step(torch.bfloat16)
+    for got, parts in ((out[0], ((dg, off * s["u"].double() * slope, s["wg"].double()), (du, off * a, s["wu"].double()))),
+                       (out[1], ((dg.T, (off * s["u"].double() * slope).T, s["x"].double()),)),
+                       (out[2], ((du.T, (off * a).T, s["x"].double()),)),
+                       (out[3], ((s["dy"].double().T, torch.zeros(40, 9, device="cuda", dtype=torch.float64), h),))):
+        want = sum(p @ m for p, _, m in parts)
+        # (u_ on either operand, whichever was rounded)
+        bound = sum((e + (2 * u_ + acc(49) + 2.0 ** -20) * p.abs()) @ m.abs() for p, e, m in parts)
+        within(got, want, bound + u_ * (want.abs() + bound) + tiny(torch.bfloat16), "gradient")
