@@ -515,6 +515,16 @@ struct FusedWork {
       const int col0 = c.nb * BN + me.half * Cfg::OUT_COLS;
       __syncwarp();
       if (col0 < p.out_cols) fetch(c, row0, col0);       // they do not depend on the product
+      // vec of the thread's row (q x), or of every 32nd column of the warp's from `lane` on (x q);
+      // asked for here, because in the loop below its way from L2 would be waited for
+      [[maybe_unused]] float scale[OP == kOpUpdateTall ? Cfg::OUT_COLS / 32 : 1] = {};
+      if constexpr (Cfg::UPDATE) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(scale) / sizeof(float)); ++i) {
+          const int at = OP == kOpUpdateTall ? col0 + i * 32 + me.lane : row;
+          if (at < (OP == kOpUpdateTall ? p.out_cols : p.M)) scale[i] = __ldcg(p.vec + c.z * p.vec_ld + at);
+        }
+      }
       r.ok = mbar_wait_warp(me.tmem_full_bar(r.acc), r.acc_ph, me.wc, kDevTimeoutTmemFull);
       if (!r.ok) break;
       tcgen05_fence_after_sync();
@@ -559,23 +569,15 @@ struct FusedWork {
               put(2, half, h, IntTag<DT>{});
             } else {
               // x = vec x + D / S; vec belongs to rows (q x) or columns (x q)
-              if constexpr (OP == kOpUpdateWide) {
-                const float s = row < p.M ? __ldcg(p.vec + c.z * p.vec_ld + row) : 0.0f;
+              float of_columns = 0.0f;
+              if constexpr (OP == kOpUpdateTall) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  v[j] = s * (element(raw0, j) + element(raw1, j)) + __uint_as_float(d[j]) * p.inv_scale;
-              } else {
-                // (rows of vec are padded to 64; what lies in the padding meets columns that are not stored)
-                const float4* s4 = reinterpret_cast<const float4*>(p.vec + c.z * p.vec_ld + col + half * 32);
+                for (int i = 0; i < Cfg::OUT_COLS / 32; ++i) of_columns = i == k / 32 + half ? scale[i] : of_columns;
+              }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const float4 s = __ldcg(s4 + j);
-                  const float sv[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-                  for (int i = 0; i < 4; ++i)
-                    v[4 * j + i] = sv[i] * (element(raw0, 4 * j + i) + element(raw1, 4 * j + i)) +
-                                   __uint_as_float(d[4 * j + i]) * p.inv_scale;
-                }
+              for (int j = 0; j < 32; ++j) {
+                const float f = OP == kOpUpdateTall ? __shfl_sync(0xffffffffu, of_columns, j) : scale[0];
+                v[j] = f * (element(raw0, j) + element(raw1, j)) + __uint_as_float(d[j]) * p.inv_scale;
               }
               if (p.flags & kFusedLast) {
 #pragma unroll
