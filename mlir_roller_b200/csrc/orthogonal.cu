@@ -145,6 +145,8 @@ __global__ void __launch_bounds__(256) ortho_sumsq(Source s, double* __restrict_
 
 // x = S g / (|g| + eps) as hi + lo. Every block adds the partial sums in the same order. The factor
 // itself can leave fp32's range (norms under 1e-35 or over 1e40), so a power of two goes first.
+// Norm and scaling of 8192 x 4096 in fp32 take 48 us together, about what writing hi and lo and
+// reading g twice take (403 MB, a part of the second time from L2).
 template <typename T>
 __global__ void __launch_bounds__(256)
 ortho_scale(Source s, const double* __restrict__ part, int parts, double eps, __half* __restrict__ hi,

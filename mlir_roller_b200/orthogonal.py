@@ -6,8 +6,10 @@ drives the singular values of each matrix g of a batch towards one and leaves it
 vectors. |g| is the Frobenius norm. Inputs are fp32, bf16 or fp16, [rows, cols] or [batch, rows, cols] with
 contiguous rows and any other strides; results are bf16. The products are fp16 with fp32 sums and
 x is carried with 22 bits in between, so that a matrix of low rank comes out as clean as a full
-one (about 2e-3 of |x| against 64 bits, most of it the last rounding to bf16). Where |g| is under
-about 1e-5 eps the result, itself close to zero, keeps only an absolute accuracy.
+one (about 2e-3 of |x| against 64 bits, most of it the last rounding to bf16; up to 1.4e-2 with fewer
+than eight rows or columns, where one singular value at a steep place of the iteration is all there
+is). Where |g| is under about 1e-5 eps the result, itself close to zero, keeps only an absolute
+accuracy.
 
 A plan owns the workspaces; calls only enqueue on a stream, and calls of one plan have to be ordered
 on the device. There is no CPU fallback. The reference has no counterpart: it multiplies two matrices
