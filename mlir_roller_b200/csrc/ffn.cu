@@ -5,8 +5,8 @@
 //   backward   kOpDact:  dh = dy Wd, from which dg, du and h leave together (dh itself stays in the
 //                        accumulator, and h is made again from g and u rather than kept)
 //              kOpDx:    dx = dg Wg + du Wu, one reduction over both
-//              kOpDw:    dWg = dg^T x and dWu = du^T x in one launch; dWd = dy^T h
-//              The last three launches need only what kOpDact wrote, so they overlap
+//              kOpDw:    dWg = dg^T x, dWu = du^T x and dWd = dy^T h in one launch: tiles of equal length
+//              The last two launches need only what kOpDact wrote, so they overlap
 //              (FusedParams::late_wait); kOpDx goes first, because its few long tiles leave SMs free.
 #include <cstring>
 #include <new>
@@ -19,7 +19,7 @@ namespace {
 
 constexpr int kMaxExtent = 1 << 20;
 
-enum { kPGate = 0, kPDown, kPDact, kPDx, kPDwUp, kPDwDown, kProducts };
+enum { kPGate = 0, kPDown, kPDact, kPDx, kPDw, kProducts };
 enum Operand { kX = 0, kWg, kWu, kWd, kDy, kG, kU, kOperands };
 
 }  // namespace
@@ -86,7 +86,7 @@ const FusedChoice* choices(roller_ffn_plan* p, int T) {
   if (p->chosen_tokens != T) {
     const FusedShape shapes[kProducts] = {
         {kOpGate, p->dt, T, p->f, p->d, 1}, {kOpDown, p->dt, T, p->d, p->f, 1}, {kOpDact, p->dt, T, p->f, p->d, 1},
-        {kOpDx, p->dt, T, p->d, p->f, 1},   {kOpDw, p->dt, p->f, p->d, T, 2},   {kOpDw, p->dt, p->d, p->f, T, 1}};
+        {kOpDx, p->dt, T, p->d, p->f, 1},   {kOpDw, p->dt, p->f, p->d, T, 2}};
     for (int i = 0; i < (p->training ? kProducts : kPDact); ++i) p->choice[i] = fused_choose(shapes[i], p->ctx.dev);
     p->chosen_tokens = T;
   }
@@ -266,20 +266,16 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     FUSED_OK(r.output(0, io->dx.ptr, 1, io->dx.ld, 0, bf16));
     FUSED_OK(r.launch(st));
   }
-  {
-    Product w(p->ctx, kOpDw, p->dt, F, D, T, 2, &choice[kPDwUp]);
-    w.p.late_wait = 1;   // dg, du and h were complete before the kernel above started
-    FUSED_OK(w.a_mn(p->dgu, F, T, 2, p->ldf, zs));
-    FUSED_OK(w.b_mn(0, x, D, T, 1, ldx, 0));
-    FUSED_OK(w.output(0, io->dwg.ptr, 1, io->dwg.ld, 0, bf16));
-    FUSED_OK(w.output(1, io->dwu.ptr, 1, io->dwu.ld, 0, bf16));
-    FUSED_OK(w.launch(st));
-  }
-  Product w(p->ctx, kOpDw, p->dt, D, F, T, 1, &choice[kPDwDown]);
-  w.p.late_wait = 1;
-  FUSED_OK(w.a_mn(dy, D, T, 1, ldy, 0));
-  FUSED_OK(w.b_mn(0, p->h, F, T, 1, p->ldf, 0));
-  FUSED_OK(w.output(0, io->dwd.ptr, 1, io->dwd.ld, 0, bf16));
+  Product w(p->ctx, kOpDw, p->dt, F, D, T, 2, &choice[kPDw]);
+  w.p.late_wait = 1;   // dg, du and h were complete before the kernel above started
+  fused_deal(choice[kPDx], choice[kPDw], p->ctx.dev, &w.p.head, &w.p.head_tiles);
+  FUSED_OK(w.a_mn(p->dgu, F, T, 2, p->ldf, zs));
+  FUSED_OK(w.b_mn(0, x, D, T, 1, ldx, 0));
+  FUSED_OK(w.output(0, io->dwg.ptr, 1, io->dwg.ld, 0, bf16));
+  FUSED_OK(w.output(1, io->dwu.ptr, 1, io->dwu.ld, 0, bf16));
+  FUSED_OK(w.a2_mn(dy, D, T, ldy));
+  FUSED_OK(w.b_mn(1, p->h, F, T, 1, p->ldf, 0));
+  FUSED_OK(w.output(2, io->dwd.ptr, 1, io->dwd.ld, 0, bf16));
   return w.launch(st);
 }
 

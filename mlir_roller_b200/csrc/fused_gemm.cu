@@ -170,8 +170,8 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
   double best_us = 0.0;
   const bool sym = s.op == kOpGramWide || s.op == kOpGramTall || s.op == kOpPoly;
   const double halves = s.op == kOpGate || s.op == kOpDx ? 2.0 : 1.0;
-  const double stream_us = halves * s.K * (s.op == kOpGate ? s.M / 2.0 + s.N : sym ? s.N : s.M + s.N) *
-                           (s.op == kOpDw ? 1 : s.zcount) * 2.0 / 6.2e6;
+  const double stream_us = halves * s.K * (s.op == kOpGate ? s.M / 2.0 + s.N : s.op == kOpDw ? 1.5 * s.M + s.N : sym ? s.N : s.M + s.N) *
+                           s.zcount * 2.0 / 6.2e6;
   for (const TileCost& c : kTiles) {
     const FusedVariant* kv = fused_find(s.op, c.cta_group, c.block_n, s.dt);
     if (!kv) continue;
@@ -187,7 +187,11 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
     }
     f.num_kb = static_cast<int>((s.K + 63) / 64);
     const int kbs = f.num_kb * (s.op == kOpDx ? 2 : 1);
-    const long long tiles = static_cast<long long>(f.tiles_per_z) * s.zcount;
+    if (s.op == kOpDw) {
+      f.tiles_m2 = static_cast<int>((s.N + bm - 1) / bm);
+      f.tiles_n2 = static_cast<int>((s.M + bn - 1) / bn);
+    }
+    const long long tiles = static_cast<long long>(f.tiles_per_z) * s.zcount + f.tiles_m2 * f.tiles_n2;
     for (int split = 1; split <= kv->max_split && split <= kbs; split *= 2) {
       const int ctas = c.cta_group * split;                       // of a cluster
       const long long at_once = d.clusters[ctas == 1 ? 0 : ctas == 2 ? 1 : ctas == 4 ? 2 : 3];
@@ -206,10 +210,34 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
       best_us = us;
       best = f;
       best.split = split;
+      best.tiles = static_cast<int>(tiles);
+      best.at_once = static_cast<int>(at_once);
+      best.tile_us = tile_us > epilogue_us ? tile_us : epilogue_us;
       best.grid = static_cast<int>(split > 1 ? tiles : tiles < at_once ? tiles : at_once) * ctas;
     }
   }
   return best;
+}
+
+// SMs that the last wave of `before` leaves idle start on kOpDw's tiles that much earlier, and take
+// more of them: as many more as let the busiest worker end first.
+void fused_deal(const FusedChoice& before, const FusedChoice& dw, const FusedDevice& d, int* head, int* head_tiles) {
+  *head = *head_tiles = 0;
+  if (dw.split > 1) return;
+  const int last = (before.tiles - 1) % before.at_once + 1;
+  const int h = (d.sm_count - last * before.kv->cta_group * before.split) / dw.kv->cta_group;
+  const int workers = dw.grid / dw.kv->cta_group;
+  if (h < 1 || h >= workers) return;
+  const double lead = before.tile_us / dw.tile_us;      // in tiles of kOpDw
+  double best = 0.0;
+  for (int more = 0; more <= lead + 1 && more * h <= dw.tiles; ++more) {
+    const int rest = (dw.tiles - more * h + workers - 1) / workers;
+    const double end = rest + (more > lead ? more : lead);
+    if (more > 0 && end >= best) continue;
+    best = end;
+    *head = more ? h : 0;
+    *head_tiles = more * h;
+  }
 }
 
 // What bind_device found on each device: asking again costs every new plan the better part of a

@@ -27,7 +27,8 @@ constexpr int kFusedLast = 2;   // kOpUpdate*: the result leaves as bf16, divide
 // Everything one launch needs. Matrices are [z][rows][columns]; leading dimensions in elements.
 struct FusedParams {
   CUtensorMap a;        // first operand
-  CUtensorMap b[2];     // second operand (kOpGate: Wg, Wu; kOpDx: the operand of each half)
+  CUtensorMap a2;       // kOpDw: first operand of dWd
+  CUtensorMap b[2];     // second operand (kOpGate: Wg, Wu; kOpDx: of each half; kOpDw: x, h)
   CUtensorMap o[3];     // outputs as store destinations, where out_tma says so
   void* out[3];
   long long out_ld[3];
@@ -41,6 +42,8 @@ struct FusedParams {
   int num_kb;           // k-blocks of 64 (of each half in kOpDx)
   int a_bytes;          // bytes one TMA load of A brings (fewer rows than 128 on single CTAs)
   int tiles_m, tiles_n, tiles_per_z, zcount;
+  int M2, out_cols2, tiles_m2, tiles_n2;   // kOpDw: of dWd, whose tiles come behind the zcount others
+  int head, head_tiles;                    // kOpDw: FusedWork::next
   int split;            // parts of a cluster that share a tile's k (1 = none)
   int b_early;          // the second operand may be read before the previous kernel is done ...
   int late_wait;        // ... or everything: that kernel is only waited for at the end
@@ -68,13 +71,16 @@ const FusedVariant* fused_find(int op, int cta_group, int block_n, int dt);
 // A problem as the choice of a kernel sees it.
 struct FusedShape {
   int op, dt;
-  long long M, N;       // of D (kOpGate: N = columns of one weight's product)
+  long long M, N;       // of D (kOpGate: of one weight's product; kOpDw: of dWg, and dWd is N x M)
   long long K;          // of one half in kOpDx
   int zcount;
 };
 struct FusedChoice {
   const FusedVariant* kv;
   int tiles_m, tiles_n, tiles_per_z, num_kb, split, grid;
+  int tiles_m2, tiles_n2;   // kOpDw: of dWd
+  int tiles, at_once;       // in all; clusters that run at once
+  double tile_us;           // estimated time of a tile
 };
 // What the current device holds at once: CTAs of one per SM, and clusters of 2, 4 and 8.
 struct FusedDevice {
@@ -82,4 +88,6 @@ struct FusedDevice {
   int clusters[4];     // [i]: clusters of 2^i CTAs
 };
 FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d);
+// How kOpDw's tiles are dealt when it starts beside the last wave of `before` (FusedWork::next).
+void fused_deal(const FusedChoice& before, const FusedChoice& dw, const FusedDevice& d, int* head, int* head_tiles);
 }  // namespace rb200

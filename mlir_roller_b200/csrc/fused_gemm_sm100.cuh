@@ -7,7 +7,7 @@
 //   kOpDown         h Wd^T                          D
 //   kOpDact         dh = dy Wd                      dg = dh u act'(g), du = dh act(g), h = act(g) u
 //   kOpDx           [dg du] [Wg; Wu]                D
-//   kOpDw           dg^T x, du^T x (or dy^T h)      D
+//   kOpDw           dg^T x, du^T x and dy^T h       D
 //   kOpGramWide     x x^T  (kOpGramTall: x^T x)     p = D / S, on both sides of the diagonal
 //   kOpPoly         p p                             q = b p + c D / S, likewise; vec = a + what the
 //                                                   rounding of q's diagonal lost, / S
@@ -335,7 +335,7 @@ struct FusedWork {
 
   __device__ FusedWork(const FusedParams& p_, const FusedCta& me_) : p(p_), me(me_) {
     per_z = p.tiles_per_z;
-    tiles = per_z * p.zcount;
+    tiles = per_z * p.zcount + (OP == kOpDw ? p.tiles_m2 * p.tiles_n2 : 0);
     total_kb = p.num_kb * (OP == kOpDx ? 2 : 1);
     workers = static_cast<int>(gridDim.x) / (CG * me.split);
     worker = static_cast<int>(blockIdx.x) / (CG * me.split);
@@ -344,6 +344,29 @@ struct FusedWork {
     in_boxes = me.staging + static_cast<uint32_t>(me.warp - Cfg::FIRST_EPI_WARP) * (Cfg::WARP_BOXES * Cfg::BOX_BYTES);
     boxes = in_boxes + (Cfg::WIDE ? 0 : Cfg::INPUTS) * Cfg::BOX_BYTES;
     tmem_lane = static_cast<uint32_t>(me.quarter * 32) << 16;
+  }
+
+  // Where tile t is. (kOpDw: dWd's tiles, z = 2, come behind those of dWg and dWu.)
+  __device__ __forceinline__ FusedTile tile(int t) const {
+    if constexpr (OP == kOpDw) {
+      const int behind = t - per_z * p.zcount;
+      if (behind >= 0) {
+        FusedTile c = fused_tile<0>(behind, p.tiles_m2, p.tiles_n2, p.tiles_m2 * p.tiles_n2);
+        c.z = 2;
+        return c;
+      }
+    }
+    return fused_tile<Cfg::SYM_RATIO>(t, p.tiles_m, p.tiles_n, per_z);
+  }
+  __device__ __forceinline__ int rows(const FusedTile& c) const { return OP == kOpDw && c.z == 2 ? p.M2 : p.M; }
+  __device__ __forceinline__ int cols(const FusedTile& c) const { return OP == kOpDw && c.z == 2 ? p.out_cols2 : p.out_cols; }
+  // A worker's first tile, and the one after t. In kOpDw the first `head` workers, which find an SM while the
+  // previous kernel's last wave is still busy, have the first head_tiles to themselves.
+  // (Workers start in the order of their index; if they did not, only the balance would suffer.)
+  __device__ __forceinline__ int first() const { return OP == kOpDw && worker >= p.head ? p.head_tiles + worker : worker; }
+  __device__ __forceinline__ int next(int t) const {
+    if (OP != kOpDw || t >= p.head_tiles) return t + workers;
+    return t + p.head < p.head_tiles ? t + p.head : p.head_tiles + worker;
   }
 
   // ---------------------------------------------------------------- TMA producer (warp 0)
@@ -356,8 +379,9 @@ struct FusedWork {
     auto load_a = [&](int s, uint32_t bar, const FusedTile& c, int kb) {
       const int phase = (OP == kOpDx && kb >= p.num_kb) ? 1 : 0;
       const int m0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM;
-      fused_load<Cfg::BM, Cfg::A_MN, CG == 2>(me.smem_base + s * Cfg::STAGE_BYTES, &p.a, bar, m0,
-                                              (kb - phase * p.num_kb) * Cfg::BK, OP == kOpDx ? phase : c.z);
+      const bool second = OP == kOpDw && c.z == 2;
+      fused_load<Cfg::BM, Cfg::A_MN, CG == 2>(me.smem_base + s * Cfg::STAGE_BYTES, second ? &p.a2 : &p.a, bar, m0,
+                                              (kb - phase * p.num_kb) * Cfg::BK, OP == kOpDx ? phase : second ? 0 : c.z);
     };
     auto load_b = [&](int s, uint32_t bar, const FusedTile& c, int kb) {
       const uint32_t b_dst = me.smem_base + s * Cfg::STAGE_BYTES + Cfg::A_BYTES;
@@ -375,7 +399,7 @@ struct FusedWork {
       } else {
         const int bz = (OP == kOpDw || OP == kOpDx) ? 0 : c.z;
         const int n0 = c.nb * BN + static_cast<int>(me.cta_rank) * Cfg::BNL;
-        fused_load<Cfg::BNL, Cfg::B_MN, CG == 2>(b_dst, &p.b[phase], bar, n0, k0, bz);
+        fused_load<Cfg::BNL, Cfg::B_MN, CG == 2>(b_dst, &p.b[OP == kOpDw ? c.z >> 1 : phase], bar, n0, k0, bz);
       }
     };
     // The barrier that counts the bytes of both operands (for a pair: of both CTAs, on the leader's,
@@ -388,10 +412,10 @@ struct FusedWork {
         mbar_expect_tx(me.full_bar(s), p.a_bytes + Cfg::B_BYTES);
       }
     };
-    for (int t = worker; r.ok && t < tiles; t += workers) {
-      const FusedTile c = fused_tile<Cfg::SYM_RATIO>(t, p.tiles_m, p.tiles_n, per_z);
+    for (int t = first(); r.ok && t < tiles; t = next(t)) {
+      const FusedTile c = tile(t);
       int kb = kb0;
-      if (t == worker) {
+      if (t == first()) {
         const int early = p.b_early ? min(STAGES, kb1 - kb0) : 0;    // (of a launch's first tiles)
         if (issues) {
           for (int i = 0; i < early; ++i) {
@@ -427,7 +451,7 @@ struct FusedWork {
                                               DT == 1 ? 1u : 0u);
     // one MMA covers 16 k: 32 bytes along a k-contiguous row, or 16 rows of 128 bytes
     constexpr uint64_t a_step = Cfg::A_MN ? 128 : 2, b_step = Cfg::B_MN ? 128 : 2;
-    for (int t = worker; r.ok && t < tiles; t += workers) {
+    for (int t = first(); r.ok && t < tiles; t = next(t)) {
       if (!mbar_wait_warp(me.tmem_empty_bar(r.acc), r.acc_ph ^ 1u, me.wc, kDevTimeoutTmemEmpty)) { r.ok = false; break; }
       tcgen05_fence_after_sync();
       const uint32_t d_tmem = me.tmem_base + static_cast<uint32_t>(r.acc * BN);
@@ -522,8 +546,8 @@ struct FusedWork {
     };
 
     if (!before_loads()) r.ok = false;
-    for (int t = worker; r.ok && t < tiles; t += workers) {
-      const FusedTile c = fused_tile<0>(t, p.tiles_m, p.tiles_n, per_z);
+    for (int t = first(); r.ok && t < tiles; t = next(t)) {
+      const FusedTile c = tile(t);
       const int row0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM + me.quarter * 32;
       const int row = row0 + me.lane;
       const int col0 = c.nb * BN + me.half * Cfg::OUT_COLS;
@@ -692,14 +716,14 @@ struct FusedWork {
         fence_proxy_async_smem();
         __syncwarp();
         if (me.lane == 0) {
-          if (row0 < p.M) tma_store_3d(&p.o[o], box, col, row0, oz);
+          if (row0 < rows(c)) tma_store_3d(&p.o[o], box, col, row0, oz);
           bulk_commit_group();
         }
       } else {
         // rows that start anywhere: a warp writes 32 consecutive elements per instruction
         __syncwarp();
         uint16_t* dst = static_cast<uint16_t*>(p.out[o]) + oz * p.out_zstride + static_cast<long long>(row0) * p.out_ld[o] + col + me.lane;
-        const int rows = col + me.lane < p.out_cols ? p.M - row0 : 0;
+        const int left = col + me.lane < cols(c) ? rows(c) - row0 : 0;
 #pragma unroll 1
         for (int r0 = 0; r0 < 32; r0 += 8) {
           uint16_t x[8];
@@ -711,7 +735,7 @@ struct FusedWork {
                          : "memory");
 #pragma unroll
           for (int r = 0; r < 8; ++r)
-            if (r0 + r < rows) dst[(r0 + r) * p.out_ld[o]] = x[r];
+            if (r0 + r < left) dst[(r0 + r) * p.out_ld[o]] = x[r];
         }
         if (me.lane == 0) bulk_commit_group();   // (an empty group keeps the ring's count)
       }
@@ -737,7 +761,7 @@ struct FusedWork {
     };
 
     // Whether a slab has anything to do (it decides whether inputs are sent for).
-    auto wanted = [&](int row0, int col) { return col < p.out_cols && (!Cfg::SYM || col <= row0); };
+    auto wanted = [&](const FusedTile& c, int row0, int col) { return col < cols(c) && (!Cfg::SYM || col <= row0); };
 
     // The epilogue of this warp's slabs slab0, slab0 + step, .. < slab_end of tile `c`. Slab i is the 32
     // result columns from tile column 32 i on; `sums(tile_col, v)` gives 32 columns of D.
@@ -752,13 +776,13 @@ struct FusedWork {
         for (int i = slab0; i < slab_end; i += step) {
           const int tc = i * 32, col = col_base + tc;
           // (uniform over the warp; above the diagonal a slab is the mirror image of another one)
-          if (!wanted(row0, col)) break;
+          if (!wanted(c, row0, col)) break;
           float v[32];
           uint32_t raw[Cfg::INPUTS ? Cfg::INPUTS : 1][16] = {};
           if constexpr (Cfg::INPUTS > 0) {
             r.ok = take(raw) && r.ok;
             // the next slab's inputs are on their way while this one is worked on
-            if (i + step < slab_end && wanted(row0, col + step * 32)) fetch(c, row0, col + step * 32);
+            if (i + step < slab_end && wanted(c, row0, col + step * 32)) fetch(c, row0, col + step * 32);
           }
           auto input = [&](int q, int k) {      // element k of input q
             const float2 f = fused_unpack<DT>(raw[q][k / 2]);
@@ -819,12 +843,12 @@ struct FusedWork {
 
     if (me.split == 1) {
       if (!before_loads()) r.ok = false;
-      for (int t = worker; r.ok && t < tiles; t += workers) {
-        const FusedTile c = fused_tile<Cfg::SYM_RATIO>(t, p.tiles_m, p.tiles_n, per_z);
+      for (int t = first(); r.ok && t < tiles; t = next(t)) {
+        const FusedTile c = tile(t);
         if constexpr (Cfg::INPUTS > 0) {     // they do not depend on the product
           const int col = c.nb * BN + me.half * Cfg::OUT_COLS;
           const int row0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM + me.quarter * 32;
-          if (wanted(row0, col)) fetch(c, row0, col);
+          if (wanted(c, row0, col)) fetch(c, row0, col);
         }
         r.ok = __all_sync(0xffffffffu, mbar_wait(me.tmem_full_bar(r.acc), r.acc_ph, me.wc, kDevTimeoutTmemFull));
         if (!r.ok) break;
@@ -844,9 +868,9 @@ struct FusedWork {
     } else {
       // ---- the cluster holds the tile's parts: their sums are put together, each CTA taking a share
       // of the slabs: slab i is received by part i / share, or by every `apart`-th part
-      const FusedTile c = fused_tile<Cfg::SYM_RATIO>(worker, p.tiles_m, p.tiles_n, per_z);
+      const FusedTile c = tile(worker);
       const int row0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM + me.quarter * 32;
-      const bool row_ok = row0 + me.lane < p.M;
+      const bool row_ok = row0 + me.lane < rows(c);
       const int share = max(Cfg::SLABS / me.split, 1), apart = max(me.split / Cfg::SLABS, 1);
       const int my_slab = static_cast<int>(me.part) / apart * share;
       const bool receives = static_cast<int>(me.part) % apart == 0 && me.half < share;
@@ -854,7 +878,7 @@ struct FusedWork {
         before_loads();
         if constexpr (Cfg::INPUTS > 0) {
           const int col = c.nb * BN + (my_slab + me.half) * 32;
-          if (receives && wanted(row0, col)) fetch(c, row0, col);
+          if (receives && wanted(c, row0, col)) fetch(c, row0, col);
         }
         r.ok = __all_sync(0xffffffffu, mbar_wait(me.tmem_full_bar(0), 0u, me.wc, kDevTimeoutTmemFull));
       }
@@ -930,7 +954,7 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&p.a);
     tma_prefetch_desc(&p.b[0]);
-    if (Cfg::OP == kOpGate || Cfg::OP == kOpDx) tma_prefetch_desc(&p.b[1]);
+    if (Cfg::OP == kOpGate || Cfg::OP == kOpDx || Cfg::OP == kOpDw) tma_prefetch_desc(&p.b[1]);
     tma_prefetch_desc(&p.o[0]);
   }
   const FusedCta x = fused_begin<Cfg>(smem_dyn, p.split, p.status, p.spin_limit);

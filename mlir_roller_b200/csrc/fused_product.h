@@ -86,6 +86,10 @@ struct Product {
     p.tiles_m = c.tiles_m;
     p.tiles_n = c.tiles_n;
     p.tiles_per_z = c.tiles_per_z;
+    p.M2 = static_cast<int>(N);
+    p.out_cols2 = static_cast<int>(M);
+    p.tiles_m2 = c.tiles_m2;
+    p.tiles_n2 = c.tiles_n2;
     p.zcount = z;
     p.split = c.split;
     p.status = x.status;
@@ -104,6 +108,9 @@ struct Product {
     p.a_bytes = 128 * 128;
     return encode_batch16(&p.a, base, cols, rows, z, ld, zs, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, bf16);
   }
+  int a2_mn(const void* base, long long cols, long long rows, long long ld) {
+    return encode_batch16(&p.a2, base, cols, rows, 1, ld, 0, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, bf16);
+  }
   int b_k(int i, const void* base, long long cols, long long rows, long long z, long long ld, long long zs) {
     const int box = op == kOpGate ? c.kv->block_n / 2 : c.kv->block_n / c.kv->cta_group;
     return encode_batch16(&p.b[i], base, cols, rows, z, ld, zs, 64, box, CU_TENSOR_MAP_SWIZZLE_128B, bf16);
@@ -112,9 +119,9 @@ struct Product {
     return encode_batch16(&p.b[i], base, cols, rows, z, ld, zs, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, bf16);
   }
   // The boxes one epilogue warp reads and writes (FusedCfg::WIDE).
-  int box_map(CUtensorMap* map, const void* base, long long z, long long ld, long long zs, bool as_bf16) const {
+  int box_map(CUtensorMap* map, const void* base, long long z, long long ld, long long zs, bool as_bf16, bool second = false) const {
     const bool wide = op == kOpDact || op == kOpUpdateWide || op == kOpUpdateTall;
-    return encode_batch16(map, base, p.out_cols, p.M, z, ld, zs, wide ? 64 : 32, 32,
+    return encode_batch16(map, base, second ? p.out_cols2 : p.out_cols, second ? p.M2 : p.M, z, ld, zs, wide ? 64 : 32, 32,
                           wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, as_bf16);
   }
   int output(int i, void* base, long long z, long long ld, long long zs, bool as_bf16) {
@@ -123,7 +130,7 @@ struct Product {
     p.out_zstride = zs;
     if (!aligned16(base, ld) || (z > 1 && (zs % 8 != 0 || zs < ld * p.M))) return ROLLER_OK;
     p.out_tma |= 1 << i;
-    return box_map(&p.o[i], base, z, ld, zs, as_bf16);
+    return box_map(&p.o[i], base, z, ld, zs, as_bf16, op == kOpDw && i == 2);
   }
   // A matrix that the epilogue reads beside D.
   int input(int i, const void* base, long long z, long long ld, long long zs) {
