@@ -220,7 +220,8 @@ FusedChoice fused_choose(const FusedShape& s, const FusedDevice& d) {
 }
 
 // SMs that the last wave of `before` leaves idle start on kOpDw's tiles that much earlier, and take
-// more of them: as many more as let the busiest worker end first.
+// more of them: as many more as let the busiest worker end first. (Backward of 333 x 768 x 2048: 25.6 us
+// dealt evenly, 23.9 so; 700 x 4096 x 1000: 59.7, 55.8; 1999 x 2048 x 5461 and longer: within 1 %.)
 void fused_deal(const FusedChoice& before, const FusedChoice& dw, const FusedDevice& d, int* head, int* head_tiles) {
   *head = *head_tiles = 0;
   if (dw.split > 1) return;

@@ -47,13 +47,14 @@
 // Measured on B200 (times by events over whole calls, operands beyond L2; shares from counters on
 // 4096 tokens x 2048 x 4096, one launch at a time):
 //   kOpGate, kOpDown   8192 x 4096 x 8192, bf16: 1.19 ms = 1.39 PFLOP/s, what the power limit leaves the
-//                      library's GEMM too. Tensor pipe busy 86 and 81 % of the active cycles, 80 and
-//                      64 % of all (128 tiles of kOpDown on 74 pairs run as two waves).
+//                      library's GEMM too. Tensor pipe busy 85 and 81 % of the active cycles, 79 and
+//                      65 % of all (128 tiles of kOpDown on 74 pairs run as two waves).
 //                      1 x 2048 x 8192: 25 us for 101 MB, 3-5 us of them each kernel's start and end;
 //                      1 x 8192 x 32768: 6.4 TB/s.
-//   kOpDact, kOpDx, kOpDw   8192 x 4096 x 8192, bf16: 2.60 ms together = 1.27 PFLOP/s. Tensor pipe 51,
-//                      90, 89 %: kOpDact moves five matrices beside its product (175 MB of DRAM traffic
-//                      there) and is bound by them.
+//   kOpDact, kOpDx, kOpDw   8192 x 4096 x 8192, bf16: 2.60 ms together = 1.27 PFLOP/s. Tensor pipe 53,
+//                      90, 92 %: kOpDact moves five matrices beside its product (174 MB of DRAM traffic
+//                      there) and is bound by them. 200 x 1024 x 2816: 28.5 us, the latency of three
+//                      launches of which two overlap.
 //   kOpGram*, kOpPoly, kOpUpdate*   8192 x 4096, five steps: 2.18 ms = 1.10 PFLOP/s, triangles counted
 //                      as such; 512 x 512: 5.6 to 6.7 us a product, nearly all of it the way from one
 //                      launch's results to the next one's loads.
