@@ -441,3 +441,28 @@ def test_far_out_activations_stay_finite(act):
         # (u_ on either operand, whichever was rounded)
         bound = sum((e + (2 * u_ + acc(49) + 2.0 ** -20) * p.abs()) @ m.abs() for p, e, m in parts)
         within(got, want, bound + u_ * (want.abs() + bound) + tiny(torch.bfloat16), "gradient")
+
+
+@pytest.mark.parametrize("shape", [(333, 768, 2048), (700, 1024, 1000), (300, 130, 4001), (70, 2050, 700)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weight_gradients_dealt_unevenly(shape, dtype):
+    # the weights' tiles start beside dx's last wave, which leaves part of the SMs to them
+    tokens, d, f = shape
+    s = make(*shape, dtype, seed=22)
+    plan = GatedFfnPlan(tokens, d, f, dtype=dtype, training=True)
+    y, s["g"], s["u"] = run_forward(s, "silu", dtype, plan=plan)
+    first = None
+    for _ in range(3):
+        out = {}
+        bufs = {}
+        for k, v in (("dx", "x"), ("dwg", "wg"), ("dwu", "wu"), ("dwd", "wd")):
+            bufs[k], out[k] = guarded(*s[v].shape, dtype, pad_cols=8 if s[v].shape[1] % 8 == 0 else 3)
+        plan.backward(s["x"], s["wg"], s["wu"], s["wd"], s["g"], s["u"], s["dy"], **out)
+        plan.check_status()
+        assert all(untouched(bufs[k], *out[k].shape) for k in out)
+        if first is None:
+            first = out
+            for name, (want, bound) in backward_bounds(s, "silu", dtype).items():
+                within(out[name], want, bound, name)
+        assert all(torch.equal(first[k], out[k]) for k in out)
+    plan.destroy()
