@@ -156,7 +156,8 @@ __device__ __forceinline__ void activation(float v, float& y, float& slope) {
     const float w = fminf(v * v, 1e30f);     // (an infinite one would meet the slope's zero)
     const float p = sigmoidf_(2.0f * c * v * (1.0f + 0.044715f * w));
     y = v * p;
-    slope = p + 2.0f * c * v * p * (1.0f - p) * (1.0f + 3.0f * 0.044715f * w);
+    // (p (1 - p) before v: it is zero where 2 c v may be infinite)
+    slope = p + 2.0f * c * (v * (p * (1.0f - p))) * (1.0f + 3.0f * 0.044715f * w);
   }
 }
 
