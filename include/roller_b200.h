@@ -329,7 +329,9 @@ int roller_b200_gemm_destroy(roller_plan* plan);
  * outputs x inputs). Sums are kept in fp32. H and the gradients of G and U are rounded to the
  * operand type once, because they are operands of a tensor-core product; Y, G, U and the
  * gradients are rounded once when they are stored. (In fp16, H, dG and dU have fp16's range: over
- * 65504 they become infinite, under 6e-8 zero; gradients want the usual loss scale.) Any d_model, d_ff and tokens are accepted, and any row
+ * 65504 they become infinite, under 6e-8 zero; gradients want the usual loss scale.) Activations keep
+ * their relative accuracy for negative gates too, until act(v) / v falls under 2^-126 and counts as zero
+ * (near v = -87 in silu, -13 in gelu, -10 in gelu_tanh). Any d_model, d_ff and tokens are accepted, and any row
  * stride that is at least the row's length; a product's operand whose base or row stride is not a
  * multiple of 16 bytes is first copied into rows that are. */
 typedef struct roller_ffn_plan roller_ffn_plan;

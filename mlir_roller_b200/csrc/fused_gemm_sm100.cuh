@@ -139,8 +139,9 @@ __device__ __forceinline__ float2 fused_unpack(uint32_t w) {
 
 __device__ __forceinline__ float sigmoidf_(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 
-// act(v) and its slope. tanh appears only as 1 + tanh(z) = 2 sigmoid(2 z): a difference of small
-// numbers never occurs, and the 2^-11 error of the hardware tanh stays out of fp16 results.
+// act(v) and its slope. tanh appears only as 1 + tanh(z) = 2 sigmoid(2 z) and 1 + erf(z) as erfc(-z): a
+// difference of nearly equal numbers never occurs, and the 2^-11 error of the hardware tanh stays out of fp16
+// results. A factor act(v) / v under 2^-126 is zero.
 template <int ACT>
 __device__ __forceinline__ void activation(float v, float& y, float& slope) {
   if constexpr (ACT == kActSilu) {
@@ -148,9 +149,22 @@ __device__ __forceinline__ void activation(float v, float& y, float& slope) {
     y = v * p;
     slope = p * (1.0f + v * (1.0f - p));
   } else if constexpr (ACT == kActGelu) {
-    const float p = 0.5f + 0.5f * erff(v * 0.70710678118654752f);
+    // Phi(-|v|) = e R with e = exp(-v^2 / 2), which the slope needs as well, and R = erfc(|v| / sqrt 2) / (2 e), a
+    // smooth function: a polynomial in t = 1 / (1 + 0.3 |v|), fitted for the least largest relative error
+    // over |v| < 14 (beyond, e is zero): 5e-7 in fp32. 1 - q is never under a half. erfcf in its place: 1.5-8 %
+    // of the whole call (backward of 4096 x 1024 x 4096: 216 -> 234 us).
+    const float t = __fdividef(1.0f, 1.0f + 0.3f * fabsf(v)), e = __expf(-0.5f * v * v);
+    float r = 0.035674773f;
+    r = fmaf(r, t, -0.157203078f);
+    r = fmaf(r, t, 0.206353486f);
+    r = fmaf(r, t, -0.0536836311f);
+    r = fmaf(r, t, 0.128561616f);
+    r = fmaf(r, t, 0.0999134928f);
+    r = fmaf(r, t, 0.120753959f);
+    r = fmaf(r, t, 0.119629301f);
+    const float q = e * (r * t), p = v < 0.0f ? q : 1.0f - q;
     y = v * p;
-    slope = p + v * 0.39894228040143268f * __expf(-0.5f * v * v);
+    slope = p + v * 0.39894228040143268f * e;
   } else {
     constexpr float c = 0.79788456080286536f;
     const float w = fminf(v * v, 1e30f);     // (an infinite one would meet the slope's zero)
