@@ -614,7 +614,7 @@ struct FusedWork {
                 float y, slope;
                 activation<ACT>(element(raw0, j), y, slope);
                 const float dh = __uint_as_float(d[j]), uu = element(raw1, j);
-                v[j] = dh * uu * slope;    // dg
+                v[j] = dh * slope * uu;    // dg (dh uu may overflow where the slope is zero)
                 du[j] = dh * y;
                 h[j] = y * uu;
               }

@@ -89,3 +89,11 @@ def test_negative_gates_keep_their_digits(act, dtype, lowest, dh):
     want = scale * a * g.double()
     # h is rounded to the type before it meets Wd (a power of two)
     block.within(y[0], want, rel * want.abs() + scale * 12 * small, "y")
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_a_closed_gate_passes_nothing_however_large_the_rest(act):
+    """dh u is beyond fp32 here, but the slope it is multiplied by is zero to 1e-80."""
+    g = torch.full((40,), -200.0, device="cuda").bfloat16()
+    dg, du, h = elements(act, g, torch.full_like(g, 1e30), dh=1e20)
+    assert all(bool((t == 0).all()) for t in (dg, du, h))
