@@ -383,7 +383,8 @@ int roller_b200_ffn_forward(roller_ffn_plan* plan, const roller_ffn_io* io, void
 int roller_b200_ffn_backward(roller_ffn_plan* plan, const roller_ffn_io* io, void* stream);
 
 /* Reads and clears the plan's device status word, as roller_b200_last_status does for a GEMM plan
- * (stands in for the per-hint try/except, src/benchmark.py:43-58). Synchronises the device. */
+ * (stands in for the per-hint try/except, src/benchmark.py:43-58). Synchronises the device, which has to be
+ * the plan's (ROLLER_ERR_DEVICE otherwise). */
 int roller_b200_ffn_status(roller_ffn_plan* plan, uint32_t* device_status);
 
 /* Releases the plan and its workspaces (module lifetime in the reference, src/roller.py:504-505). */
@@ -424,7 +425,8 @@ int roller_b200_ortho_run(roller_ortho_plan* plan, const void* g, long long ld_g
                           void* out, long long ld_out, long long zs_out, void* stream);
 
 /* Reads and clears the plan's device status word (stands in for the per-hint try/except,
- * src/benchmark.py:43-58). Synchronises the device. */
+ * src/benchmark.py:43-58). Synchronises the device, which has to be the plan's
+ * (ROLLER_ERR_DEVICE otherwise). */
 int roller_b200_ortho_status(roller_ortho_plan* plan, uint32_t* device_status);
 
 /* Releases the plan and its workspaces (module lifetime in the reference, src/roller.py:504-505). */

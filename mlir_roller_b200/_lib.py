@@ -247,6 +247,18 @@ def on_device(device, stream, fn, *args) -> int:
         return fn(*args, ptr)
 
 
+def check_plan_status(device, fn, handle, name: str) -> None:
+    """Reads a plan's device status word with its device current (that is the one to wait for); raises
+    RollerError(TIMEOUT) when it is set."""
+    import torch
+    st = C.c_uint32()
+    with torch.cuda.device(device):
+        rc = fn(handle, C.byref(st))
+    if rc == ERR_TIMEOUT:
+        raise RollerError(rc, f"device status word = {st.value}")
+    check(rc, name)
+
+
 def gemm_static_scratch(tile: KTile, mode: int, M: int, N: int, K: int, lda: int, ldb: int,
                         ldc: int, a_ptr: int, b_ptr: int, c_ptr: int, status_ptr: int = 0,
                         stream=None) -> None:

@@ -297,6 +297,8 @@ void fused_context_destroy(FusedContext* c) {
 
 int fused_context_status(FusedContext* c, uint32_t* device_status) {
   uint32_t h = 0;
+  int cur = -1;
+  if (cudaGetDevice(&cur) != cudaSuccess || cur != c->device) return ROLLER_ERR_DEVICE;
   FUSED_CUDA(cudaDeviceSynchronize());
   FUSED_CUDA(cudaMemcpy(&h, c->status, sizeof(h), cudaMemcpyDeviceToHost));
   if (device_status) *device_status = h;

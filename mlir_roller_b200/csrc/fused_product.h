@@ -35,7 +35,7 @@ struct FusedContext {
 };
 int fused_context_create(FusedContext* c);    // on the current device; a roller_status
 void fused_context_destroy(FusedContext* c);
-int fused_context_status(FusedContext* c, uint32_t* device_status);   // reads and clears
+int fused_context_status(FusedContext* c, uint32_t* device_status);   // reads and clears; on its device
 
 // One allocation for all workspaces of a plan: sizes are asked for first, pointers given afterwards
 // (each on a 1024-byte boundary).

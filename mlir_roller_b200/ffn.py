@@ -126,12 +126,8 @@ class GatedFfnPlan:
 
     def check_status(self) -> None:
         """Raises RollerError(TIMEOUT) if a launch since the last check gave up on a device-side
-        wait. Synchronises the device."""
-        st = C.c_uint32()
-        rc = self._lib.roller_b200_ffn_status(self._h, C.byref(st))
-        if rc == _lib.ERR_TIMEOUT:
-            raise _lib.RollerError(rc, f"device status word = {st.value}")
-        _lib.check(rc, "roller_b200_ffn_status")
+        wait. Synchronises the plan's device."""
+        _lib.check_plan_status(self.device, self._lib.roller_b200_ffn_status, self._h, "roller_b200_ffn_status")
 
     def destroy(self) -> None:
         if self._h:

@@ -104,3 +104,44 @@ def test_sizes_beyond_a_c_int_are_refused():
         with pytest.raises(_lib.RollerError) as e:
             make()
         assert e.value.status == _lib.ERR_INVALID
+
+
+@pytest.mark.parametrize("kind", ["block", "update"])
+def test_status_is_read_on_the_plan_s_own_device(monkeypatch, kind):
+    """Two devices, in imitation: a plan of the second one, asked while the first one is current."""
+    from contextlib import contextmanager
+
+    from mlir_roller_b200 import GatedFfnPlan, OrthogonalPlan
+    current = [0]
+
+    @contextmanager
+    def device(d):
+        before, current[0] = current[0], torch.device(d).index
+        yield
+        current[0] = before
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    seen = []
+
+    class Library:
+        def status(self, handle, word):
+            seen.append(current[0])
+            word._obj.value = 6
+            return _lib.ERR_TIMEOUT
+
+        roller_b200_ffn_status = roller_b200_ortho_status = status
+
+        def destroy(self, handle):
+            return _lib.OK
+
+        roller_b200_ffn_destroy = roller_b200_ortho_destroy = destroy
+
+    cls = GatedFfnPlan if kind == "block" else OrthogonalPlan
+    plan = cls.__new__(cls)
+    plan._lib, plan._h, plan.device = Library(), C.c_void_p(1), torch.device("cuda", 1)
+    with pytest.raises(_lib.RollerError, match="= 6") as e:
+        plan.check_status()
+    assert e.value.status == _lib.ERR_TIMEOUT
+    assert seen == [1] and current == [0]
+    plan.destroy()
