@@ -558,6 +558,7 @@ struct FusedWork {
             if (r0 + k < rows) dst[(r0 + k) * p.out_ld[0] + h * 32] = w[k];
         }
       }
+      fence_proxy_async_smem();      // (the TMA unit writes the next inputs over what was put here)
       __syncwarp();
     };
 
