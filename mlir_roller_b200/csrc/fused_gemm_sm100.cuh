@@ -529,8 +529,6 @@ struct FusedWork {
     };
     // the first n boxes to outputs 0 .. n - 1, through the TMA unit
     auto hand_over = [&](int n, const FusedTile& c, int row0, int col) {
-      fence_proxy_async_smem();
-      __syncwarp();
       if (me.lane == 0) {
         if (row0 < p.M)
           for (int o = 0; o < n; ++o) tma_store_3d(&p.o[o], in_boxes + o * Cfg::BOX_BYTES, col, row0, c.z);
@@ -539,7 +537,6 @@ struct FusedWork {
     };
     // box 0 to rows that start anywhere: a warp writes 32 consecutive elements per instruction
     auto store_unaligned = [&](const FusedTile& c, int row0, int col) {
-      __syncwarp();
       uint16_t* dst = static_cast<uint16_t*>(p.out[0]) + c.z * p.out_zstride + static_cast<long long>(row0) * p.out_ld[0] + col + me.lane;
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
@@ -558,7 +555,6 @@ struct FusedWork {
             if (r0 + k < rows) dst[(r0 + k) * p.out_ld[0] + h * 32] = w[k];
         }
       }
-      fence_proxy_async_smem();      // (the TMA unit writes the next inputs over what was put here)
       __syncwarp();
     };
 
@@ -646,6 +642,10 @@ struct FusedWork {
               }
             }
           }
+          // what was put into the boxes comes before the TMA unit's next access, be it the store that reads
+          // them or, behind ordinary stores, the next inputs that overwrite them
+          fence_proxy_async_smem();
+          __syncwarp();
           if (OP == kOpDact) hand_over(3, c, row0, col);
           else if (!(p.flags & kFusedLast)) hand_over(2, c, row0, col);
           else if (p.out_tma & 1) hand_over(1, c, row0, col);
