@@ -43,8 +43,9 @@ double epilogue_weight(int op) {
 
 // Copies the jobs' 16-bit rows into rows that start on 16 bytes. A warp takes 256 words (of two
 // elements) of a row at a time, a thread eight of them, all on their way together: a source row
-// that starts between two words gives each word from two neighbouring ones. (A word that holds an
-// element of the row may be read whole.)
+// that starts between two words gives each word from two neighbouring ones, the second of which the
+// next lane has. (A word that holds an element of the row may be read whole. Ordinary loads, not those of
+// constant data: the kernel before may still be writing an operand when this one starts.)
 // A 2048 x 5461 weight costs a forward call 5 us (45 MB, overlapped with the first product's end).
 // jobs.late: as FusedParams::late_wait, the copies need nothing from the previous kernel.
 __global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__ AlignJobs jobs) {
@@ -62,16 +63,17 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__
     const uint32_t* src = reinterpret_cast<const uint32_t*>(at & ~static_cast<uintptr_t>(3));
     uint32_t* dst = reinterpret_cast<uint32_t*>(j.dst + row * j.ld_dst);
     const bool between = (at & 2) != 0;
-    uint32_t x[8], y[8];
+    const int sources = (j.cols + (between ? 2 : 1)) / 2;
+    uint32_t x[9];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = w0 + 32 * k < sources ? src[w0 + 32 * k] : 0u;
+    x[8] = between && lane == 31 && w0 + 225 < sources ? src[w0 + 225] : 0u;   // (only lane 31's neighbour)
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int w = w0 + 32 * k;
-      x[k] = w < words ? __ldg(src + w) : 0u;
-      y[k] = between && 2 * w + 1 < j.cols ? __ldg(src + w + 1) : 0u;
+      uint32_t next = __shfl_sync(0xffffffffu, lane == 0 ? x[k + 1] : x[k], (lane + 1) & 31);
+      if (k == 7 && lane == 31) next = x[8];
+      if (w0 + 32 * k < words) dst[w0 + 32 * k] = between ? __byte_perm(x[k], next, 0x5432) : x[k];
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (w0 + 32 * k < words) dst[w0 + 32 * k] = between ? __byte_perm(x[k], y[k], 0x5432) : x[k];
   }
   if (jobs.late) grid_dependency_wait();
 }

@@ -40,14 +40,15 @@ __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { retu
 template <>
 __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
 
-// Eight consecutive elements of a row (those beyond the row's end are zero).
+// Eight consecutive elements of a row (those beyond the row's end are zero). Ordinary loads, not those of
+// constant data (ld.global.nc): the kernel before may still be writing them when this one starts.
 template <typename T>
 __device__ __forceinline__ void load8(const T* row, int col, int cols, bool vec, float (&v)[8]) {
   if (vec && col + 8 <= cols) {
     alignas(16) T t[8];
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-      reinterpret_cast<uint4*>(t)[i] = __ldg(reinterpret_cast<const uint4*>(row + col) + i);
+      reinterpret_cast<uint4*>(t)[i] = reinterpret_cast<const uint4*>(row + col)[i];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = to_float(t[j]);
   } else {
@@ -149,27 +150,32 @@ __global__ void __launch_bounds__(256) ortho_sumsq(Source s, double* __restrict_
 // reading g twice take (403 MB, a part of the second time from L2).
 template <typename T>
 __global__ void __launch_bounds__(256)
-ortho_scale(Source s, const double* __restrict__ part, int parts, double eps, __half* __restrict__ hi,
+ortho_scale(Source s, const double* part, int parts, double eps, __half* __restrict__ hi,
             __half* __restrict__ lo, long long ldx, long long zsx) {
   grid_dependency_wait();
   grid_launch_dependents();
+  const T* g = static_cast<const T*>(s.g) + blockIdx.y * s.zs;
+  const uint32_t rows = static_cast<uint32_t>(s.rows);
+  Walk w(s.per_row);
+  Walk back = w;
+  float v[kGroupsAtOnce][8];
+  auto load = [&]() {
+    back = w;
+#pragma unroll
+    for (int i = 0; i < kGroupsAtOnce; ++i, w.step())
+      if (w.r < rows) load8(g + w.r * s.ld, static_cast<int>(w.c) * 8, s.cols, s.vec, v[i]);
+  };
+  load();      // on their way while the norm is put together
+
   double sum = 0.0;
-  for (int i = threadIdx.x; i < parts; i += 256) sum += part[blockIdx.y * kSumBlocks + i];
+  for (int i = threadIdx.x; i < parts; i += 256) sum += __ldcg(part + blockIdx.y * kSumBlocks + i);
   sum = block_sum(sum);
   const double norm = sqrt(sum) + eps;
   const int e = ((__double2hiint(norm) >> 20) & 0x7FF) - 1023;
   const float near_one = __uint_as_float(static_cast<uint32_t>(127 - max(-100, min(100, e))) << 23);
   const float scale = static_cast<float>(static_cast<double>(kScale) / (norm * near_one));
 
-  const T* g = static_cast<const T*>(s.g) + blockIdx.y * s.zs;
-  const uint32_t rows = static_cast<uint32_t>(s.rows);
-  Walk w(s.per_row);
-  while (w.r < rows) {
-    float v[kGroupsAtOnce][8];
-    Walk back = w;
-#pragma unroll
-    for (int i = 0; i < kGroupsAtOnce; ++i, w.step())
-      if (w.r < rows) load8(g + w.r * s.ld, static_cast<int>(w.c) * 8, s.cols, s.vec, v[i]);
+  while (back.r < rows) {
 #pragma unroll
     for (int i = 0; i < kGroupsAtOnce; ++i, back.step()) {
       if (back.r >= rows) break;
@@ -184,6 +190,7 @@ ortho_scale(Source s, const double* __restrict__ part, int parts, double eps, __
       *reinterpret_cast<uint4*>(hi + at) = *reinterpret_cast<const uint4*>(h);
       *reinterpret_cast<uint4*>(lo + at) = *reinterpret_cast<const uint4*>(l);
     }
+    load();
   }
 }
 

@@ -52,3 +52,29 @@ def test_a_new_plan_is_ready_for_any_stream(kind):
     assert torch.equal(out.view(torch.int16), want.view(torch.int16))
     plan.check_status()
     plan.destroy()
+
+
+@pytest.mark.parametrize("d", [1, 2, 63, 510, 511, 512, 513, 514, 1025])
+def test_rows_that_start_anywhere(d):
+    """Copies of unaligned rows, around the 512 elements that a warp moves at a time: from every offset the
+    same bits as from aligned rows, and nothing beside a row counts (it is NaN here)."""
+    tokens, f = 37, 72
+    s = block.make(tokens, d, f, torch.bfloat16, seed=71)
+    plan = GatedFfnPlan(tokens, d, f)
+
+    def view(t, lead, ld):
+        buf = torch.full((t.shape[0], ld), float("nan"), dtype=t.dtype, device="cuda")
+        v = buf[:, lead:lead + t.shape[1]]
+        v.copy_(t)
+        return v
+
+    y, again = (torch.empty(tokens, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    aligned = (d + 7) // 8 * 8
+    plan.forward(*(view(s[k], 0, aligned) for k in ("x", "wg", "wu")), s["wd"], y)
+    for lead in range(8):
+        for more in (0, 1, 5):
+            plan.forward(*(view(s[k], lead, aligned + lead + more) for k in ("x", "wg", "wu")), s["wd"], again.zero_())
+            assert torch.equal(again, y), (lead, more)
+    plan.check_status()
+    plan.destroy()
+    assert bool(y.isfinite().all())
