@@ -7,7 +7,7 @@
 //              kOpDx:    dx = dg Wg + du Wu, one reduction over both
 //              kOpDw:    dWg = dg^T x, dWu = du^T x and dWd = dy^T h in one launch: tiles of equal length
 //              The last two launches need only what kOpDact wrote, so they overlap
-//              (FusedParams::late_wait); kOpDx goes first, because its few long tiles leave SMs free.
+//              (FusedParams::late_wait, LaunchOrder); kOpDx goes first, because its few long tiles leave SMs free.
 #include <cstring>
 #include <new>
 
@@ -178,12 +178,13 @@ int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* s
   // Copies of unaligned operands: those of the first product before it, the others behind it, where
   // they run on the SMs that its last wave leaves idle.
   AlignJobs jobs, later;
+  LaunchOrder order;
   later.late = 1;
   FUSED_OK(usable(p, kX, io->x, T, st, &jobs, &x, &ldx));
   FUSED_OK(usable(p, kWg, io->wg, F, st, &jobs, &wg, &ldg));
   FUSED_OK(usable(p, kWu, io->wu, F, st, &jobs, &wu, &ldu));
   FUSED_OK(usable(p, kWd, io->wd, D, st, &later, &wd, &ldd));
-  FUSED_CUDA(align_rows(jobs, p->ctx.dev.sm_count, st));
+  FUSED_CUDA(align_rows(jobs, order, p->ctx.dev.sm_count, st));
   {
     Product g(p->ctx, kOpGate, p->dt, T, F, D, 1, &choice[kPGate]);
     g.p.act = p->act;
@@ -196,15 +197,15 @@ int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* s
       FUSED_OK(g.output(2, io->u.ptr, 1, io->u.ld, 0, bf16));
       g.p.flags |= kFusedSave;
     }
-    FUSED_OK(g.launch(st));
+    FUSED_OK(g.launch(order, st));
   }
-  FUSED_CUDA(align_rows(later, p->ctx.dev.sm_count, st));
+  FUSED_CUDA(align_rows(later, order, p->ctx.dev.sm_count, st));
   Product d(p->ctx, kOpDown, p->dt, T, D, F, 1, &choice[kPDown]);
-  d.p.b_early = later.n == 0;   // Wd does not come from the gate kernel
+  d.p.b_early = later.n == 0;   // Wd comes neither from the gate kernel nor from a copy
   FUSED_OK(d.a_k(p->h, F, T, 1, p->ldf, 0));
   FUSED_OK(d.b_k(0, wd, F, D, 1, ldd, 0));
   FUSED_OK(d.output(0, io->y.ptr, 1, io->y.ld, 0, bf16));
-  return d.launch(st);
+  return d.launch(order, st);
 }
 
 int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* stream) {
@@ -234,6 +235,7 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
   // Copies of unaligned operands: those of the first product before it, the others behind it, where
   // they run on the SMs that its last wave leaves idle.
   AlignJobs jobs, later;
+  LaunchOrder order;
   later.late = 1;
   FUSED_OK(usable(p, kX, io->x, T, st, &later, &x, &ldx));
   FUSED_OK(usable(p, kWg, io->wg, F, st, &later, &wg, &ldg));
@@ -242,7 +244,7 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
   FUSED_OK(usable(p, kDy, io->dy, T, st, &jobs, &dy, &ldy));
   FUSED_OK(usable(p, kG, io->g, T, st, &jobs, &g, &ldsg));
   FUSED_OK(usable(p, kU, io->u, T, st, &jobs, &u, &ldsu));
-  FUSED_CUDA(align_rows(jobs, p->ctx.dev.sm_count, st));
+  FUSED_CUDA(align_rows(jobs, order, p->ctx.dev.sm_count, st));
   const long long zs = static_cast<long long>(p->max_tokens) * p->ldf;   // dg to du
   {
     Product a(p->ctx, kOpDact, p->dt, T, F, D, 1, &choice[kPDact]);
@@ -254,17 +256,17 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     FUSED_OK(a.output(2, p->h, 1, p->ldf, 0, bf16));
     FUSED_OK(a.input(0, g, 1, ldsg, 0));
     FUSED_OK(a.input(1, u, 1, ldsu, 0));
-    FUSED_OK(a.launch(st));
+    FUSED_OK(a.launch(order, st));
   }
-  FUSED_CUDA(align_rows(later, p->ctx.dev.sm_count, st));
+  FUSED_CUDA(align_rows(later, order, p->ctx.dev.sm_count, st));
   {
     Product r(p->ctx, kOpDx, p->dt, T, D, F, 1, &choice[kPDx]);
-    r.p.b_early = later.n == 0;   // Wg and Wu do not come from the kernel above
+    r.p.b_early = later.n == 0;   // Wg and Wu come neither from the kernel above nor from a copy
     FUSED_OK(r.a_k(p->dgu, F, T, 2, p->ldf, zs));
     FUSED_OK(r.b_mn(0, wg, D, F, 1, ldg, 0));
     FUSED_OK(r.b_mn(1, wu, D, F, 1, ldu, 0));
     FUSED_OK(r.output(0, io->dx.ptr, 1, io->dx.ld, 0, bf16));
-    FUSED_OK(r.launch(st));
+    FUSED_OK(r.launch(order, st));
   }
   Product w(p->ctx, kOpDw, p->dt, F, D, T, 2, &choice[kPDw]);
   w.p.late_wait = 1;   // dg, du and h were complete before the kernel above started
@@ -276,7 +278,7 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
   FUSED_OK(w.a2_mn(dy, D, T, ldy));
   FUSED_OK(w.b_mn(1, p->h, F, T, 1, p->ldf, 0));
   FUSED_OK(w.output(2, io->dwd.ptr, 1, io->dwd.ld, 0, bf16));
-  return w.launch(st);
+  return w.launch(order, st);
 }
 
 int roller_b200_ffn_status(roller_ffn_plan* p, uint32_t* device_status) {

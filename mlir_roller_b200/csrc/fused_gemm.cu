@@ -80,8 +80,9 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__
 
 }  // namespace
 
-cudaError_t align_rows(AlignJobs& jobs, int sm_count, cudaStream_t stream) {
+cudaError_t align_rows(AlignJobs& jobs, LaunchOrder& order, int sm_count, cudaStream_t stream) {
   if (jobs.n == 0) return cudaSuccess;
+  order.next(nullptr, &jobs.late);
   // blocks in proportion to the jobs' sizes, eight per SM in all
   double total = 0.0;
   for (int i = 0; i < jobs.n; ++i) total += static_cast<double>(jobs.job[i].rows) * jobs.job[i].cols;

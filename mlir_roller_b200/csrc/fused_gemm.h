@@ -54,6 +54,22 @@ struct FusedParams {
   long long spin_limit;
 };
 
+// What a launch may take for granted about the launches before it in its call. `waited`: the last one let
+// its successor start only after its own wait, so that everything before it is complete by then. Only then may
+// the next one read operands early (b_early) or wait late (late_wait, AlignJobs::late); it says so here, and
+// one that waits late itself, or a launch of somebody else (the start of a call), gives nothing for granted.
+struct LaunchOrder {
+  bool waited = false;
+  // The liberties that the next launch wants, as far as it may take them.
+  void next(int* b_early, int* late_wait) {
+    if (!waited) {
+      if (b_early) *b_early = 0;
+      *late_wait = 0;
+    }
+    waited = *late_wait == 0;
+  }
+};
+
 struct FusedVariant {
   int op, cta_group, block_n, dt;   // dt: 1 = bf16, 2 = fp16
   int threads, smem_bytes, max_split;

@@ -34,15 +34,16 @@
 // every access of a warp touches 32 lines.
 //
 // A launch may be scheduled while the previous one of its stream still runs (programmatic
-// dependent launch). It touches memory only behind griddepcontrol.wait, with two exceptions, both
-// resting on this: a kernel here lets its successor start only after its own wait has returned,
-// so when the successor starts, everything before its predecessor is complete.
-//   * p.b_early: weights may be fetched before the wait, when the previous kernel is one of these
-//     and does not write them;
+// dependent launch). It touches memory only behind griddepcontrol.wait, with two exceptions:
+//   * p.b_early: weights that the previous kernel does not write may be fetched before the wait;
 //   * p.late_wait: a kernel that needs nothing from its predecessor (and writes nothing that one
 //     touches) waits for it only before it ends, so that its CTAs fill the SMs that the
 //     predecessor's last wave leaves idle. It ends after its predecessor, so what follows
 //     in the stream still finds both complete.
+// Both read what kernels before the predecessor wrote, and need these complete when they start. That holds
+// if the predecessor let its successor start only after its own wait had returned, as a launch without
+// late_wait does. It does not hold behind one with late_wait, behind late copies (AlignJobs::late), or
+// behind a launch that is not of this call; there the two flags are taken back (LaunchOrder).
 //
 // Measured on B200 (times by events over whole calls, operands beyond L2; shares from counters on
 // 4096 tokens x 2048 x 4096, one launch at a time):

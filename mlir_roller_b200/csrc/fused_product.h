@@ -63,9 +63,9 @@ struct AlignJob {
 struct AlignJobs {
   AlignJob job[8];
   int n = 0;
-  int late = 0;     // the previous kernel of the stream is one of these and has nothing to do with them
+  int late = 0;     // the previous kernel of the call has nothing to do with them (taken back if LaunchOrder says so)
 };
-cudaError_t align_rows(AlignJobs& jobs, int sm_count, cudaStream_t stream);
+cudaError_t align_rows(AlignJobs& jobs, LaunchOrder& order, int sm_count, cudaStream_t stream);
 
 // D is M x N, reduced over K, for z matrices; operand matrices are [z][rows][cols] in memory.
 struct Product {
@@ -143,6 +143,10 @@ struct Product {
   int launch(cudaStream_t st) {
     FUSED_CUDA(c.kv->launch(p, c.grid, st));
     return ROLLER_OK;
+  }
+  int launch(LaunchOrder& order, cudaStream_t st) {
+    order.next(&p.b_early, &p.late_wait);
+    return launch(st);
   }
 };
 
