@@ -191,10 +191,10 @@ int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* s
     FUSED_OK(g.a_k(x, D, T, 1, ldx, 0));
     FUSED_OK(g.b_k(0, wg, D, F, 1, ldg, 0));
     FUSED_OK(g.b_k(1, wu, D, F, 1, ldu, 0));
-    FUSED_OK(g.output(0, p->h, 1, p->ldf, 0, bf16));
+    FUSED_OK(g.output(0, p->h, 1, p->ldf, 0, bf16, true));
     if (save) {
-      FUSED_OK(g.output(1, io->g.ptr, 1, io->g.ld, 0, bf16));
-      FUSED_OK(g.output(2, io->u.ptr, 1, io->u.ld, 0, bf16));
+      FUSED_OK(g.output(1, io->g.ptr, 1, io->g.ld, 0, bf16, false));
+      FUSED_OK(g.output(2, io->u.ptr, 1, io->u.ld, 0, bf16, false));
       g.p.flags |= kFusedSave;
     }
     FUSED_OK(g.launch(order, st));
@@ -204,7 +204,7 @@ int roller_b200_ffn_forward(roller_ffn_plan* p, const roller_ffn_io* io, void* s
   d.p.b_early = later.n == 0;   // Wd comes neither from the gate kernel nor from a copy
   FUSED_OK(d.a_k(p->h, F, T, 1, p->ldf, 0));
   FUSED_OK(d.b_k(0, wd, F, D, 1, ldd, 0));
-  FUSED_OK(d.output(0, io->y.ptr, 1, io->y.ld, 0, bf16));
+  FUSED_OK(d.output(0, io->y.ptr, 1, io->y.ld, 0, bf16, false));
   return d.launch(order, st);
 }
 
@@ -251,9 +251,9 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     a.p.act = p->act;
     FUSED_OK(a.a_k(dy, D, T, 1, ldy, 0));
     FUSED_OK(a.b_mn(0, wd, F, D, 1, ldd, 0));
-    FUSED_OK(a.output(0, p->dgu, 1, p->ldf, 0, bf16));
-    FUSED_OK(a.output(1, static_cast<uint16_t*>(p->dgu) + zs, 1, p->ldf, 0, bf16));
-    FUSED_OK(a.output(2, p->h, 1, p->ldf, 0, bf16));
+    FUSED_OK(a.output(0, p->dgu, 1, p->ldf, 0, bf16, true));
+    FUSED_OK(a.output(1, static_cast<uint16_t*>(p->dgu) + zs, 1, p->ldf, 0, bf16, true));
+    FUSED_OK(a.output(2, p->h, 1, p->ldf, 0, bf16, true));
     FUSED_OK(a.input(0, g, 1, ldsg, 0));
     FUSED_OK(a.input(1, u, 1, ldsu, 0));
     FUSED_OK(a.launch(order, st));
@@ -265,7 +265,7 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
     FUSED_OK(r.a_k(p->dgu, F, T, 2, p->ldf, zs));
     FUSED_OK(r.b_mn(0, wg, D, F, 1, ldg, 0));
     FUSED_OK(r.b_mn(1, wu, D, F, 1, ldu, 0));
-    FUSED_OK(r.output(0, io->dx.ptr, 1, io->dx.ld, 0, bf16));
+    FUSED_OK(r.output(0, io->dx.ptr, 1, io->dx.ld, 0, bf16, false));
     FUSED_OK(r.launch(order, st));
   }
   Product w(p->ctx, kOpDw, p->dt, F, D, T, 2, &choice[kPDw]);
@@ -273,11 +273,11 @@ int roller_b200_ffn_backward(roller_ffn_plan* p, const roller_ffn_io* io, void* 
   fused_deal(choice[kPDx], choice[kPDw], p->ctx.dev, &w.p.head, &w.p.head_tiles);
   FUSED_OK(w.a_mn(p->dgu, F, T, 2, p->ldf, zs));
   FUSED_OK(w.b_mn(0, x, D, T, 1, ldx, 0));
-  FUSED_OK(w.output(0, io->dwg.ptr, 1, io->dwg.ld, 0, bf16));
-  FUSED_OK(w.output(1, io->dwu.ptr, 1, io->dwu.ld, 0, bf16));
+  FUSED_OK(w.output(0, io->dwg.ptr, 1, io->dwg.ld, 0, bf16, false));
+  FUSED_OK(w.output(1, io->dwu.ptr, 1, io->dwu.ld, 0, bf16, false));
   FUSED_OK(w.a2_mn(dy, D, T, ldy));
   FUSED_OK(w.b_mn(1, p->h, F, T, 1, p->ldf, 0));
-  FUSED_OK(w.output(2, io->dwd.ptr, 1, io->dwd.ld, 0, bf16));
+  FUSED_OK(w.output(2, io->dwd.ptr, 1, io->dwd.ld, 0, bf16, false));
   return w.launch(order, st);
 }
 

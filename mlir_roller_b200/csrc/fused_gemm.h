@@ -35,6 +35,9 @@ struct FusedParams {
   long long out_zstride;
   int out_cols;         // columns of the outputs (those beyond are not written)
   int out_tma;          // bit o: output o leaves through o[o] (16-byte aligned base and rows)
+  int out_whole;        // bit o: and so do boxes that reach beyond the last column. A TMA store drops what lies
+                        // there in units of 16 bytes only: up to 7 columns behind the last one are written, which
+                        // must be none (a width of whole units) or the library's own padding.
   CUtensorMap i[2];     // element-wise inputs of the epilogue
   float* vec;           // kOpPoly writes, kOpUpdate* reads: one value per row of q, [z][vec_ld]
   int vec_ld;

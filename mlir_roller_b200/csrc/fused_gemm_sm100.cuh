@@ -536,7 +536,7 @@ struct FusedWork {
         bulk_commit_group();
       }
     };
-    // box 0 to rows that start anywhere: a warp writes 32 consecutive elements per instruction
+    // box 0 to rows that start or end anywhere: a warp writes 32 consecutive elements per instruction
     auto store_unaligned = [&](const FusedTile& c, int row0, int col) {
       uint16_t* dst = static_cast<uint16_t*>(p.out[0]) + c.z * p.out_zstride + static_cast<long long>(row0) * p.out_ld[0] + col + me.lane;
 #pragma unroll 1
@@ -649,7 +649,7 @@ struct FusedWork {
           __syncwarp();
           if (OP == kOpDact) hand_over(3, c, row0, col);
           else if (!(p.flags & kFusedLast)) hand_over(2, c, row0, col);
-          else if (p.out_tma & 1) hand_over(1, c, row0, col);
+          else if ((p.out_tma & 1) && (col + 64 <= p.out_cols || (p.out_whole & 1))) hand_over(1, c, row0, col);
           else store_unaligned(c, row0, col);
         }
       };
@@ -730,7 +730,7 @@ struct FusedWork {
       const uint32_t box = free_box();
       put(box, v, as_bf16);
       const int oz = OP == kOpDw ? 0 : c.z;
-      if (p.out_tma & (1 << o)) {
+      if (((col + 32 <= cols(c) ? p.out_tma : p.out_whole) >> o) & 1) {
         fence_proxy_async_smem();
         __syncwarp();
         if (me.lane == 0) {
@@ -738,7 +738,7 @@ struct FusedWork {
           bulk_commit_group();
         }
       } else {
-        // rows that start anywhere: a warp writes 32 consecutive elements per instruction
+        // rows that start or end anywhere: a warp writes 32 consecutive elements per instruction
         __syncwarp();
         uint16_t* dst = static_cast<uint16_t*>(p.out[o]) + oz * p.out_zstride + static_cast<long long>(row0) * p.out_ld[o] + col + me.lane;
         const int left = col + me.lane < cols(c) ? rows(c) - row0 : 0;

@@ -124,13 +124,16 @@ struct Product {
     return encode_batch16(map, base, second ? p.out_cols2 : p.out_cols, second ? p.M2 : p.M, z, ld, zs, wide ? 64 : 32, 32,
                           wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, as_bf16);
   }
-  int output(int i, void* base, long long z, long long ld, long long zs, bool as_bf16) {
+  // padded: the rows are the library's own and have room up to the next 16 bytes.
+  int output(int i, void* base, long long z, long long ld, long long zs, bool as_bf16, bool padded) {
+    const bool second = op == kOpDw && i == 2;
     p.out[i] = base;
     p.out_ld[i] = ld;
     p.out_zstride = zs;
     if (!aligned16(base, ld) || (z > 1 && (zs % 8 != 0 || zs < ld * p.M))) return ROLLER_OK;
     p.out_tma |= 1 << i;
-    return box_map(&p.o[i], base, z, ld, zs, as_bf16, op == kOpDw && i == 2);
+    if (padded || (second ? p.out_cols2 : p.out_cols) % 8 == 0) p.out_whole |= 1 << i;
+    return box_map(&p.o[i], base, z, ld, zs, as_bf16, second);
   }
   // A matrix that the epilogue reads beside D.
   int input(int i, const void* base, long long z, long long ld, long long zs) {

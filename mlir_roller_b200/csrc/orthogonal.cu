@@ -264,7 +264,7 @@ int build_products(roller_ortho_plan* p) {
       FUSED_OK(g.a_k(hi, C, R, Z, p->ldx, p->zsx));
       FUSED_OK(g.b_k(0, hi, C, R, Z, p->ldx, p->zsx));
     }
-    FUSED_OK(g.output(0, p->pm, Z, p->ldm, p->zsm, false));
+    FUSED_OK(g.output(0, p->pm, Z, p->ldm, p->zsm, false, true));
     FUSED_OK(g.mirror(p->pm, Z, p->ldm, p->zsm));
     g.p.inv_scale = 1.0f / kScale;
     for (int final_step = 0; final_step < 2; ++final_step) {
@@ -287,8 +287,8 @@ int build_products(roller_ortho_plan* p) {
       if (final_step) {
         u.p.flags |= kFusedLast;      // (its output is set by each call)
       } else {
-        FUSED_OK(u.output(0, p->x[1 - w][0], Z, p->ldx, p->zsx, false));
-        FUSED_OK(u.output(1, p->x[1 - w][1], Z, p->ldx, p->zsx, false));
+        FUSED_OK(u.output(0, p->x[1 - w][0], Z, p->ldx, p->zsx, false, true));
+        FUSED_OK(u.output(1, p->x[1 - w][1], Z, p->ldx, p->zsx, false, true));
       }
     }
   }
@@ -298,7 +298,7 @@ int build_products(roller_ortho_plan* p) {
   FUSED_OK(q.a_k(p->pm, m, m, Z, p->ldm, p->zsm));
   FUSED_OK(q.b_k(0, p->pm, m, m, Z, p->ldm, p->zsm));
   FUSED_OK(q.input(0, p->pm, Z, p->ldm, p->zsm));
-  FUSED_OK(q.output(0, p->qm, Z, p->ldm, p->zsm, false));
+  FUSED_OK(q.output(0, p->qm, Z, p->ldm, p->zsm, false, true));
   FUSED_OK(q.mirror(p->qm, Z, p->ldm, p->zsm));
   q.p.vec = p->vec;
   q.p.vec_ld = static_cast<int>(p->ldm);
@@ -426,7 +426,7 @@ int roller_b200_ortho_run(roller_ortho_plan* p, const void* g, long long ld_g, l
       continue;
     }
     Product u = *p->last[w];
-    FUSED_OK(u.output(0, out, p->batch, ld_out, zs_out, true));
+    FUSED_OK(u.output(0, out, p->batch, ld_out, zs_out, true, false));
     FUSED_OK(u.launch(st));
   }
   return ROLLER_OK;
