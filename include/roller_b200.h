@@ -81,7 +81,8 @@ typedef enum roller_status {
                                           destination (C in another GPU's memory, mapped into
                                           this process) does not hold the warps up. The library
                                           uses this path by itself where it can: fp32 C with
-                                          16-byte aligned base and row stride, no
+                                          16-byte aligned base and row stride, rows that
+                                          are a multiple of 16 bytes long (N % 4 == 0), no
                                           ROLLER_FLAG_ACCUMULATE, an rTile whose kernel has the
                                           staging area. 1 insists on it (ROLLER_ERR_UNSUPPORTED /
                                           _INVALID where it cannot work); 0 turns it off */

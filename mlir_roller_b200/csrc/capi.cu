@@ -392,9 +392,11 @@ int roller_b200_gemm_create(const roller_ktile* tile, int M, int N, int K, int l
   p->stage_a = layout != 3 && (static_cast<long long>(lda) * elem % 16) != 0;
   p->stage_b = layout != 3 && (static_cast<long long>(ldb) * elem % 16) != 0;
 
-  // Whether C can leave through TMA stores at all (the base address is checked per launch).
+  // Whether C can leave through TMA stores at all (the base address is checked per launch). The
+  // unit drops what lies beyond a row's end in steps of 16 bytes only, so a row has to be a
+  // multiple of that long too: up to three columns behind it would be overwritten.
   const bool c_fits_tma = layout != 2 && p->c_elem == 4 && !(flags & ROLLER_FLAG_ACCUMULATE) &&
-                          ldc % 4 == 0;
+                          ldc % 4 == 0 && N % 4 == 0;
   // A kernel whose ring fills shared memory also exists with one stage less and the staging
   // area of that path; for the pair tile that form is the faster one up to K = 4096 (see
   // GemmCfg; the single-CTA 128 x 128 tile gains nothing from it and switches only on request).
@@ -745,7 +747,8 @@ int roller_b200_gemm_set_option(roller_plan* p, int option, long long value) {
       if (value != 0) {
         if (p->layout == 2 || p->c_elem != 4 || (p->flags & ROLLER_FLAG_ACCUMULATE))
           return ROLLER_ERR_UNSUPPORTED;
-        if (p->ldc % 4 != 0) return ROLLER_ERR_INVALID;   // TMA needs 16-byte row strides
+        // TMA needs 16-byte row strides, and row lengths (see c_fits_tma)
+        if (p->ldc % 4 != 0 || p->N % 4 != 0) return ROLLER_ERR_INVALID;
         if (p->kv->staging_bytes == 0) {
           // the form of the kernel with a shorter ring has the staging area
           const KernelVariant* staged = find_staged_form(p->kv);

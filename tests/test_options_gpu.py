@@ -477,3 +477,35 @@ def test_early_exit_leaves_the_result_alone():
     plan.check_status()
     assert int(flags[0].item()) == 7 and np.array_equal(dC.cpu().numpy(), ref)
     plan.destroy()
+
+
+@pytest.mark.parametrize("mode", [1, 3, _lib.MODE_BF16])
+@pytest.mark.parametrize("N", [1, 6, 130, 517])
+def test_aligned_rows_of_any_length_end_where_they_should(mode, N):
+    """A C with rows on 16 bytes that are no multiple of 16 bytes long: the columns behind them stay as they
+    were with every rTile, and insisting on TMA stores, which cannot keep to that, is refused."""
+    M, K, ldc = 300, 96, (N + 7) // 4 * 4
+    gen = torch.Generator(device="cuda").manual_seed(N)
+    dt = torch.bfloat16 if mode == _lib.MODE_BF16 else torch.float32
+    A, B = (torch.rand(*s, device="cuda", generator=gen).to(dt) for s in ((M, K), (K, N)))
+    want = A.double() @ B.double()
+    ran = 0
+    for tile in _lib.kernel_tiles():
+        try:
+            plan = _lib.GemmPlan(tile, M, N, K, ldc=ldc, mode=mode)
+        except _lib.RollerError as e:
+            assert e.status == _lib.ERR_UNSUPPORTED       # (not every rTile exists in every mode)
+            continue
+        C = torch.full((M + 1, ldc), -7.0, device="cuda")
+        plan.run(A, B, C)
+        plan.check_status()
+        # (TF32 keeps 11 bits: 2^-10 for each operand of a product at most)
+        assert (C[:M, :N] - want).abs().max() <= 2e-3 * want.max()
+        C[:M, :N] = -7.0
+        assert bool((C == -7.0).all())
+        with pytest.raises(_lib.RollerError) as e:
+            plan.set_option(_lib.OPT_TMA_STORE, 1)
+        assert e.value.status in (_lib.ERR_INVALID, _lib.ERR_UNSUPPORTED)
+        plan.destroy()
+        ran += 1
+    assert ran >= 4
