@@ -111,9 +111,10 @@ struct FusedCfg {
   static_assert(SYM_RATIO >= -2 && SYM_RATIO <= 2, "triangle of tiles");
   // The exchange of partial sums in a splitting cluster goes through the ring's memory: each CTA
   // receives its share of the columns of 128 rows from every other part. (With more parts than
-  // slabs of 32 columns, some only give.)
+  // slabs of 32 columns, some only give.) Products whose epilogue reads matrices are not split: there is no
+  // size at which the estimate would have it.
   static constexpr int SLABS = (OP == kOpGate ? BN / 2 : BN) / 32;
-  static constexpr int MAX_SPLIT = WIDE ? 1 : CG == 2 ? (OP == kOpGate ? 2 : 4) : OP == kOpGate ? 4 : 8;
+  static constexpr int MAX_SPLIT = INPUTS > 0 ? 1 : CG == 2 ? (OP == kOpGate ? 2 : 4) : OP == kOpGate ? 4 : 8;
   static constexpr int exchange_bytes(int split) {
     return (split - 1) * (SLABS > split ? SLABS / split : 1) * (OP == kOpGate ? 2 : 1) * 16384;
   }
@@ -440,7 +441,7 @@ struct FusedWork {
             load_b(i, counts(i), c, kb + i);
           }
         }
-        if (!before_loads()) { r.ok = false; break; }
+        before_loads();
         if (issues)
           for (int i = 0; i < early; ++i) load_a(i, counts(i), c, kb + i);
         __syncwarp();
@@ -559,7 +560,7 @@ struct FusedWork {
       __syncwarp();
     };
 
-    if (!before_loads()) r.ok = false;
+    before_loads();
     for (int t = first(); r.ok && t < tiles; t = next(t)) {
       const FusedTile c = tile(t);
       const int row0 = (c.mb * CG + static_cast<int>(me.cta_rank)) * Cfg::BM + me.quarter * 32;
@@ -710,14 +711,12 @@ struct FusedWork {
       return b;
     };
     // 32 columns of this warp's 32 rows, as 16-bit values, into a box ...
-    auto put = [&](uint32_t box, const float (&v)[32], bool as_bf16) {
+    auto put = [&](uint32_t box, const float (&v)[32]) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] = (as_bf16 && DT != 1) ? fused_pack<1>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1])
-                                      : fused_pack<DT>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
+        for (int i = 0; i < 4; ++i) w[i] = fused_pack<DT>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
         // 64-byte swizzle: 16-byte chunks of a 64-byte row, exchanged by bits 1..2 of the row
         const int chunk = j ^ ((me.lane >> 1) & 3);
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + me.lane * 64 + chunk * 16),
@@ -726,9 +725,9 @@ struct FusedWork {
       }
     };
     // ... and from there to columns col.. of output `o`.
-    auto emit = [&](int o, const FusedTile& c, int row0, int col, const float (&v)[32], bool as_bf16) {
+    auto emit = [&](int o, const FusedTile& c, int row0, int col, const float (&v)[32]) {
       const uint32_t box = free_box();
-      put(box, v, as_bf16);
+      put(box, v);
       const int oz = OP == kOpDw ? 0 : c.z;
       if (((col + 32 <= cols(c) ? p.out_tma : p.out_whole) >> o) & 1) {
         fence_proxy_async_smem();
@@ -811,8 +810,8 @@ struct FusedWork {
             sums(tc, v);
             sums(tc + BN / 2, w);
             if (p.flags & kFusedSave) {
-              emit(1, c, row0, col, v, false);
-              emit(2, c, row0, col, w, false);
+              emit(1, c, row0, col, v);
+              emit(2, c, row0, col, w);
             }
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
@@ -820,10 +819,10 @@ struct FusedWork {
               activation<ACT>(v[j], y, slope);
               v[j] = y * w[j];
             }
-            emit(0, c, row0, col, v, false);
+            emit(0, c, row0, col, v);
           } else if constexpr (OP == kOpDown || OP == kOpDx || OP == kOpDw) {
             sums(tc, v);
-            emit(OP == kOpDw ? c.z : 0, c, row0, col, v, false);
+            emit(OP == kOpDw ? c.z : 0, c, row0, col, v);
           } else if constexpr (Cfg::SYM) {
             if constexpr (OP == kOpPoly) {
               sums(tc, v);
@@ -843,7 +842,7 @@ struct FusedWork {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] *= p.inv_scale;
             }
-            emit(0, c, row0, col, v, false);
+            emit(0, c, row0, col, v);
             if (col < row0) emit_mirror(c, row0, col, v);
           }
         }
@@ -859,8 +858,8 @@ struct FusedWork {
 
     constexpr int kSlabs = Cfg::OUT_COLS / 32;     // slabs of one warp of a whole tile
 
-    if (me.split == 1) {
-      if (!before_loads()) r.ok = false;
+    if (Cfg::MAX_SPLIT == 1 || me.split == 1) {
+      before_loads();
       for (int t = first(); r.ok && t < tiles; t = next(t)) {
         const FusedTile c = tile(t);
         if constexpr (Cfg::INPUTS > 0) {     // they do not depend on the product
@@ -894,10 +893,6 @@ struct FusedWork {
       const bool receives = static_cast<int>(me.part) % apart == 0 && me.half < share;
       if (me.epi) {
         before_loads();
-        if constexpr (Cfg::INPUTS > 0) {
-          const int col = c.nb * BN + (my_slab + me.half) * 32;
-          if (receives && wanted(c, row0, col)) fetch(c, row0, col);
-        }
         r.ok = __all_sync(0xffffffffu, mbar_wait(me.tmem_full_bar(0), 0u, me.wc, kDevTimeoutTmemFull));
       }
       __syncwarp();
@@ -980,13 +975,11 @@ fused_gemm_kernel(const __grid_constant__ FusedParams p) {
   FusedRing r;
   auto previous = [&]() {
     if (!p.late_wait) grid_dependency_wait();
-    return true;
   };
   if (x.warp == 0) {
     work.produce(r, elect_one(), [&]() {
       previous();
       grid_launch_dependents();
-      return true;
     });
     fused_end_producer<Cfg>(x, r);
   } else if (x.warp == 1 && x.is_leader) {
