@@ -80,3 +80,47 @@ def test_updates(batch, rows, cols):
     out.fill_(776.0)
     assert bool((buf == 776.0).all())
     plan.destroy()
+
+
+@pytest.mark.parametrize("stride", [2 ** 31 + 8, 2 ** 31 + 3])
+def test_row_strides_beyond_32_bits(stride):
+    """Every operand and output of the block, and the matrices of an update, with rows 4 GB apart, at once
+    in one buffer; on 16 bytes and not."""
+    tokens, d, f, dtype = 3, 3, 2, torch.bfloat16
+    s = block.make(tokens, d, f, dtype, seed=75)
+    plan = GatedFfnPlan(tokens, d, f, training=True)
+    y, g, u = block.run_forward(s, "silu", dtype, plan=plan)
+    want = dict(y=y, g=g, u=u, **{k: torch.empty_like(s[v]) for k, v in (("dx", "x"), ("dwg", "wg"), ("dwu", "wu"), ("dwd", "wd"))})
+    plan.backward(s["x"], s["wg"], s["wu"], s["wd"], g, u, s["dy"], *(want[k] for k in ("dx", "dwg", "dwu", "dwd")))
+    buf = torch.empty(2 * stride + 2048, dtype=dtype, device="cuda")
+    v = {}
+    for i, (k, t) in enumerate({**s, **want}.items()):
+        for r in range(t.shape[0]):
+            buf[r * stride + 64 * i:r * stride + 64 * (i + 1)] = 776.0
+        v[k] = buf[64 * i + 8:].as_strided(t.shape, (stride, 1))
+    for k in s:
+        v[k].copy_(s[k])
+    plan.forward(v["x"], v["wg"], v["wu"], v["wd"], v["y"], v["g"], v["u"])
+    plan.backward(v["x"], v["wg"], v["wu"], v["wd"], v["g"], v["u"], v["dy"], v["dx"], v["dwg"], v["dwu"], v["dwd"])
+    plan.check_status()
+    plan.destroy()
+    for i, (k, t) in enumerate({**s, **want}.items()):
+        assert torch.equal(v[k], t), k
+        for r in range(t.shape[0]):
+            around = buf[r * stride + 64 * i:r * stride + 64 * (i + 1)].clone()
+            around[8:8 + t.shape[1]] = 776.0
+            assert bool((around == 776.0).all()), k
+
+    # updates: matrices far apart, and rows far apart with the matrices interleaved
+    m = torch.randn(2, 3, 5, device="cuda").to(dtype)
+    plan = OrthogonalPlan(3, 5, batch=2)
+    out = torch.empty_like(m)
+    plan.run(m, out)
+    for strides in ((stride, 16, 1), (16, stride, 1), (13, stride, 1)):
+        a, b = buf.as_strided((2, 3, 5), strides), buf[512:].as_strided((2, 3, 5), strides)
+        a.copy_(m)
+        b.zero_()
+        plan.run(a, b)
+        assert torch.equal(b, out), strides
+    plan.check_status()
+    plan.destroy()
