@@ -143,6 +143,16 @@ namespace rb200 {
 
 int report_cuda_error(cudaError_t e, const char* what) { return cuda_fail(e, what); }
 
+cudaError_t zero_now(void* words, size_t bytes) {
+  cudaStream_t st = nullptr;
+  cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+  if (e != cudaSuccess) return e;
+  e = cudaMemsetAsync(words, 0, bytes, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  const cudaError_t destroyed = cudaStreamDestroy(st);
+  return e == cudaSuccess ? destroyed : e;
+}
+
 int encode_batch16(CUtensorMap* tm, const void* base, long long cols, long long rows, long long z,
                    long long ld, long long z_stride, int box_cols, int box_rows,
                    CUtensorMapSwizzle swz, bool bf16) {
@@ -410,7 +420,7 @@ int roller_b200_gemm_create(const roller_ktile* tile, int M, int N, int K, int l
   cudaError_t e = layout == 3 ? cudaSuccess : bind_variant(p, kv);
   p->tma_store = p->kv->staging_bytes > 0 && c_fits_tma;
   if (e == cudaSuccess) e = cudaMalloc(&p->status, 2 * sizeof(uint32_t));
-  if (e == cudaSuccess) e = cudaMemset(p->status, 0, 2 * sizeof(uint32_t));
+  if (e == cudaSuccess) e = rb200::zero_now(p->status, 2 * sizeof(uint32_t));
   if (e == cudaSuccess && p->stage_a) {
     p->ws_lda = round_up_ld(K, elem);
     e = cudaMalloc(&p->ws_a, static_cast<size_t>(elem) * p->ws_lda * M);
@@ -726,8 +736,8 @@ int roller_b200_last_status(roller_plan* p, uint32_t* device_status) {
   if (h != 0) {
     // Read and clear: the failed launch has been reported, later launches start clean. The
     // stream-K flags of a launch that gave up may be left raised, so they are reset as well.
-    RB_CUDA(cudaMemset(p->status, 0, 2 * sizeof(uint32_t)));   // (with the arrival counter)
-    if (p->sk_flags) RB_CUDA(cudaMemset(p->sk_flags, 0, sizeof(uint32_t) * p->sk_slots * 2));
+    RB_CUDA(rb200::zero_now(p->status, 2 * sizeof(uint32_t)));   // (with the arrival counter)
+    if (p->sk_flags) RB_CUDA(rb200::zero_now(p->sk_flags, sizeof(uint32_t) * p->sk_slots * 2));
   }
   return h == 0 ? ROLLER_OK : ROLLER_ERR_TIMEOUT;
 }
@@ -993,7 +1003,7 @@ static int plan_configure(roller_plan* p) {
     const int slots = p->max_workers * kv->cta_group * 4;
     cudaError_t e = cudaMalloc(&p->sk_ws, slot_bytes * slots);
     if (e == cudaSuccess) e = cudaMalloc(&p->sk_flags, sizeof(uint32_t) * slots * 2);
-    if (e == cudaSuccess) e = cudaMemset(p->sk_flags, 0, sizeof(uint32_t) * slots * 2);
+    if (e == cudaSuccess) e = rb200::zero_now(p->sk_flags, sizeof(uint32_t) * slots * 2);
     if (e != cudaSuccess) {
       cudaGetLastError();
       return ROLLER_ERR_NOMEM;

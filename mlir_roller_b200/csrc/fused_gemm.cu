@@ -264,19 +264,6 @@ static cudaError_t device_facts(int dev, FusedDevice* d) {
   return e;
 }
 
-// Zeroes the status word, and returns when that is done: the first launch may come at once, on a stream that
-// does not wait for the default one, and a word left over from an earlier owner of the memory would end its waits.
-// (A stream of its own, because the default one may be busy for long.)
-static cudaError_t clear_status(uint32_t* status) {
-  cudaStream_t st = nullptr;
-  cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
-  if (e != cudaSuccess) return e;
-  e = cudaMemsetAsync(status, 0, sizeof(uint32_t), st);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  const cudaError_t destroyed = cudaStreamDestroy(st);
-  return e == cudaSuccess ? destroyed : e;
-}
-
 int fused_context_create(FusedContext* c) {
   memset(c, 0, sizeof(*c));
   FUSED_CUDA(cudaGetDevice(&c->device));
@@ -285,7 +272,7 @@ int fused_context_create(FusedContext* c) {
   if (major != 10) return ROLLER_ERR_DEVICE;
   cudaError_t e = device_facts(c->device, &c->dev);
   if (e == cudaSuccess) e = cudaMalloc(&c->status, sizeof(uint32_t));
-  if (e == cudaSuccess) e = clear_status(c->status);
+  if (e == cudaSuccess) e = zero_now(c->status, sizeof(uint32_t));
   if (e == cudaSuccess) return ROLLER_OK;
   const int rc = e == cudaErrorMemoryAllocation ? ROLLER_ERR_NOMEM : report_cuda_error(e, "plan setup");
   cudaGetLastError();
@@ -306,7 +293,7 @@ int fused_context_status(FusedContext* c, uint32_t* device_status) {
   FUSED_CUDA(cudaMemcpy(&h, c->status, sizeof(h), cudaMemcpyDeviceToHost));
   if (device_status) *device_status = h;
   if (h == 0) return ROLLER_OK;
-  FUSED_CUDA(clear_status(c->status));
+  FUSED_CUDA(zero_now(c->status, sizeof(uint32_t)));
   return ROLLER_ERR_TIMEOUT;
 }
 

@@ -509,3 +509,34 @@ def test_aligned_rows_of_any_length_end_where_they_should(mode, N):
         plan.destroy()
         ran += 1
     assert ran >= 4
+
+
+@pytest.mark.parametrize("shape", [(256, 256, 8192), (512, 768, 1024)])
+def test_a_new_plan_is_ready_for_any_stream(shape):
+    """A plan whose tiles are cut along K, made while the default stream is busy, on memory that was used
+    before, and run at once on a stream that does not wait for that one."""
+    import ctypes
+    M, N, K = shape
+    A, B = g.make_inputs(M, N, K, "uniform", seed=3)
+    want = run_plan(A, B, (128, 128, 1), 3, [(_lib.OPT_PROGRESSIVE_ROUNDS, 2)])[0]
+    dA, dB = torch.from_numpy(A).cuda(), torch.from_numpy(B).cuda()
+    dC = torch.zeros(M, N, device="cuda")
+    rt = ctypes.CDLL("libcudart.so.12")
+    pieces = []
+    for size in [4, 8, 64, 512, 2048, 4736, 8192] * 8:
+        pieces.append(ctypes.c_void_p())
+        assert rt.cudaMalloc(ctypes.byref(pieces[-1]), ctypes.c_size_t(size)) == 0
+        assert rt.cudaMemset(pieces[-1], 255, ctypes.c_size_t(size)) == 0
+    torch.cuda.synchronize()
+    for p in pieces:
+        assert rt.cudaFree(p) == 0
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)       # about a tenth of a second
+    plan = _lib.GemmPlan(_lib.find_tile(128, 128, 1), M, N, K, mode=3)
+    plan.set_option(_lib.OPT_PROGRESSIVE_ROUNDS, 2)
+    plan.run(dA, dB, dC, stream=side)
+    side.synchronize()
+    assert np.array_equal(dC.cpu().numpy(), want)
+    plan.check_status()
+    plan.destroy()
