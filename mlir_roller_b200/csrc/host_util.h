@@ -11,8 +11,8 @@ int report_cuda_error(cudaError_t e, const char* what);
 
 // Zeroes device memory that a plan has just got, and returns when that is done: the first launch may come at
 // once, on a stream that does not wait for the default one, and a word left over from an earlier owner of the
-// memory would end its waits or pass for a flag. (On a stream of its own, because the default one may be busy
-// for long.)
+// memory would end its waits or pass for a flag. (On a stream of its own where the default one is busy, which may
+// be for long.)
 cudaError_t zero_now(void* words, size_t bytes);
 
 // Tensor map of a batch of `z` row-major 16-bit matrices. base, ld and z_stride have to be
