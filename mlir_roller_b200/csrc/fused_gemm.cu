@@ -17,7 +17,7 @@ const FusedVariant* table(int i, int* n) {
 }
 
 // Measured on B200 over widths 512 .. 8192, 1 .. 8192 rows (every kernel and split timed beside the
-// others); the choice by them comes within 1 % of the fastest on average.
+// others).
 struct TileCost {
   int cta_group, block_n;
   double alone_us, busy_us;   // one k-block of one tile, on a few SMs and on all of them
@@ -46,7 +46,8 @@ double epilogue_weight(int op) {
 // that starts between two words gives each word from two neighbouring ones, the second of which the
 // next lane has. (A word that holds an element of the row may be read whole. Ordinary loads, not those of
 // constant data: the kernel before may still be writing an operand when this one starts.)
-// A 2048 x 5461 weight costs a forward call 5 us (45 MB, overlapped with the first product's end).
+// A 2048 x 5461 weight costs a forward call of 777 tokens 8 us of 72 (45 MB, overlapped with the first
+// product's end).
 // jobs.late: as FusedParams::late_wait, the copies need nothing from the previous kernel.
 __global__ void __launch_bounds__(256) align_rows_kernel(const __grid_constant__ AlignJobs jobs) {
   if (!jobs.late) grid_dependency_wait();
@@ -163,7 +164,7 @@ static cudaError_t bind_device(FusedDevice* d) {
 // x (their cost) + the fill and drain; the smallest estimate wins.
 //   * whole tiles: the busiest CTA (or pair) gets ceil(tiles / workers) of them. (Dealing the tiles
 //     that do not fill a last wave out along k was built and measured: writing and reading back the
-//     fp32 sums of 256 x 256 tiles costs 15-25 us, more than an even share of k saves up to
+//     fp32 sums of 256 x 256 tiles costs 13-26 us, more than an even share of k saves up to
 //     K = 8192.)
 //   * a cluster per tile: 1 / split of a tile's k-blocks per wave of clusters, and the exchange.
 // No launch is shorter than its operands' way from memory: with few rows this decides, and the

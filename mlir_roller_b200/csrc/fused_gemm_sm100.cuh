@@ -45,19 +45,20 @@
 // late_wait does. It does not hold behind one with late_wait, behind late copies (AlignJobs::late), or
 // behind a launch that is not of this call; there the two flags are taken back (LaunchOrder).
 //
-// Measured on B200 (times by events over whole calls, operands beyond L2; shares from counters on
-// 4096 tokens x 2048 x 4096, one launch at a time):
+// Measured on B200 (whole calls by events, operands beyond L2; shares of the cycles in which an SM has
+// work from counters on 4096 tokens x 2048 x 4096, one launch at a time):
 //   kOpGate, kOpDown   8192 x 4096 x 8192, bf16: 1.19 ms = 1.39 PFLOP/s, what the power limit leaves the
-//                      library's GEMM too. Tensor pipe busy 85 and 81 % of the active cycles, 79 and
-//                      65 % of all (128 tiles of kOpDown on 74 pairs run as two waves).
-//                      1 x 2048 x 8192: 25 us for 101 MB, 3-5 us of them each kernel's start and end;
-//                      1 x 8192 x 32768: 6.4 TB/s.
-//   kOpDact, kOpDx, kOpDw   8192 x 4096 x 8192, bf16: 2.60 ms together = 1.27 PFLOP/s. Tensor pipe 53,
-//                      90, 92 %: kOpDact moves five matrices beside its product (174 MB of DRAM traffic
-//                      there) and is bound by them. 200 x 1024 x 2816: 28.5 us, the latency of three
-//                      launches of which two overlap.
-//   kOpGram*, kOpPoly, kOpUpdate*   8192 x 4096, five steps: 2.18 ms = 1.10 PFLOP/s, triangles counted
-//                      as such; 512 x 512: 5.6 to 6.7 us a product, nearly all of it the way from one
+//                      library's GEMM too. Tensor pipe busy 86 and 81 %, of all cycles 79 and 64 %
+//                      (128 tiles of kOpDown on 74 pairs run as two waves).
+//                      1 x 2048 x 8192: 25 us for 101 MB, of which the kernels' starts and ends and a second
+//                      stream that begins when the first one has ended; 1 x 8192 x 32768: 6.4 TB/s.
+//   kOpDact, kOpDx, kOpDw   8192 x 4096 x 8192, bf16: 2.58 ms together = 1.28 PFLOP/s. Tensor pipe 52,
+//                      90, 92 %: with 2048 to reduce over, a tile of kOpDact is 19 us of epilogue beside 11 us of
+//                      MMAs, and neither the memory (2.3 TB/s) nor the tensor pipe is busy then: inputs, arithmetic
+//                      and results of 64 columns follow one another. 200 x 1024 x 2816: 30 us, three launches of
+//                      which two overlap, the first one on 44 of 148 SMs.
+//   kOpGram*, kOpPoly, kOpUpdate*   8192 x 4096, five steps: 2.19 ms = 1.10 PFLOP/s, triangles counted
+//                      as such; 512 x 512: 95 us, 5 to 7 us a product, nearly all of it the way from one
 //                      launch's results to the next one's loads.
 #pragma once
 
@@ -84,7 +85,7 @@ struct FusedCfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   // Columns of the result one epilogue warp owns. They leave in boxes of 32 rows x 32 columns, or
   // 64 where an epilogue reads two matrices and writes two or three: half as many copies, worth
-  // 3-6 % of a small orthogonalisation (512 x 512: 99.8 -> 96.9 us) and under 2 % of kOpDact. These
+  // 3-6 % of a small orthogonalisation and under 2 % of kOpDact. These
   // boxes serve twice: a matrix read is replaced, in place, by one written.
   static constexpr int OUT_COLS = (OP == kOpGate ? BN / 4 : BN / 2);
   static constexpr int INPUTS = (OP == kOpDact || UPDATE) ? 2 : OP == kOpPoly ? 1 : 0;
