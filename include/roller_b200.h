@@ -373,7 +373,8 @@ int roller_b200_ffn_create(int max_tokens, int d_model, int d_ff, int mode, int 
  * be captured in a CUDA graph, with one exception: the first call that passes an unaligned operand
  * for which the plan has no padded copy yet allocates one, which a capturing stream refuses
  * (ROLLER_ERR_UNSUPPORTED; make one such call before the capture). Launches of one plan, and
- * replays of graphs captured from it, share its workspaces and have to be ordered on the device.
+ * replays of graphs captured from it, share its workspaces and have to be ordered on the device; the plan
+ * has to outlive the graphs.
  * There is no counterpart in the reference (src/roller.py:47-68 emits a plain matmul). */
 int roller_b200_ffn_forward(roller_ffn_plan* plan, const roller_ffn_io* io, void* stream);
 
@@ -420,8 +421,8 @@ int roller_b200_ortho_create(int batch, int rows, int cols, int in_type, int ste
 /* Enqueues the iteration for `batch` matrices at g (row stride ld_g, matrix stride zs_g, in
  * elements) into out (bf16). Matrices may follow one another or be interleaved row by row; g is
  * not changed, out must not share memory with it. Only enqueues; may be captured. Launches of one
- * plan, and replays of graphs captured from it, have to be ordered on the device. There is no
- * counterpart in the reference (src/roller.py:47-68). */
+ * plan, and replays of graphs captured from it, have to be ordered on the device, and the plan has to outlive
+ * the graphs. There is no counterpart in the reference (src/roller.py:47-68). */
 int roller_b200_ortho_run(roller_ortho_plan* plan, const void* g, long long ld_g, long long zs_g,
                           void* out, long long ld_out, long long zs_out, void* stream);
 

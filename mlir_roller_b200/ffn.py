@@ -6,7 +6,8 @@ x and y are [tokens, d_model], Wg and Wu [d_ff, d_model], Wd [d_model, d_ff] (a 
 weight: outputs x inputs), all bf16 or all fp16, row-major with any row stride. As with the GEMM
 plans (`_lib.GemmPlan`), a plan owns the workspaces, the caller owns operands and outputs, calls only
 enqueue on a stream, and calls of one plan have to be ordered on the device: use one plan per
-stream, and do not replay two graphs captured from one plan at the same time. Sums are kept in
+stream, do not replay two graphs captured from one plan at the same time, and keep a plan for as
+long as graphs captured from it are replayed (they use its workspaces). Sums are kept in
 fp32; h and the gradients of g and u are operands of a product and hold the operand type (in fp16
 with its range: over 65504 they become infinite). There is no CPU fallback.
 

@@ -12,7 +12,7 @@ is). Where |g| is under about 1e-5 eps the result, itself close to zero, keeps o
 accuracy.
 
 A plan owns the workspaces; calls only enqueue on a stream, and calls of one plan have to be ordered
-on the device. There is no CPU fallback. The reference has no counterpart: it multiplies two matrices
+on the device. Graphs captured from a plan need it for as long as they are replayed. There is no CPU fallback. The reference has no counterpart: it multiplies two matrices
 (src/roller.py:47-68).
 """
 from __future__ import annotations
